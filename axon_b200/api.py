@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from .config.base import ModelConfig, architecture_of, load_config
-from .engine.build import build_engine, parse_dtype
+from .engine.build import build_engine, parse_dtype, parse_kv
 from .engine.step import Engine, StepEntry, StepError
 from .kernels import lib, ops
 from .sampling.sampler import RowSampler, SampleCfg, pick_tokens
@@ -77,6 +77,7 @@ class BackendOptions:
     _parallel: int = 16
     _kv_tokens: Optional[int] = None
     _step_tokens: int = 8192
+    _kv: str = "auto"
 
     def device(self, device: str) -> "BackendOptions":
         """Where the model runs: a CUDA device (there is no CPU path)."""
@@ -92,13 +93,11 @@ class BackendOptions:
         return replace(self, _dtype=dtype)
 
     def kv(self, kv: str) -> "BackendOptions":
-        """The cache type.  The cache always has the model's dtype here (no quantized
-        caches); ``bf16``/``f32``/``auto`` are accepted when they agree with it."""
-        if kv not in ("auto", "bf16", "bfloat16", "f32", "float32"):
-            raise ValueError(f"KV type '{kv}' is not supported (bf16 with a bfloat16 model, f32 with a float32 one)")
-        if kv != "auto" and parse_dtype(kv) != parse_dtype(self._dtype):
-            raise ValueError(f"the cache has the model's dtype ({self._dtype}); '{kv}' differs")
-        return self
+        """The cache type.  ``auto``, ``bf16`` and ``f32``: the model's dtype (the latter two are accepted
+        when they agree with it).  ``q4``: keys and values are quantised to 4 bits as they are written
+        (4.5 bits a value with their steps, 3.6 times as many positions as bf16 in the same memory)."""
+        parse_kv(kv, self._dtype)
+        return replace(self, _kv="q4" if kv == "q4" else "auto")
 
     def page_size(self, n: int) -> "BackendOptions":
         return replace(self, _page_size=int(n))
@@ -177,7 +176,7 @@ class Backend:
             path = model.path if isinstance(model, Model) else model
             engine = build_engine(path, dtype=o._dtype, device=o._device, page_size=o._page_size,
                                   max_tokens=o._kv_tokens, max_slots=o._parallel,
-                                  max_positions=o._max_ctx, max_step_tokens=o._step_tokens)
+                                  max_positions=o._max_ctx, max_step_tokens=o._step_tokens, kv=o._kv)
         self.engine = engine
         self.config = engine.config
 

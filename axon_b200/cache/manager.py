@@ -22,7 +22,7 @@ import numpy as np
 import torch
 
 from ..kernels import lib
-from ..kernels.ops import KvView
+from ..kernels.ops import KvView, kv_read
 from ..parts.spec import KvNeed, StateNeed
 
 _STATE_DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "int32": torch.int32}
@@ -93,7 +93,7 @@ class PagedCache:
                     continue
                 self._entry_parts.setdefault(i, []).append(name)
                 if isinstance(need, KvNeed):
-                    key = (need.kv_heads, need.head_dim, need.window, need.value_dim, need.planes)
+                    key = (need.kv_heads, need.head_dim, need.window, need.value_dim, need.planes, need.bits)
                     if key not in by_key:
                         by_key[key] = len(self.groups)
                         self.groups.append(_Group(need, []))
@@ -118,11 +118,13 @@ class PagedCache:
         if allocate:
             for gi, g in enumerate(self.groups):
                 n = g.need
-                if n.planes == 2 and n.value_dim == n.head_dim:
+                if n.bits:
+                    shape = (n_pages + 1, len(g.members), n.page_bytes(page_size, 0))
+                elif n.planes == 2 and n.value_dim == n.head_dim:
                     shape = (n_pages + 1, len(g.members), 2, n.kv_heads, page_size, n.head_dim)
                 else:
                     shape = (n_pages + 1, len(g.members), page_size * n.elements_per_token)
-                g.pool = torch.zeros(shape, dtype=dtype, device=self.device)
+                g.pool = torch.zeros(shape, dtype=torch.uint8 if n.bits else dtype, device=self.device)
                 stride = self.manager.table_stride(gi)
                 g.table = torch.full((max_slots, stride), n_pages, dtype=torch.int32, device=self.device)
                 g.staging = [torch.empty((max_slots, stride), dtype=torch.int32).pin_memory() for _ in range(_TABLE_STAGES)]
@@ -198,7 +200,8 @@ class PagedCache:
             gi, plane = self._member_group[key]
             g = self.groups[gi]
             v = KvView(g.pool, g.table, plane, self.page_size, g.need.kv_heads, g.need.head_dim,
-                       g.need.window or 0, v_dim=g.need.value_dim, planes=g.need.planes, fault=self._fault)
+                       g.need.window or 0, v_dim=g.need.value_dim, planes=g.need.planes, fault=self._fault,
+                       bits=g.need.bits)
             self._views[key] = v
         return v
 
@@ -219,15 +222,43 @@ class PagedCache:
 
     def bytes_per_token(self) -> int:
         """Cache bytes one position takes over all groups."""
-        return bytes_per_token([g.need for g in self.groups for _ in g.members], self.dtype)
+        return bytes_per_token([g.need for g in self.groups for _ in g.members], self.dtype, self.page_size)
+
+    def read(self, slot: int, entry: int, part: Optional[str] = None, first: int = 0,
+             count: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What a request holds for one part of schedule entry ``entry``: its keys ``[count][kv_heads][head_dim]``
+        and values ``[count][kv_heads][v_dim]`` at positions ``first ..`` (by default all it holds), in the
+        model's dtype, read back from the pages whatever form they keep rows in.  Positions that a
+        window has given back are refused."""
+        v = self.view(entry, part)
+        if not isinstance(v, KvView):
+            raise ValueError(f"schedule entry {entry} has no one part that keeps keys and values; name it")
+        if not self.manager.is_open(slot):
+            raise ValueError(f"slot {slot} is not open")
+        n = self.length(slot)
+        count = n - first if count is None else count
+        kept = max(0, n - v.window) if v.window else 0
+        if first < kept or count < 0 or first + count > n:
+            raise ValueError(f"slot {slot} holds positions {kept}..{n - 1}, not {first}..{first + count - 1}")
+        self.sync_tables()
+        if v.bits:
+            keys = torch.empty((count, v.kv_heads, v.head_dim), dtype=self.dtype, device=self.device)
+            values = torch.empty((count, v.kv_heads, v.v_dim), dtype=self.dtype, device=self.device)
+            spans = torch.tensor([[slot], [first], [count], [0]], dtype=torch.int32, device=self.device)
+            kv_read(v, spans, keys, values)
+            return keys, values
+        at = torch.arange(first, first + count, device=self.device)
+        pages = v.block_table[slot, at // self.page_size].long()
+        return v.keys()[pages, :, at % self.page_size], v.values()[pages, :, at % self.page_size]
 
 
-def bytes_per_token(needs: Sequence[Union[Need, Mapping[str, Need]]], dtype: torch.dtype) -> int:
-    """Cache bytes one position takes for these needs (state slabs do not grow with positions)."""
+def bytes_per_token(needs: Sequence[Union[Need, Mapping[str, Need]]], dtype: torch.dtype, page_size: int = 16) -> int:
+    """Cache bytes one position takes for these needs (state slabs do not grow with positions).  Parts of
+    quantised pages are padded to 16 bytes, which adds a little at page sizes that are no multiple of 16."""
     item = torch.empty((), dtype=dtype).element_size()
     total = 0
     for n in needs:
         for need in (n.values() if isinstance(n, Mapping) else (n,)):
             if isinstance(need, KvNeed):
-                total += need.elements_per_token * item
+                total += -(-need.page_bytes(page_size, item) // page_size)
     return total

@@ -38,7 +38,7 @@ flags:
   -k K        logits: how many candidates to print (default 10)
   --device D  cuda or cuda:N (there is no CPU path)
   --ctx N     gen: room for N positions (default: prompt + N + 1)
-  --kv T      cache type: auto, bf16 or f32 (it follows --dtype)
+  --kv T      cache type: auto, bf16 or f32 (it follows --dtype), or q4 (4 bits a value)
   --dtype T   bfloat16 (default) or float32 (every kernel in true 32-bit)
   --verbose   gen: print the configuration and the kernels' library
 

@@ -7,6 +7,14 @@
 // (equal for ordinary attention).  With `planes` == 1 there is one plane per entry: a
 // mixer that keeps a single latent row per position; kernels then read values from the
 // key plane (v_offset 0, v_dim == head_dim).
+//
+// With `bits` == 4 the pool is bytes, and so are the units of page_stride and entry_offset;
+// v_offset is not used.  An entry is one record per kv head:
+//   [key codes][key steps] and, with two planes, [value codes][value steps],
+// each part padded to 16 bytes: codes are [page_size][width / 2] bytes (two values a byte, the even
+// one in the low nibble), steps [page_size][width / 16] bytes (one per 16 consecutive values).  A value is
+// (nibble - 8) * step, a step byte b standing for the half-precision number with the bits b << 7
+// (five exponent and three mantissa bits; kv_q4.cuh says how they are chosen).
 #pragma once
 
 #include <stdint.h>
@@ -27,6 +35,6 @@ struct AxonKvLayout {
     // larger or negative one is not followed: the kernel reads or writes the sink page
     // instead, sets fault[0] = 1 and fault[1] = the entry.  Null switches the check off.
     int32_t n_pages;
-    int32_t reserved;
+    int32_t bits;                // 0: rows of the pool's element type; 4: quantised rows (below)
     uint32_t* fault;
 };

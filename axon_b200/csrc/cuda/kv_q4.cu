@@ -1,0 +1,451 @@
+// The 4-bit cache's plain operators: rotating and quantising rows as they are written, reading
+// positions back, attention for any sizes, and the fold of partial results of key shares.  The format is in
+// kv_layout.h, the arithmetic in kv_q4.cuh.
+#include "kv_q4.cuh"
+
+namespace axon {
+
+__device__ __forceinline__ float4 q4_load4(const float* row, const SplitFold& fold, int t, int n) {
+    return fold.partial ? fold.at4(t, n) : *reinterpret_cast<const float4*>(row + n);
+}
+
+// Rotation and quantised cache write: a warp per (token, head) row, four consecutive channels a
+// lane, so that a group of 16 is four neighbouring lanes (two shuffles for its maximum) and a lane's codes are two
+// whole bytes.  Rotated values are products and sums rounded to 32 bits one by one (no
+// fused multiply-add), so a key's codes do not depend on how a compiler contracts them.  VEC: rows
+// and the rotation table are read as float4s (rot % 8 == 0, 16-byte aligned operands).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+rope_kv_write_q4_kernel(const float* __restrict__ qkv, const float2* __restrict__ table, const int32_t* __restrict__ positions,
+                        const int32_t* __restrict__ token_slot, T* __restrict__ q_out, uint8_t* __restrict__ pool, PagedQ4 kv,
+                        int heads, int rot, int adjacent, int write_kv, SplitFold fold) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t = blockIdx.x, lane = threadIdx.x & 31;
+    const int h = blockIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int rows = heads + kv.planes * kv.kv_heads;
+    if (h >= rows || (h >= heads && !write_kv)) return;
+    const bool is_v = h >= heads + kv.kv_heads;
+    const int q_dim = heads * kv.hd, k_dim = kv.kv_heads * kv.hd;
+    const int width = is_v ? kv.vd : kv.hd;
+    const int col = is_v ? q_dim + k_dim + (h - heads - kv.kv_heads) * kv.vd : h * kv.hd;
+    const float* row = qkv + (long long)t * (q_dim + k_dim + (kv.planes == 2 ? kv.kv_heads * kv.vd : 0));
+    const int rhalf = rot / 2;
+    const float2* cs = table + (long long)t * rhalf;
+    uint8_t *codes = nullptr, *steps = nullptr;
+    if (h >= heads) {
+        const int pos = positions[t], lp = pos / kv.page_size, in_page = pos - lp * kv.page_size;
+        uint8_t* rec = pool + kv.record_at(token_slot[t], lp, is_v ? h - heads - kv.kv_heads : h - heads);
+        codes = rec + (is_v ? kv.v_codes : 0) + (long long)in_page * (width / 2);
+        steps = rec + (is_v ? kv.v_steps : kv.k_steps) + (long long)in_page * (width / Q4_GROUP);
+    }
+    for (int base = 0; base < width; base += 128) {
+        const int c0 = base + 4 * lane;
+        const bool mine = c0 < width;                          // whole groups of four lanes have or have not
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (mine) {
+            if (VEC) {
+                const float4 own = q4_load4(row, fold, t, col + c0);
+                x[0] = own.x; x[1] = own.y; x[2] = own.z; x[3] = own.w;
+                if (!is_v && table != nullptr && c0 < rot) {
+                    if (adjacent) {
+                        const float4 w = *reinterpret_cast<const float4*>(cs + c0 / 2);
+                        x[0] = __fsub_rn(__fmul_rn(own.x, w.x), __fmul_rn(own.y, w.y));
+                        x[1] = __fadd_rn(__fmul_rn(own.x, w.y), __fmul_rn(own.y, w.x));
+                        x[2] = __fsub_rn(__fmul_rn(own.z, w.z), __fmul_rn(own.w, w.w));
+                        x[3] = __fadd_rn(__fmul_rn(own.z, w.w), __fmul_rn(own.w, w.z));
+                    } else {
+                        const bool first = c0 < rhalf;
+                        const int i0 = first ? c0 : c0 - rhalf;
+                        const float4 other = q4_load4(row, fold, t, col + (first ? c0 + rhalf : i0));
+                        const float4 w01 = *reinterpret_cast<const float4*>(cs + i0), w23 = *reinterpret_cast<const float4*>(cs + i0 + 2);
+                        const float o[4] = {other.x, other.y, other.z, other.w};
+                        const float c[4] = {w01.x, w01.z, w23.x, w23.z}, s[4] = {w01.y, w01.w, w23.y, w23.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            x[j] = first ? __fsub_rn(__fmul_rn(x[j], c[j]), __fmul_rn(o[j], s[j]))
+                                         : __fadd_rn(__fmul_rn(o[j], s[j]), __fmul_rn(x[j], c[j]));
+                    }
+                }
+            } else {
+                auto at = [&](int n) { return fold.partial ? fold.at(t, col + n) : row[col + n]; };
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int c = c0 + j;
+                    x[j] = at(c);
+                    if (!is_v && table != nullptr && c < rot) {
+                        const bool first = adjacent ? !(c & 1) : c < rhalf;
+                        const int i = adjacent ? c >> 1 : first ? c : c - rhalf;
+                        const float o = at(adjacent ? c ^ 1 : first ? c + rhalf : c - rhalf);
+                        const float2 w = cs[i];
+                        x[j] = first ? __fsub_rn(__fmul_rn(x[j], w.x), __fmul_rn(o, w.y))
+                                     : __fadd_rn(__fmul_rn(o, w.y), __fmul_rn(x[j], w.x));
+                    }
+                }
+            }
+        }
+        if (h < heads) {
+            if (mine) {
+                T* dst = q_out + (long long)t * q_dim + col + c0;
+                stf(dst, x[0]); stf(dst + 1, x[1]); stf(dst + 2, x[2]); stf(dst + 3, x[3]);
+            }
+            continue;
+        }
+        // magnitudes compare as integers, and what is not finite is larger than all that is
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int byte = q4_step_byte(top);
+        const float inv = q4_inverse(byte);
+        uint32_t two = 0x8888u;
+        if (byte != Q4_NAN) two = q4_code(x[0], inv) | q4_code(x[1], inv) << 4 | q4_code(x[2], inv) << 8 | q4_code(x[3], inv) << 12;
+        if (mine) {
+            *reinterpret_cast<uint16_t*>(codes + c0 / 2) = (uint16_t)two;
+            if ((lane & 3) == 0) steps[c0 / Q4_GROUP] = (uint8_t)byte;
+        }
+    }
+}
+
+// Positions back as rows of T.  A CTA owns up to 32 consecutive rows of the output: its first
+// threads find each row's span and page once, then all threads turn words of eight codes into
+// eight values, neighbouring threads along a row and then along positions, which is how both sides lie in
+// memory.  Output row r of plane p and kv head h starts at
+//   (r / block) * block_stride + (r % block) * row_stride + h * head_stride.
+struct Q4Out {
+    void *k, *v;
+    long long block_stride, row_stride, head_stride;
+    int block;
+};
+template <typename T>
+__device__ __forceinline__ void q4_store8(T* dst, uint32_t word, float s);
+template <>
+__device__ __forceinline__ void q4_store8<float>(float* dst, uint32_t word, float s) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = q4_digit(word, i) * s;
+    reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+template <>
+__device__ __forceinline__ void q4_store8<__nv_bfloat16>(__nv_bfloat16* dst, uint32_t word, float s) {
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __nv_bfloat162 b = __floats2bfloat162_rn(q4_digit(word, 2 * i) * s, q4_digit(word, 2 * i + 1) * s);
+        o[i] = *reinterpret_cast<uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+constexpr int Q4_READ_ROWS = 32, Q4_READ_THREADS = 256;
+template <typename T>
+__global__ void __launch_bounds__(Q4_READ_THREADS)
+kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* __restrict__ spans, int n_spans, int n_slots,
+                  long long n_rows, int rows_per_cta, Q4Out out) {
+    __shared__ long long rec[Q4_READ_ROWS];                    // the row's record of kv head 0, or -1: not written
+    __shared__ int at[Q4_READ_ROWS];                           // its place in the page
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long r0 = (long long)blockIdx.x * rows_per_cta;
+    if (threadIdx.x < rows_per_cta) {
+        const long long r = r0 + threadIdx.x;
+        long long where = -1;
+        int in_page = 0;
+        for (int s = 0; s < n_spans && r < n_rows; ++s) {
+            const long long i = r - spans[3 * n_spans + s];
+            if (i < 0 || i >= spans[2 * n_spans + s]) continue;
+            const int slot = spans[s];
+            const long long pos = spans[n_spans + s] + i, lp = pos / kv.page_size;
+            if (slot >= 0 && slot < n_slots && pos >= 0 && lp < kv.table_stride) {
+                where = kv.record_at(slot, (int)lp, 0);
+                in_page = (int)(pos - lp * kv.page_size);
+            }
+            break;
+        }
+        rec[threadIdx.x] = where;
+        at[threadIdx.x] = in_page;
+    }
+    __syncthreads();
+    const int kw = kv.hd / 8, vw = kv.vd / 8;                  // words of a row
+    const int k_items = out.k ? kv.kv_heads * rows_per_cta * kw : 0, v_items = out.v ? kv.kv_heads * rows_per_cta * vw : 0;
+    for (int i = threadIdx.x; i < k_items + v_items; i += Q4_READ_THREADS) {
+        const bool is_v = i >= k_items;
+        const int words = is_v ? vw : kw, j = is_v ? i - k_items : i;
+        const int w = j % words, r = j / words % rows_per_cta, h = j / words / rows_per_cta;
+        if (rec[r] < 0) continue;
+        const uint8_t* from = pool + rec[r] + (long long)h * kv.record;
+        const uint32_t word = *reinterpret_cast<const uint32_t*>(from + (is_v ? kv.v_codes : 0) + ((long long)at[r] * words + w) * 4);
+        const float s = q4_step(from[(is_v ? kv.v_steps : kv.k_steps) + (long long)at[r] * (words / 2) + w / 2]);
+        const long long row = r0 + r;
+        T* dst = (T*)(is_v ? out.v : out.k) + row / out.block * out.block_stride + row % out.block * out.row_stride + h * out.head_stride + w * 8;
+        q4_store8<T>(dst, word, s);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Causal attention for any sizes (and the 32-bit model): a CTA per (token, up to eight heads of
+// a kv head, share of the keys).  64 keys at a time are widened to float in shared memory, scored by FFMA
+// (a thread per key and four heads), folded with a running maximum and sum, then the same
+// tile holds the values (a thread per channel and eight heads).  Scores are in log2 units.
+constexpr int Q4P_KEYS = 64, Q4P_HEADS = 8, Q4P_THREADS = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(Q4P_THREADS)
+attention_q4_plain_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pool, const int32_t* __restrict__ positions,
+                          const int32_t* __restrict__ token_slot, T* __restrict__ out, PagedQ4 kv, int heads, float scale_log2,
+                          int window, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+    extern __shared__ float q4p_smem[];
+    const int hd = kv.hd, vd = kv.vd, group = heads / kv.kv_heads, blocks = (group + Q4P_HEADS - 1) / Q4P_HEADS;
+    const int t = blockIdx.x, kh = blockIdx.y / blocks, h0 = kh * group + blockIdx.y % blocks * Q4P_HEADS;
+    const int n_heads = min(Q4P_HEADS, (kh + 1) * group - h0);
+    const int pitch = max(hd, vd) + 1;                         // odd: a column of the tile falls into 32 banks
+    float* qs = q4p_smem;                                      // [8][hd]
+    float* tile = qs + Q4P_HEADS * hd;                         // [64][pitch]
+    float* sc = tile + Q4P_KEYS * pitch;                       // [64][8] scores, then weights
+    __shared__ float m_run[Q4P_HEADS], l_run[Q4P_HEADS], corr[Q4P_HEADS];
+    __shared__ long long rec[Q4P_KEYS];
+    __shared__ int at[Q4P_KEYS];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tid = threadIdx.x, pos = positions[t], slot = token_slot[t];
+    const int lo_all = (window > 0 && pos - window + 1 > 0) ? pos - window + 1 : 0;
+    const int tiles = (pos + 1 - lo_all + Q4P_KEYS - 1) / Q4P_KEYS, per = (tiles + gridDim.z - 1) / gridDim.z;
+    const int lo = lo_all + (int)blockIdx.z * per * Q4P_KEYS, hi = min(pos + 1, lo + per * Q4P_KEYS);
+    for (int i = tid; i < Q4P_HEADS * hd; i += Q4P_THREADS)
+        qs[i] = i / hd < n_heads ? ldf(q + ((long long)t * heads + h0) * hd + i) * scale_log2 : 0.f;
+    if (tid < Q4P_HEADS) { m_run[tid] = -INFINITY; l_run[tid] = 0.f; }
+    float acc[2][Q4P_HEADS];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < Q4P_HEADS; ++i) acc[c][i] = 0.f;
+    const int key = tid & 63, half = tid >> 6;
+
+    for (int p0 = lo; p0 < hi; p0 += Q4P_KEYS) {
+        const int cnt = min(Q4P_KEYS, hi - p0);
+        __syncthreads();                                       // the tile before has been used
+        if (tid < cnt) {
+            const int lp = (p0 + tid) / kv.page_size;
+            rec[tid] = kv.record_at(slot, lp, kh);
+            at[tid] = p0 + tid - lp * kv.page_size;
+        }
+        __syncthreads();
+        auto widen = [&](int codes, int steps, int width) {
+            const int words = width / 8;
+            for (int i = tid; i < cnt * words; i += Q4P_THREADS) {
+                const int r = i / words, w = i % words;
+                const uint8_t* from = pool + rec[r];
+                const uint32_t word = *reinterpret_cast<const uint32_t*>(from + codes + ((long long)at[r] * words + w) * 4);
+                const float s = q4_step(from[steps + (long long)at[r] * (words / 2) + w / 2]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) tile[r * pitch + w * 8 + j] = q4_digit(word, j) * s;
+            }
+        };
+        widen(0, kv.k_steps, hd);
+        __syncthreads();
+        {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            if (key < cnt) {
+                const float* kr = tile + key * pitch;
+                for (int d = 0; d < hd; ++d) {
+                    const float k = kr[d];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[i] = fmaf(qs[(half * 4 + i) * hd + d], k, s[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[key * Q4P_HEADS + half * 4 + i] = key < cnt ? s[i] : -INFINITY;
+        }
+        __syncthreads();
+        // a warp per two heads: maximum, weights and sum of the tile's 64 scores
+        {
+            const int warp = tid >> 5, lane = tid & 31;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int h = warp * 2 + i;
+                const float a = sc[lane * Q4P_HEADS + h], b = sc[(lane + 32) * Q4P_HEADS + h];
+                const float m_old = m_run[h], m_new = fmaxf(m_old, warp_max(fmaxf(a, b)));
+                const float use = m_new == -INFINITY ? 0.f : m_new;
+                const float pa = exp2f(a - use), pb = exp2f(b - use);
+                const float l = warp_sum(pa + pb);
+                sc[lane * Q4P_HEADS + h] = pa;
+                sc[(lane + 32) * Q4P_HEADS + h] = pb;
+                __syncwarp();
+                if (lane == 0) {
+                    const float f = exp2f(m_old - use);
+                    corr[h] = f;
+                    l_run[h] = l_run[h] * f + l;
+                    m_run[h] = m_new;
+                }
+            }
+        }
+        widen(kv.v_codes, kv.v_steps, vd);
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < Q4P_HEADS; ++i) acc[c][i] *= corr[i];
+        for (int j = 0; j < cnt; ++j) {
+            const float4 a = *reinterpret_cast<const float4*>(sc + j * Q4P_HEADS), b = *reinterpret_cast<const float4*>(sc + j * Q4P_HEADS + 4);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int d = tid + c * Q4P_THREADS;
+                if (d < vd) {
+                    const float v = tile[j * pitch + d];
+                    acc[c][0] = fmaf(a.x, v, acc[c][0]); acc[c][1] = fmaf(a.y, v, acc[c][1]);
+                    acc[c][2] = fmaf(a.z, v, acc[c][2]); acc[c][3] = fmaf(a.w, v, acc[c][3]);
+                    acc[c][4] = fmaf(b.x, v, acc[c][4]); acc[c][5] = fmaf(b.y, v, acc[c][5]);
+                    acc[c][6] = fmaf(b.z, v, acc[c][6]); acc[c][7] = fmaf(b.w, v, acc[c][7]);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const long long part = (((long long)t * gridDim.y + blockIdx.y) * gridDim.z + blockIdx.z) * Q4P_HEADS;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int d = tid + c * Q4P_THREADS;
+        if (d >= vd) continue;
+#pragma unroll
+        for (int i = 0; i < Q4P_HEADS; ++i) {
+            if (i >= n_heads) continue;
+            if (part_o == nullptr) stf(out + ((long long)t * heads + h0 + i) * vd + d, acc[c][i] / l_run[i]);
+            else part_o[(part + i) * vd + d] = acc[c][i];
+        }
+    }
+    if (part_o != nullptr && tid < Q4P_HEADS) part_ml[part + tid] = make_float2(m_run[tid], l_run[tid]);
+}
+
+// The shares of a (token, head block) folded in ascending order: a CTA each.
+template <typename T>
+__global__ void __launch_bounds__(Q4P_THREADS)
+attention_q4_plain_fold_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, int heads,
+                               int kv_heads, int vd, int splits) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int group = heads / kv_heads, blocks = (group + Q4P_HEADS - 1) / Q4P_HEADS;
+    const int t = blockIdx.x, kh = blockIdx.y / blocks, h0 = kh * group + blockIdx.y % blocks * Q4P_HEADS;
+    const int n_heads = min(Q4P_HEADS, (kh + 1) * group - h0);
+    const long long part = ((long long)t * gridDim.y + blockIdx.y) * splits * Q4P_HEADS;
+    for (int i = threadIdx.x; i < n_heads * vd; i += Q4P_THREADS) {
+        const int h = i / vd, d = i % vd;
+        float m = -INFINITY;
+        for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[part + s * Q4P_HEADS + h].x);
+        const float use = m == -INFINITY ? 0.f : m;
+        float l = 0.f, o = 0.f;
+        for (int s = 0; s < splits; ++s) {
+            const float2 ml = part_ml[part + s * Q4P_HEADS + h];
+            const float f = exp2f(ml.x - use);
+            l = fmaf(ml.y, f, l);
+            o = fmaf(part_o[(part + s * Q4P_HEADS + h) * vd + d], f, o);
+        }
+        stf(out + ((long long)t * heads + h0 + h) * vd + d, o / l);
+    }
+}
+
+template <typename T>
+static int attention_q4_plain_launch(const T* q, const uint8_t* pool, const int32_t* positions, const int32_t* token_slot, T* out,
+                                     const PagedQ4& kv, int n, int heads, float scale_log2, int window, int splits, float* scratch,
+                                     cudaStream_t stream) {
+    const int group = heads / kv.kv_heads, gy = kv.kv_heads * ((group + Q4P_HEADS - 1) / Q4P_HEADS);
+    const size_t smem = (Q4P_HEADS * kv.hd + Q4P_KEYS * ((kv.hd > kv.vd ? kv.hd : kv.vd) + 1) + Q4P_KEYS * Q4P_HEADS) * sizeof(float);
+    constexpr size_t most = (Q4P_HEADS * 256 + Q4P_KEYS * 257 + Q4P_KEYS * Q4P_HEADS) * sizeof(float);
+    if (int st = ensure_dynamic_smem<attention_q4_plain_kernel<T>>(most, "axon_attention_q4_plain")) return st;
+    float* po = splits > 1 ? scratch : nullptr;
+    float2* ml = splits > 1 ? reinterpret_cast<float2*>(scratch + (long long)n * gy * splits * Q4P_HEADS * kv.vd) : nullptr;
+    launch_pdl(attention_q4_plain_kernel<T>, dim3(n, gy, splits), dim3(Q4P_THREADS), smem, stream, q, pool, positions, token_slot, out, kv,
+               heads, scale_log2, window, po, ml);
+    if (int st = launch_status("axon_attention_q4_plain")) return st;
+    if (splits > 1) {
+        launch_pdl(attention_q4_plain_fold_kernel<T>, dim3(n, gy), dim3(Q4P_THREADS), 0, stream, (const float*)po, (const float2*)ml, out,
+                   heads, kv.kv_heads, kv.vd, splits);
+        return launch_status("axon_attention_q4_plain fold");
+    }
+    return AXON_OK;
+}
+
+}  // namespace axon
+
+using namespace axon;
+
+enum { AXON_Q4_F32 = 0, AXON_Q4_BF16 = 1 };          // the dtype codes of generic.cu
+
+// Rotates q and k (as axon_rope_kv_write), writes q in `dtype` and k and v quantised into the pool.
+AXON_API int axon_rope_kv_write_q4(const float* qkv, const float* table, const int32_t* positions, const int32_t* token_slot,
+                                   void* q_out, void* pool, int dtype, const AxonKvLayout* layout, int n, int heads, int rot,
+                                   int adjacent, int write_kv, const float* partial, int splits, int ntok, const float* bias,
+                                   cudaStream_t stream) {
+    if (n <= 0) return AXON_OK;
+    if (partial != nullptr && (splits < 1 || ntok < n)) { set_error("axon_rope_kv_write_q4: bad partial sums (splits %d, tokens %d of %d)", splits, n, ntok); return AXON_BAD_ARGUMENT; }
+    PagedQ4 kv;
+    if (int st = to_q4(layout, pool, "axon_rope_kv_write_q4", &kv)) return st;
+    if (rot % 2 || rot > kv.hd || rot < 0) { set_error("axon_rope_kv_write_q4: rotated size %d must be even and at most the head size %d", rot, kv.hd); return AXON_BAD_ARGUMENT; }
+    if (dtype != AXON_Q4_F32 && dtype != AXON_Q4_BF16) { set_error("axon_rope_kv_write_q4: unknown dtype %d", dtype); return AXON_BAD_ARGUMENT; }
+    const SplitFold fold{partial, partial ? bias : nullptr, splits, ntok};
+    const int rows = heads + kv.planes * kv.kv_heads;
+    const dim3 grid(n, (rows + 7) / 8);
+    const bool vec = rot % 8 == 0 && (((uintptr_t)qkv | (uintptr_t)table | (uintptr_t)partial | (uintptr_t)bias) & 15) == 0;
+#define AXON_Q4_WRITE(T, VEC) launch_pdl(rope_kv_write_q4_kernel<T, VEC>, grid, dim3(256), 0, stream, qkv, (const float2*)table, positions, token_slot, (T*)q_out, (uint8_t*)pool, kv, heads, rot, adjacent, write_kv, fold)
+    if (dtype == AXON_Q4_F32) { if (vec) AXON_Q4_WRITE(float, true); else AXON_Q4_WRITE(float, false); }
+    else { if (vec) AXON_Q4_WRITE(__nv_bfloat16, true); else AXON_Q4_WRITE(__nv_bfloat16, false); }
+#undef AXON_Q4_WRITE
+    return launch_status("axon_rope_kv_write_q4");
+}
+
+// Output rows 0 .. n_rows - 1 ([kv_heads][width] each) from the spans [4][n_spans]: slot, first
+// position, count, first output row.  Rows of no span, and rows of a span that lies outside the block
+// table (n_slots rows), stay as they are.  keys or values may be null.
+AXON_API int axon_kv_read_q4(const void* pool, const AxonKvLayout* layout, const int32_t* spans, int n_spans, int n_slots,
+                             void* keys, void* values, int dtype, long long n_rows, cudaStream_t stream) {
+    if (n_rows <= 0 || n_spans <= 0) return AXON_OK;
+    PagedQ4 kv;
+    if (int st = to_q4(layout, pool, "axon_kv_read_q4", &kv)) return st;
+    if (((uintptr_t)keys | (uintptr_t)values) & 15) { set_error("axon_kv_read_q4: outputs must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
+    if (dtype != AXON_Q4_F32 && dtype != AXON_Q4_BF16) { set_error("axon_kv_read_q4: unknown dtype %d", dtype); return AXON_BAD_ARGUMENT; }
+    if (values != nullptr && keys != nullptr && kv.vd != kv.hd) {
+        // the two planes have strides of their own: one launch each
+        if (int st = axon_kv_read_q4(pool, layout, spans, n_spans, n_slots, keys, nullptr, dtype, n_rows, stream)) return st;
+        return axon_kv_read_q4(pool, layout, spans, n_spans, n_slots, nullptr, values, dtype, n_rows, stream);
+    }
+    const long long width = values != nullptr ? kv.vd : kv.hd;
+    const Q4Out out{keys, values, kv.kv_heads * width, 0, width, 1};
+    int rows = Q4_READ_ROWS;
+    while (rows > 1 && (n_rows + rows - 1) / rows < 2 * 148) rows /= 2;      // few rows: more CTAs rather than longer ones
+    const long long ctas = (n_rows + rows - 1) / rows;
+    if (ctas > 0x7fffffffLL) { set_error("axon_kv_read_q4: %lld rows are too many", n_rows); return AXON_BAD_ARGUMENT; }
+    if (dtype == AXON_Q4_F32)
+        launch_pdl(kv_read_q4_kernel<float>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, out);
+    else
+        launch_pdl(kv_read_q4_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, out);
+    return launch_status("axon_kv_read_q4");
+}
+
+// Floats of scratch that axon_attention_q4_plain needs for its key shares (0 for one share).
+AXON_API long long axon_attention_q4_plain_scratch(int n, int heads, int kv_heads, int v_dim, int splits) {
+    if (splits <= 1 || kv_heads < 1) return 0;
+    const int group = heads / kv_heads;
+    return (long long)n * kv_heads * ((group + Q4P_HEADS - 1) / Q4P_HEADS) * splits * Q4P_HEADS * (v_dim + 2);
+}
+
+AXON_API int axon_attention_q4_plain(const void* q, const void* pool, int dtype, const int32_t* positions, const int32_t* token_slot,
+                                     void* out, const AxonKvLayout* layout, int n, int heads, float scale, int window, int splits,
+                                     float* scratch, long long scratch_floats, cudaStream_t stream) {
+    if (n <= 0) return AXON_OK;
+    PagedQ4 kv;
+    if (int st = to_q4(layout, pool, "axon_attention_q4_plain", &kv)) return st;
+    if (kv.hd > 256 || kv.vd > 256) { set_error("axon_attention_q4_plain: rows of %d and %d values exceed 256", kv.hd, kv.vd); return AXON_BAD_ARGUMENT; }
+    if (heads < 1 || heads % kv.kv_heads) { set_error("axon_attention_q4_plain: %d heads over %d kv heads", heads, kv.kv_heads); return AXON_BAD_ARGUMENT; }
+    if (splits < 1 || splits > 65535) { set_error("axon_attention_q4_plain: bad split count %d", splits); return AXON_BAD_ARGUMENT; }
+    if ((long long)kv.kv_heads * ((heads / kv.kv_heads + Q4P_HEADS - 1) / Q4P_HEADS) > 65535) { set_error("axon_attention_q4_plain: %d heads are too many", heads); return AXON_BAD_ARGUMENT; }
+    const long long need = axon_attention_q4_plain_scratch(n, heads, kv.kv_heads, kv.vd, splits);
+    if (need > 0 && (scratch == nullptr || scratch_floats < need || ((uintptr_t)scratch & 15))) { set_error("axon_attention_q4_plain: %d key shares need %lld floats of 16-byte aligned scratch", splits, need); return AXON_BAD_ARGUMENT; }
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (dtype == AXON_Q4_F32)
+        return attention_q4_plain_launch<float>((const float*)q, (const uint8_t*)pool, positions, token_slot, (float*)out, kv, n, heads, scale_log2, window, splits, scratch, stream);
+    if (dtype == AXON_Q4_BF16)
+        return attention_q4_plain_launch<__nv_bfloat16>((const __nv_bfloat16*)q, (const uint8_t*)pool, positions, token_slot, (__nv_bfloat16*)out, kv, n, heads, scale_log2, window, splits, scratch, stream);
+    set_error("axon_attention_q4_plain: unknown dtype %d", dtype);
+    return AXON_BAD_ARGUMENT;
+}

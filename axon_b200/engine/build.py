@@ -30,6 +30,17 @@ def parse_dtype(d: Union[str, torch.dtype]) -> torch.dtype:
         raise ValueError(f"dtype '{d}' is not bfloat16 or float32") from None
 
 
+def parse_kv(kv: str, dtype: Union[str, torch.dtype]) -> int:
+    """Bits of a cached value for a cache type by name: 0 stands for the model's dtype."""
+    if kv in ("auto", "q4"):
+        return 4 if kv == "q4" else 0
+    if kv not in ("bf16", "bfloat16", "f32", "float32"):
+        raise ValueError(f"KV type '{kv}' is not supported (bf16 with a bfloat16 model, f32 with a float32 one, q4 with either)")
+    if parse_dtype(kv) != parse_dtype(dtype):
+        raise ValueError(f"the cache has the model's dtype ({dtype}) or 4 bits a value; '{kv}' differs")
+    return 0
+
+
 def require_gpu(device: Union[str, torch.device]) -> torch.device:
     """The engine has no CPU path: the device must be a CUDA GPU and the kernels must load."""
     dev = torch.device(device)
@@ -54,7 +65,7 @@ def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] 
                  device: Union[str, torch.device] = "cuda:0", page_size: int = 16,
                  max_tokens: Optional[int] = 4096, max_slots: int = 16, max_positions: Optional[int] = None,
                  shuffle_seed: int = 0, max_step_tokens: int = 8192, gain_std: float = 0.1,
-                 check_tables: Optional[bool] = None) -> Engine:
+                 check_tables: Optional[bool] = None, kv: str = "auto") -> Engine:
     """An engine over the model in ``folder`` (config.json + safetensors), or over seeded
     random weights of ``config`` made on the device when no folder is given.
 
@@ -65,7 +76,8 @@ def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] 
     ``max_position_embeddings``).  ``check_tables`` (default: the environment's
     ``AXON_CHECK_TABLES=1``) is a debugging mode in which the kernels compare every
     block-table entry they read with the pool's size and the step raises instead of
-    following a bad one.
+    following a bad one.  ``kv`` is the cache type: ``auto`` (the model's dtype) or ``q4`` (quantised to
+    4 bits as it is written, in every part that takes it).
     """
     dev = require_gpu(device)
     dt = parse_dtype(dtype)
@@ -75,7 +87,7 @@ def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] 
         raise ValueError("build_engine needs a model folder or a configuration")
     arch = architecture_of(config.to_dict())
     spec = arch.build_spec(config)
-    rt = Runtime(dt, dev)
+    rt = Runtime(dt, dev, kv_bits=parse_kv(kv, dt))
     with torch.cuda.device(dev):
         if folder is not None:
             weights = load_weights(folder, spec, dt, dev)
@@ -88,7 +100,7 @@ def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] 
             torch.cuda.synchronize(dev)
             torch.cuda.empty_cache()            # what loading set free counts as free
             free, _ = torch.cuda.mem_get_info(dev)
-            max_tokens = plan_pool_tokens(free, bytes_per_token(model.needs, dt), page_size, max_slots, max_positions,
+            max_tokens = plan_pool_tokens(free, bytes_per_token(model.needs, dt, page_size), page_size, max_slots, max_positions,
                                           step_workspace_bytes(spec.hidden_size, spec.vocab_size,
                                                                min(max_step_tokens, max_slots * max_positions), max_slots))
             if max_tokens < page_size:

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+from dataclasses import replace
 from typing import Any, Dict, List, Optional, Union
 
 import torch
@@ -51,7 +52,9 @@ class DecoderModel:
         #: what each schedule entry keeps in the cache: {part path: need} over the cache-keeping
         #: parts of its layer (empty when it keeps nothing of its own)
         self.needs: List[Dict[str, Union[KvNeed, StateNeed]]] = []
-        per_layer = [layer_cache_needs(l) for l in spec.layers]
+        per_layer = [layer_cache_needs(l, rt.kv_bits) for l in spec.layers]
+        if rt.kv_bits and not any(getattr(n, "bits", 0) for needs in per_layer for n in needs.values()):
+            raise ValueError(f"no part of this model keeps its cache in {rt.kv_bits} bits")
         for e in spec.schedule:
             self.needs.append({} if e.cache_of is not None else dict(per_layer[e.layer]))
 
@@ -110,17 +113,20 @@ class DecoderModel:
         return logits
 
 
-def layer_cache_needs(layer) -> Dict[str, Union[KvNeed, StateNeed]]:
+def layer_cache_needs(layer, kv_bits: int = 0) -> Dict[str, Union[KvNeed, StateNeed]]:
     """What a layer keeps in the cache: ``{part path: need}`` for every part of its arrangement,
     nested ones included (paths are dotted: ``"mixer"``, ``"mixer.inner"``), whose class
     answers ``cache_need`` with something.  A layer may hold several such parts (attention
-    beside a mixer with state, say) or none; no part name is special."""
+    beside a mixer with state, say) or none; no part name is special.  With ``kv_bits`` the
+    parts that take that format (``Part.kv_bits``) ask for it."""
     out: Dict[str, Union[KvNeed, StateNeed]] = {}
 
     def rec(category: str, ps: PartSpec, path: str) -> None:
         cls = part_class(category, ps.kind)
         need = cls.cache_need(ps)
         if need is not None:
+            if kv_bits and isinstance(need, KvNeed) and kv_bits in cls.kv_bits:
+                need = replace(need, bits=kv_bits)
             out[path or ps.kind] = need
         nested = getattr(cls, "nested", {})
         for name, sub in ps.parts.items():

@@ -279,7 +279,7 @@ def attention_decode_fused(qkv, pending, table, rot: int, adjacent: bool, kv, ct
     the q/k/v product (or the partial sums it is still owed) instead of rotated queries.
     Refuses what ``attention`` refuses, steps with prompt portions, partial or adjacent-pair
     rotation, and head sizes that are no multiple of 8; the caller then takes the two kernels."""
-    if not (ENABLED["attention_decode"] and ENABLED["attention_fused"]) or ctx.unit_items is None:
+    if not (ENABLED["attention_decode"] and ENABLED["attention_fused"]) or ctx.unit_items is None or kv.bits:
         return False
     if out.dtype != torch.bfloat16 or kv.pool.dtype != torch.bfloat16 or kv.head_dim not in FA_HEAD_DIMS:
         return False
@@ -316,7 +316,7 @@ def attention_decode_fused(qkv, pending, table, rot: int, adjacent: bool, kv, ct
 def attention(q, kv, ctx, out, heads: int, scale: float) -> bool:
     """Tensor-core attention over the paged cache; refuses head sizes other than
     16/32/64/128, groups of more than 64 heads, and dtypes other than bfloat16."""
-    if not (ENABLED["attention_prefill"] and ENABLED["attention_decode"]):
+    if kv.bits or not (ENABLED["attention_prefill"] and ENABLED["attention_decode"]):
         return False
     if q.dtype != torch.bfloat16 or kv.pool.dtype != torch.bfloat16 or kv.head_dim not in FA_HEAD_DIMS:
         return False
@@ -349,3 +349,22 @@ def attention(q, kv, ctx, out, heads: int, scale: float) -> bool:
                                    it["pre"].data_ptr(), it["n_pre"], kv._ref, heads, float(scale), int(kv.window),
                                    0, it["tpt_pre"], 1, None, None, _stream()))
     return True
+
+
+# -- a cache held in 4 bits -------------------------------------------------
+
+#: keys that a CTA of the plain 4-bit attention folds at a time, heads that it serves, and how many
+#: CTAs its key shares aim at (five fit an SM at head size 128)
+Q4_PLAIN_KEYS, Q4_PLAIN_HEADS, Q4_PLAIN_CTAS = 64, 8, 5 * SM_COUNT
+
+
+def q4_plain_splits(ctx, heads: int, kv_heads: int, window: int) -> int:
+    """Into how many shares the plain 4-bit attention cuts each token's keys: as many as fill the GPU."""
+    keys = min(ctx.max_kv_len, window) if window else ctx.max_kv_len
+    ctas = ctx.n_tokens * kv_heads * -(-(heads // kv_heads) // Q4_PLAIN_HEADS)
+    return max(1, min(-(-keys // Q4_PLAIN_KEYS), Q4_PLAIN_CTAS // max(ctas, 1)))
+
+
+def q4_graph_key(ctx, heads: int, kv_heads: int, head_dim: int, window: int, precise: bool):
+    """What the 4-bit attention's launches take from the host beside the batch shape."""
+    return (("q4_plain", q4_plain_splits(ctx, heads, kv_heads, window)),)

@@ -37,7 +37,7 @@ class KvLayout(ctypes.Structure):
         ("v_dim", ctypes.c_int32),
         ("planes", ctypes.c_int32),
         ("n_pages", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
+        ("bits", ctypes.c_int32),
         ("fault", c_void_p),
     ]
 
@@ -53,6 +53,11 @@ _SIGNATURES = {
     "axon_rope_table": [P, P, P, c_int, c_int, c_float, P],
     "axon_rope_kv_write": [P, P, P, P, P, P, c_int, ctypes.POINTER(KvLayout), c_int, c_int, c_int, c_int, c_int,
                            P, c_int, c_int, P, P],
+    "axon_rope_kv_write_q4": [P, P, P, P, P, P, c_int, ctypes.POINTER(KvLayout), c_int, c_int, c_int, c_int, c_int,
+                              P, c_int, c_int, P, P],
+    "axon_kv_read_q4": [P, ctypes.POINTER(KvLayout), P, c_int, c_int, P, P, c_int, c_longlong, P],
+    "axon_attention_q4_plain": [P, P, c_int, P, P, P, ctypes.POINTER(KvLayout), c_int, c_int, c_float, c_int, c_int, P,
+                                c_longlong, P],
     "axon_attention_plain": [P, P, c_int, P, P, P, ctypes.POINTER(KvLayout), c_int, c_int, c_float, c_int, P],
     "axon_residual_add": [P, P, c_int, c_longlong, P],
     "axon_convert": [P, c_int, P, c_int, c_longlong, P],
@@ -111,6 +116,8 @@ def cuda() -> ctypes.CDLL:
         lib.axon_last_error.argtypes = []
         lib.axon_topk_max.restype = c_int
         lib.axon_topk_max.argtypes = []
+        lib.axon_attention_q4_plain_scratch.restype = c_longlong
+        lib.axon_attention_q4_plain_scratch.argtypes = [c_int, c_int, c_int, c_int, c_int]
         lib.axon_gemm_tc_force_tile.restype = None
         lib.axon_gemm_modelled_us.argtypes = [c_int, c_int, c_int, c_int, c_int]
         lib.axon_gemm_modelled_us.restype = ctypes.c_double

@@ -46,11 +46,12 @@ def linear_swiglu(h: torch.Tensor, w_gate_up: torch.Tensor, act: torch.Tensor, r
 
 def attention(q: torch.Tensor, kv: ops.KvView, ctx, out: torch.Tensor, heads: int, scale: float,
               precise: bool = False) -> None:
-    if not precise:
-        from . import fast
-        if fast.attention(q, kv, ctx, out, heads, scale):
-            return
-    ops.attention_plain(q, kv, ctx.positions, ctx.token_slot, out, heads, scale)
+    """Attention of the step's tokens over the paged cache (in the model's dtype or in 4 bits)."""
+    from . import fast
+    if not precise and fast.attention(q, kv, ctx, out, heads, scale):
+        return
+    splits = fast.q4_plain_splits(ctx, heads, kv.kv_heads, kv.window) if kv.bits else 1
+    ops.attention_plain(q, kv, ctx.positions, ctx.token_slot, out, heads, scale, rt=ctx.rt, splits=splits)
 
 
 def attention_decode_fused(qkv: torch.Tensor, pending, table, rot: int, adjacent: bool, kv: ops.KvView, ctx,

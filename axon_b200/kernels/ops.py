@@ -17,6 +17,7 @@ import torch
 
 from . import lib
 from .lib import KvLayout, check
+from ..parts.spec import KvNeed
 
 F32, BF16 = 0, 1
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
@@ -53,6 +54,11 @@ class KvView:
     read values from the key plane.  ``block_table`` is the group's device table
     ``[slots][stride]`` of int32.  ``fault`` (two uint32 on the device) switches checked
     tables on: see ``kv_layout.h``.
+
+    With ``bits`` 4 rows are quantised: ``pool`` is uint8 ``[pages + 1][entries][bytes]``, an entry
+    holding for each kv head the codes and steps of its key rows and those of its value rows
+    (``kv_layout.h``).  :func:`rope_kv_write` quantises what it writes, :func:`kv_read` gives
+    positions back as rows, and the attention functions read the pages as they are.
     """
 
     pool: torch.Tensor
@@ -65,12 +71,16 @@ class KvView:
     v_dim: int = 0
     planes: int = 2
     fault: Optional[torch.Tensor] = None
+    bits: int = 0
 
     def __post_init__(self) -> None:
         if self.planes not in (1, 2):
             raise ValueError(f"a cache entry has one or two planes, not {self.planes}")
         self.v_dim = self.head_dim if self.planes == 1 or not self.v_dim else self.v_dim
         entries = self.pool.shape[1]
+        if self.bits:
+            self._init_quantised(entries)
+            return
         self.k_plane = self.kv_heads * self.page_size * self.head_dim
         self.v_plane = self.kv_heads * self.page_size * self.v_dim if self.planes == 2 else 0
         per_entry = self.k_plane + self.v_plane
@@ -82,10 +92,30 @@ class KvView:
             page_size=self.page_size, kv_heads=self.kv_heads, head_dim=self.head_dim,
             page_stride=entries * per_entry, entry_offset=self.entry * per_entry,
             v_offset=self.k_plane if self.planes == 2 else 0, v_dim=self.v_dim, planes=self.planes,
-            n_pages=self.n_pages, reserved=0, fault=None if self.fault is None else self.fault.data_ptr())
+            n_pages=self.n_pages, bits=0, fault=None if self.fault is None else self.fault.data_ptr())
+        self._ref = ctypes.byref(self.layout)
+
+    def _init_quantised(self, entries: int) -> None:
+        need = KvNeed(self.kv_heads, self.head_dim, None, self.v_dim, self.planes, self.bits)
+        per_entry = need.page_bytes(self.page_size, 1)
+        if self.pool.dtype != torch.uint8 or not self.pool.is_contiguous():
+            raise ValueError(f"a {self.bits}-bit pool is contiguous bytes (uint8), not {self.pool.dtype}")
+        if self.pool[0].numel() != entries * per_entry:
+            raise ValueError(f"a page of {self.pool[0].numel()} bytes does not hold {entries} entries of {per_entry}")
+        if self.block_table.dtype != torch.int32 or not self.block_table.is_contiguous():
+            raise ValueError("a block table is contiguous int32")
+        self.n_pages = self.pool.shape[0] - 1
+        self.layout = KvLayout(
+            block_table=self.block_table.data_ptr(), table_stride=self.block_table.shape[1],
+            page_size=self.page_size, kv_heads=self.kv_heads, head_dim=self.head_dim,
+            page_stride=entries * per_entry, entry_offset=self.entry * per_entry, v_offset=0, v_dim=self.v_dim,
+            planes=self.planes, n_pages=self.n_pages, bits=self.bits,
+            fault=None if self.fault is None else self.fault.data_ptr())
         self._ref = ctypes.byref(self.layout)
 
     def _plane(self, offset: int, dim: int) -> torch.Tensor:
+        if self.bits:
+            raise ValueError(f"rows of a {self.bits}-bit cache are no view of its pool: read them with kv_read")
         flat = self.pool.view(self.pool.shape[0], -1)
         start = self.layout.entry_offset + offset
         return flat[:, start:start + self.kv_heads * self.page_size * dim].view(-1, self.kv_heads, self.page_size, dim)
@@ -171,18 +201,30 @@ def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, table: torch.Ten
 def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: torch.Tensor,
                   token_slot: torch.Tensor, q_out: torch.Tensor, kv: KvView, heads: int, rot: int,
                   adjacent: bool = False, write_kv: bool = True, pending=None) -> None:
-    """``pending`` (a ``fast.PendingFold`` whose output is ``qkv``): the product is still in
-    partial sums; they are folded here (with the bias) and ``qkv`` itself is not read."""
+    """Rotates queries and keys and writes queries to ``q_out``, keys and values to the cache (quantised
+    when ``kv`` has 4 bits).  ``pending`` (a ``fast.PendingFold`` whose output is ``qkv``): the product is
+    still in partial sums; they are folded here (with the bias) and ``qkv`` itself is not read."""
     _dev(qkv, table, positions, token_slot, q_out, kv.pool)
     n = q_out.shape[0]
     width = (heads + kv.kv_heads) * kv.head_dim + (kv.kv_heads * kv.v_dim if kv.planes == 2 else 0)
     if qkv.dtype != torch.float32 or qkv.shape[1] != width:
         raise ValueError("rope_kv_write reads float32 [n][(heads + kv_heads) * head_dim + kv_heads * v_dim]")
-    if q_out.dtype != kv.pool.dtype:
-        raise TypeError("queries and the cache have one dtype")
+    if kv.bits:
+        _quantised("rope_kv_write", kv, qkv, q_out, positions, token_slot, table)
+        if q_out.shape[1] != heads * kv.head_dim or qkv.shape[0] < n or positions.numel() < n or token_slot.numel() < n:
+            raise ValueError("rope_kv_write takes a row of qkv, a position and a slot for each row of q_out")
+        if (positions.dtype, token_slot.dtype) != (torch.int32, torch.int32):
+            raise TypeError("positions and slots are int32")
+        if table is not None and (table.dtype != torch.float32 or table.numel() < n * rot):
+            raise ValueError("rope_kv_write takes a float32 rotation table [n][rot / 2][2]")
+        write = lib.cuda().axon_rope_kv_write_q4
+    else:
+        if q_out.dtype != kv.pool.dtype:
+            raise TypeError("queries and the cache have one dtype")
+        write = lib.cuda().axon_rope_kv_write
     if pending is not None:
         pending.claim(qkv, accumulate=False)
-    check(lib.cuda().axon_rope_kv_write(_ptr(qkv), _ptr(table), _ptr(positions), _ptr(token_slot), _ptr(q_out),
+    check(write(_ptr(qkv), _ptr(table), _ptr(positions), _ptr(token_slot), _ptr(q_out),
                                         _ptr(kv.pool), dtype_code(q_out), kv._ref, n, heads, rot, int(adjacent),
                                         int(write_kv), None if pending is None else _ptr(pending.partial),
                                         0 if pending is None else pending.splits,
@@ -190,10 +232,58 @@ def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: t
                                         None if pending is None else _ptr(pending.bias), _stream()))
 
 
+def _quantised(what: str, kv: KvView, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuse a view without quantised rows, or operands on another device than the one launches go to."""
+    if not kv.bits:
+        raise ValueError(f"{what} takes a cache with quantised rows")
+    here = torch.cuda.current_device()
+    for t in (kv.pool, kv.block_table, *tensors):
+        if t is not None and t.device.index != here:
+            raise ValueError(f"{what}: an operand is on {t.device}, the current device is cuda:{here}")
+
+
+def kv_read(kv: KvView, spans: torch.Tensor, keys: Optional[torch.Tensor], values: Optional[torch.Tensor] = None) -> None:
+    """Positions of requests out of a cache with quantised rows.
+
+    ``spans`` is int32 ``[4][n]``: slot, first position, count and first output row of each span.  Row
+    ``r`` of ``keys`` (``[rows][kv_heads][head_dim]``) and of ``values`` (``[rows][kv_heads][v_dim]``), float32 or
+    bfloat16, receives the position whose span covers ``r`` (the first such span); the numbers are exact in
+    both types.  Rows of no span stay as they are, and so do those of positions outside the block table.
+    Either output may be None; with one plane values are the keys."""
+    _quantised("kv_read", kv, spans, keys, values)
+    _dev(spans, keys, values, kv.pool)
+    if spans.dtype != torch.int32 or spans.dim() != 2 or spans.shape[0] != 4:
+        raise ValueError("kv_read takes int32 spans [4][n]: slot, first position, count, first output row")
+    if keys is None and values is None:
+        raise ValueError("kv_read takes keys, values or both to write to")
+    rows = (keys if keys is not None else values).shape[0]
+    for t, width, name in ((keys, kv.head_dim, "keys"), (values, kv.v_dim, "values")):
+        if t is not None and tuple(t.shape) != (rows, kv.kv_heads, width):
+            raise ValueError(f"kv_read writes {name} as [{rows}][{kv.kv_heads}][{width}], not {list(t.shape)}")
+    if keys is not None and values is not None and keys.dtype != values.dtype:
+        raise TypeError("keys and values are read back in one dtype")
+    check(lib.cuda().axon_kv_read_q4(_ptr(kv.pool), kv._ref, _ptr(spans), spans.shape[1], kv.block_table.shape[0], _ptr(keys),
+                                     _ptr(values), dtype_code(keys if keys is not None else values), rows, _stream()))
+
+
 def attention_plain(q: torch.Tensor, kv: KvView, positions: torch.Tensor, token_slot: torch.Tensor,
-                    out: torch.Tensor, heads: int, scale: float) -> None:
+                    out: torch.Tensor, heads: int, scale: float, rt=None, splits: int = 1) -> None:
+    """Attention of each token over its request's positions up to its own, by the plain kernels.  ``splits``
+    (4-bit caches only; scratch comes from ``rt``): into how many shares each token's keys are cut."""
     _dev(q, positions, token_slot, out, kv.pool)
     n = q.shape[0]
+    if kv.bits:
+        _quantised("attention_plain", kv, q, positions, token_slot, out)
+        if out.dtype != q.dtype or out.numel() != n * heads * kv.v_dim or q.numel() != n * heads * kv.head_dim:
+            raise ValueError("attention_plain takes queries [n][heads * head_dim] and writes [n][heads * v_dim] in their dtype")
+        scratch, floats = None, 0
+        if splits > 1:
+            floats = lib.cuda().axon_attention_q4_plain_scratch(n, heads, kv.kv_heads, kv.v_dim, splits)
+            scratch = rt.buffer("q4_plain_scratch", (floats,), torch.float32)
+        check(lib.cuda().axon_attention_q4_plain(_ptr(q), _ptr(kv.pool), dtype_code(q), _ptr(positions), _ptr(token_slot), _ptr(out),
+                                                 kv._ref, n, heads, float(scale), int(kv.window), splits, _ptr(scratch), floats,
+                                                 _stream()))
+        return
     if q.dtype != kv.pool.dtype or out.dtype != q.dtype:
         raise TypeError("queries, cache and output have one dtype")
     check(lib.cuda().axon_attention_plain(_ptr(q), _ptr(kv.pool), dtype_code(q), _ptr(positions), _ptr(token_slot),

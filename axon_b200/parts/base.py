@@ -41,11 +41,15 @@ class Runtime:
     """What parts share at run time: the model's dtype and device, and named
     scratch buffers that are reused from step to step (a buffer only ever grows)."""
 
-    def __init__(self, dtype: torch.dtype, device: Union[str, torch.device]):
+    def __init__(self, dtype: torch.dtype, device: Union[str, torch.device], kv_bits: int = 0):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"the engine runs in float32 or bfloat16, not {dtype}")
         self.dtype = dtype
         self.device = torch.device(device)
+        if kv_bits not in (0, 4):
+            raise ValueError(f"cache rows have the model's dtype (0) or 4 bits a value, not {kv_bits}")
+        #: bits of a cached value (0: the model's dtype) in the caches of parts that take them (``Part.kv_bits``)
+        self.kv_bits = kv_bits
         #: the true 32-bit path: plain FFMA kernels everywhere
         self.precise = dtype == torch.float32
         self._buffers: Dict[str, torch.Tensor] = {}
@@ -157,6 +161,9 @@ class Part:
     #: branching on device data, no allocation.  Steps of a model whose parts are all safe
     #: may be captured into CUDA graphs.
     graph_safe: ClassVar[bool] = False
+    #: quantised row formats (``KvNeed.bits``) in which this part can keep its cache; the engine asks
+    #: for one with ``Runtime.kv_bits``, and parts that do not take it keep the model's dtype
+    kv_bits: ClassVar[Tuple[int, ...]] = ()
     #: Owed sums.  A product for few rows may be split over K and leave its partial sums in
     #: scratch for the next reader of its output (``kernels.fast.PendingFold``), which saves
     #: that product a pass.  A mixer or feed-forward whose class sets ``may_defer`` takes

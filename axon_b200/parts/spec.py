@@ -93,13 +93,22 @@ class KvNeed:
     """Rows in pages, per token and kv head: a key row of ``head_dim`` elements and, with
     ``planes`` 2, a value row of ``v_dim`` (None: as wide as the key).  ``planes`` 1 keeps one
     row only (a latent that serves as key and value).  ``window`` None keeps every position,
-    else only the last ``window``."""
+    else only the last ``window``.  ``bits`` 0 keeps rows in the model's dtype, 4 quantised
+    (``kv_layout.h``: two values a byte and a step byte for every sixteen; widths are then
+    multiples of 16)."""
 
     kv_heads: int
     head_dim: int
     window: Optional[int] = None
     v_dim: Optional[int] = None
     planes: int = 2
+    bits: int = 0
+
+    def __post_init__(self) -> None:
+        if self.bits not in (0, 4):
+            raise ValueError(f"cache rows have the model's dtype (bits 0) or 4 bits a value, not {self.bits}")
+        if self.bits and (self.head_dim % 16 or self.value_dim % 16 or self.head_dim <= 0):
+            raise ValueError(f"a 4-bit cache holds rows of a multiple of 16 values, not {self.head_dim} and {self.value_dim}")
 
     @property
     def value_dim(self) -> int:
@@ -109,6 +118,13 @@ class KvNeed:
     def elements_per_token(self) -> int:
         """Cache elements one position takes in one schedule entry."""
         return self.kv_heads * (self.head_dim + (self.value_dim if self.planes == 2 else 0))
+
+    def page_bytes(self, page_size: int, itemsize: int) -> int:
+        """Bytes one schedule entry takes of a page, in a model whose dtype has ``itemsize`` bytes."""
+        if not self.bits:
+            return self.elements_per_token * page_size * itemsize
+        widths = (self.head_dim, self.value_dim)[:self.planes]
+        return self.kv_heads * sum(-(-page_size * part // 16) * 16 for w in widths for part in (w // 2, w // 16))
 
 
 @dataclass(frozen=True)

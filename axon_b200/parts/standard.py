@@ -108,6 +108,7 @@ class Attention(Mixer):
     category, kind = "mixer", "attention"
     graph_safe = True
     may_defer = True
+    kv_bits = (4,)
     nested = {"position": "position"}
 
     @classmethod
@@ -149,9 +150,11 @@ class Attention(Mixer):
     def graph_key(self, ctx: StepContext):
         """The split count of the decode-shape attention, which follows the longest context among
         the segments short enough for that shape (every segment, in a step of single tokens)."""
+        from ..kernels import fast
+        if self.rt.kv_bits:
+            return fast.q4_graph_key(ctx, self.heads, self.kv_heads, self.head_dim, self.window, self.rt.precise)
         if self.rt.precise:
             return ()
-        from ..kernels import fast
         group = self.heads // self.kv_heads
         fits = 16 // group if group <= 16 else 0
         short = [kv for n, kv in zip(ctx.seg_q_len, ctx.seg_kv_len) if n <= fits]

@@ -1,0 +1,88 @@
+"""The 4-bit cache without a GPU: its format's bounds, what a part's cache need takes, options and refusals."""
+
+import numpy as np
+import pytest
+import torch
+
+import plain_q4 as q4
+from conftest import TINY
+
+
+def test_every_value_is_off_by_half_a_step_at_most():
+    rng = np.random.default_rng(1)
+    for scale in (1e-4, 0.02, 1.0, 300.0, 7e3):
+        x = (rng.standard_normal((500, 64)) * scale).astype(np.float32)
+        x[np.abs(x) > 57600] = 0
+        n, s = q4.quantise(x)
+        back = q4.values(n, s)
+        step = np.repeat(np.array([q4.step_of(b) for b in s.reshape(-1)]).reshape(s.shape), 16, -1)
+        # x * (1 / s) is rounded twice to 32 bits before rint: 2^-23 of at most 7.5
+        assert (np.abs(back - x) <= step * (0.5 + 7.5 * 2.0 ** -22)).all()
+
+
+def test_values_are_exact_in_bfloat16_and_steps_cover_the_range():
+    assert q4.STEPS[1] == 2.0 ** -17 and q4.STEPS[-1] == 7680.0 and (np.diff(q4.STEPS) > 0).all()
+    n, s = np.meshgrid(np.arange(1, 16), np.arange(q4.TOP + 1), indexing="ij")
+    v = torch.from_numpy(q4.values(np.repeat(n.reshape(-1, 1), 16, 1), s.reshape(-1, 1)))
+    assert torch.equal(v.to(torch.bfloat16).double(), v) and torch.equal(v.float().double(), v)
+
+
+def test_needs_of_quantised_rows():
+    from axon_b200.cache.manager import bytes_per_token
+    from axon_b200.parts.spec import KvNeed
+    for ps, hd, vd, planes in ((16, 128, 128, 2), (4, 64, 64, 2), (1, 16, 16, 2), (5, 48, 32, 2), (7, 32, 32, 1)):
+        need = KvNeed(3, hd, v_dim=vd, planes=planes, bits=4)
+        assert need.page_bytes(ps, 2) == 3 * q4.parts(ps, hd, vd, planes)[1]
+    assert bytes_per_token([KvNeed(4, 128, bits=4)], torch.bfloat16) == 4 * 2 * 72
+    assert bytes_per_token([KvNeed(4, 128)], torch.bfloat16) == 4 * 2 * 256
+    assert bytes_per_token([KvNeed(1, 16, bits=4)], torch.float32, 1) == 64      # four parts padded to 16 bytes
+    with pytest.raises(ValueError, match="multiple of 16"):
+        KvNeed(2, 24, bits=4)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        KvNeed(2, 32, v_dim=40, bits=4)
+    with pytest.raises(ValueError, match="not 8"):
+        KvNeed(2, 32, bits=8)
+
+
+def test_only_parts_that_take_it_keep_a_quantised_cache():
+    from axon_b200.config import config_from_dict
+    from axon_b200.config.base import architecture_of
+    from axon_b200.engine.model import layer_cache_needs
+    cfg = config_from_dict(TINY["A"])
+    spec = architecture_of(cfg.to_dict()).build_spec(cfg)
+    assert [n.bits for n in layer_cache_needs(spec.layers[0]).values()] == [0]
+    assert [n.bits for n in layer_cache_needs(spec.layers[0], 4).values()] == [4]
+    from axon_b200.parts.base import Mixer, Runtime
+    assert Mixer.kv_bits == ()
+    with pytest.raises(ValueError, match="4 bits"):
+        Runtime(torch.bfloat16, "cpu", kv_bits=8)
+
+
+def test_cache_types_by_name():
+    from axon_b200.api import BackendOptions
+    from axon_b200.engine.build import parse_kv
+    assert BackendOptions().kv("q4")._kv == "q4" and BackendOptions().kv("bf16")._kv == "auto"
+    assert BackendOptions().kv("q4").kv("auto")._kv == "auto"
+    assert parse_kv("q4", "float32") == 4 and parse_kv("auto", torch.bfloat16) == 0
+    with pytest.raises(ValueError, match="q8"):
+        BackendOptions().kv("q8")
+    with pytest.raises(ValueError, match="differs"):
+        BackendOptions().kv("f32")
+
+
+def test_views_of_quantised_pools_are_checked():
+    from axon_b200.kernels import ops
+    table = torch.zeros(1, 4, dtype=torch.int32)
+    good = torch.zeros(5, 2, 2 * (q4.parts(16, 64, 64, 2)[1]), dtype=torch.uint8)
+    view = ops.KvView(good, table, 1, 16, 2, 64, bits=4)
+    assert view.layout.bits == 4 and view.layout.entry_offset == good.shape[2] and view.n_pages == 4
+    with pytest.raises(ValueError, match="kv_read"):
+        view.keys()
+    with pytest.raises(ValueError, match="uint8"):
+        ops.KvView(good.to(torch.int8), table, 1, 16, 2, 64, bits=4)
+    with pytest.raises(ValueError, match="does not hold"):
+        ops.KvView(good[:, :, 16:].contiguous(), table, 1, 16, 2, 64, bits=4)
+    with pytest.raises(ValueError, match="int32"):
+        ops.KvView(good, table.long(), 1, 16, 2, 64, bits=4)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        ops.KvView(good, table, 1, 16, 2, 40, bits=4)

@@ -1,0 +1,534 @@
+"""The 4-bit cache's operators on the GPU against ``plain_q4``: rotating and quantising rows as they are
+written, reading them back, attention over the pages, and the engine with such a cache."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_q4 as q4
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+DTYPES = [torch.float32, torch.bfloat16]
+#: half a step of a rounding to each type, relative to the value
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from axon_b200.kernels import ops as o
+    return o
+
+
+class Cache:
+    """Requests of given lengths in a pool whose other bytes are all 0xFF (steps that read as NaN)."""
+
+    def __init__(self, ops, lens, kv_heads, hd, ps, v_dim=None, planes=2, window=0, seed=0, room=0, fill=True, spare=3, loud=0.0):
+        self.lens, self.kv_heads, self.hd, self.ps, self.planes = lens, kv_heads, hd, ps, planes
+        self.v_dim = hd if v_dim is None or planes == 1 else v_dim
+        rng = np.random.default_rng(seed)
+        stride = -(-(max(lens) + room) // ps)
+        held = [-(-(l + room) // ps) for l in lens]
+        n_pages = sum(held) + spare
+        order = rng.permutation(n_pages)
+        self.table = np.full((len(lens), stride), n_pages, np.int32)
+        at = 0
+        for i, n in enumerate(held):
+            self.table[i, :n] = order[at:at + n]
+            at += n
+        self.places, self.record = q4.parts(ps, hd, self.v_dim, planes)
+        pool = np.full((n_pages + 1, 2, kv_heads * self.record), 0xFF, np.uint8)
+        shift = rng.standard_normal((kv_heads, hd)) * loud
+        self.k = [(rng.standard_normal((l, kv_heads, hd)) + shift).astype(np.float32) for l in lens]
+        self.v = [rng.standard_normal((l, kv_heads, self.v_dim)).astype(np.float32) for l in lens]
+        if fill:
+            for s, l in enumerate(lens):
+                rows = [q4.quantise(self.k[s])] + ([q4.quantise(self.v[s])] if planes == 2 else [])
+                self.k[s] = q4.values(*rows[0])
+                self.v[s] = q4.values(*rows[-1])
+                for p in range(l):
+                    for h in range(kv_heads):
+                        for j, (n, b) in enumerate(rows):
+                            page = int(self.table[s, p // ps])
+                            q4.put(pool, page, 1, h, self.record, self.places[2 * j], p % ps, q4.codes_of(n[p, h]))
+                            q4.put(pool, page, 1, h, self.record, self.places[2 * j + 1], p % ps, b[p, h])
+        self.pool = torch.from_numpy(pool).to(DEV)
+        self.dev_table = torch.from_numpy(self.table).to(DEV)
+        self.view = ops.KvView(self.pool, self.dev_table, 1, ps, kv_heads, hd, window, v_dim=self.v_dim, planes=planes, bits=4)
+
+
+def rotated(x, table, rot, adjacent):
+    """Rows [n, heads, hd] of float32, every product and sum rounded to 32 bits."""
+    x = x.copy()
+    if not rot:
+        return x
+    c, s = table[:, None, :, 0], table[:, None, :, 1]
+    first, second = (slice(0, rot, 2), slice(1, rot, 2)) if adjacent else (slice(0, rot // 2), slice(rot // 2, rot))
+    a, b = x[..., first].copy(), x[..., second].copy()
+    x[..., first], x[..., second] = a * c - b * s, a * s + b * c
+    return x
+
+
+def rope(positions, rot, theta=1e4):
+    inv = theta ** (-2.0 * np.arange(rot // 2) / rot)
+    ang = np.asarray(positions, np.float64)[:, None] * inv[None]
+    return np.stack((np.cos(ang), np.sin(ang)), -1).astype(np.float32)
+
+
+def i32(x):
+    return torch.tensor(np.asarray(x, np.int32), device=DEV)
+
+
+WRITES = [  # heads, kv heads, head size, rot, adjacent, page size, v_dim, planes
+    (4, 2, 16, 16, False, 4, None, 2), (3, 1, 32, 32, True, 16, None, 2), (5, 5, 48, 16, False, 5, None, 2),
+    (7, 1, 128, 128, False, 16, None, 2), (2, 2, 64, 0, False, 1, None, 2), (4, 2, 64, 12, False, 16, None, 2),
+    (4, 2, 64, 10, True, 8, None, 2), (2, 1, 256, 256, False, 16, None, 2), (2, 2, 32, 32, False, 7, 48, 2),
+    (4, 1, 64, 64, False, 16, None, 1),
+]
+
+
+def write_case(ops, dtype, heads, kv_heads, hd, rot, adjacent, ps, v_dim, planes, qkv, positions, slots, pending=None, write_kv=True,
+               qkv_dev=None):
+    """Runs rope_kv_write on an empty cache of two requests; the cache, q and the pool it must have left."""
+    cache = Cache(ops, [40, 23], kv_heads, hd, ps, v_dim, planes, fill=False)
+    want = cache.pool.cpu().numpy().copy()
+    n = len(positions)
+    tab = rope(positions, rot) if rot else None
+    q = torch.full((n, heads * hd), 7.0, dtype=dtype, device=DEV)
+    ops.rope_kv_write(qkv_dev if qkv_dev is not None else torch.from_numpy(qkv).to(DEV), None if tab is None else torch.from_numpy(tab).to(DEV),
+                      i32(positions), i32(slots), q, cache.view, heads, rot, adjacent, write_kv=write_kv, pending=pending)
+    qd, kd = heads * hd, kv_heads * hd
+    x = rotated(qkv[:, :qd + kd].reshape(n, heads + kv_heads, hd), tab, rot, adjacent)
+    k, v = x[:, heads:], qkv[:, qd + kd:].reshape(n, -1, cache.v_dim) if planes == 2 else None
+    if write_kv:
+        for t in range(n):
+            for h in range(kv_heads):
+                q4.store_row(want, cache.table, slots[t], positions[t], 1, h, ps, hd, cache.v_dim, planes, k[t, h], None if v is None else v[t, h])
+    return cache, q, x[:, :heads].reshape(n, -1), want
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd,rot,adjacent,ps,v_dim,planes", WRITES)
+def test_write(ops, dtype, heads, kv_heads, hd, rot, adjacent, ps, v_dim, planes):
+    positions, slots = [0, 1, 2, 3, 4, 5, 16, 39, 0, 21, 22], [0] * 8 + [1] * 3
+    width = (heads + kv_heads) * hd + (kv_heads * (v_dim or hd) if planes == 2 else 0)
+    qkv = (np.random.default_rng(3).standard_normal((len(positions), width)) * 2).astype(np.float32)
+    cache, q, want_q, want = write_case(ops, dtype, heads, kv_heads, hd, rot, adjacent, ps, v_dim, planes, qkv, positions, slots)
+    got = cache.pool.cpu().numpy()
+    assert (got == want).all(), f"{(got != want).sum()} bytes of the pool differ"
+    err = np.abs(q.double().cpu().numpy() - want_q.astype(np.float64))
+    assert (err <= HALF[dtype] * np.abs(want_q) + 1e-45).all()      # q is rounded once from the same 32-bit numbers
+    cache, q, _, want = write_case(ops, dtype, heads, kv_heads, hd, rot, adjacent, ps, v_dim, planes, qkv, positions, slots, write_kv=False)
+    assert (cache.pool.cpu().numpy() == 0xFF).all()
+
+
+def test_write_of_numbers_that_quantise_badly(ops):
+    """Groups of zeros, of subnormals, below the smallest step, at its border, over the largest, not finite."""
+    rows = np.zeros((12, 48), np.float32)
+    rows[1] = 1e-42
+    rows[2] = 3.0e-6                              # less than half the smallest step: zero
+    rows[3] = 4.0e-6
+    rows[4, 5], rows[4, 20], rows[4, 40] = np.inf, np.nan, -np.inf
+    rows[4, 6] = 1.0
+    rows[5] = 6e4                                 # saturates
+    rows[6] = -3e38
+    rows[7] = np.float32(2.0 ** -14 * 7.5)        # where subnormal steps end
+    rows[8] = np.nextafter(np.float32(2.0 ** -14 * 7.5), np.float32(1))
+    rows[9] = np.repeat([7.5, 15.0, 60.0], 16)    # the step is a power of two, the largest exactly 7.5 steps: held as 7
+    rows[10] = np.tile([0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 7.0, 7.5], 6)   # halves of a step: to even
+    rows[11, ::16], rows[11, 1::16] = 1e-3, -0.0
+    qkv = np.concatenate([np.ones((12, 48), np.float32), rows, rows[::-1]], 1)
+    positions = list(range(12))
+    cache, _, _, want = write_case(ops, torch.float32, 1, 1, 48, 0, False, 16, None, 2, qkv, positions, [0] * 12)
+    assert (cache.pool.cpu().numpy() == want).all()
+    keys = torch.empty(12, 1, 48, device=DEV)
+    ops.kv_read(cache.view, i32([[0], [0], [12], [0]]), keys)
+    got = keys[:, 0].double().cpu().numpy()
+    assert np.isnan(got[4]).all() and (got[:3] == 0).all() and (got[5] == 53760).all() and (got[6] == -53760).all()
+    assert (got[10, :8] == [0, 2, 2, 0, -2, -2, 7, 7]).all()
+
+
+@pytest.mark.parametrize("splits", [1, 3, 9])
+@pytest.mark.parametrize("hd,rot", [(64, 64), (48, 12)])
+def test_write_folds_partial_sums(ops, splits, hd, rot):
+    """The q/k/v product may still lie in scratch as partial sums (slabs of 128 columns)."""
+    from axon_b200.kernels import fast
+    heads, kv_heads, n, ntok = 4, 2, 5, 16
+    width = (heads + 2 * kv_heads) * hd
+    cols = -(-width // 128)
+    rng = np.random.default_rng(5)
+    part = rng.standard_normal((cols, splits, ntok, 128)).astype(np.float32)
+    bias = rng.standard_normal(width).astype(np.float32)
+    full = np.zeros((n, cols * 128), np.float32)
+    for s in range(splits):
+        full += part[:, s, :n].transpose(1, 0, 2).reshape(n, -1)
+    qkv = full[:, :width] + bias
+    out = torch.zeros(n, width, device=DEV)
+    owed = fast.PendingFold(torch.from_numpy(part).to(DEV), splits, ntok, torch.from_numpy(bias).to(DEV), out, False)
+    cache, _, _, want = write_case(ops, torch.bfloat16, heads, kv_heads, hd, rot, False, 16, None, 2, qkv, [0, 1, 2, 17, 39], [0] * 5,
+                                   pending=owed, qkv_dev=out)
+    assert owed.claimed and (cache.pool.cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv_heads,hd,ps,v_dim,planes", [(2, 16, 4, None, 2), (1, 64, 1, None, 2), (4, 128, 16, None, 2), (3, 48, 7, 32, 2),
+                                                         (2, 32, 16, None, 1), (2, 256, 32, None, 2)])
+def test_read(ops, dtype, kv_heads, hd, ps, v_dim, planes):
+    cache = Cache(ops, [70, 1, 33], kv_heads, hd, ps, v_dim, planes, seed=4)
+    # parts of requests in no order, an empty one, rows between them that belong to none, two rows asked for twice
+    spans = [(2, 5, 28, 0), (0, 0, 70, 30), (1, 0, 1, 101), (0, 3, 0, 103), (2, 32, 1, 104), (0, 60, 4, 98)]
+    rows = 110
+    keys = torch.full((rows, kv_heads, hd), -5.0, dtype=dtype, device=DEV)
+    vals = torch.full((rows, kv_heads, cache.v_dim), -5.0, dtype=dtype, device=DEV)
+    ops.kv_read(cache.view, i32(spans).T.contiguous(), keys, vals)
+    want_k, want_v = np.full(keys.shape, -5.0), np.full(vals.shape, -5.0)
+    for slot, first, count, out in reversed(spans):
+        want_k[out:out + count], want_v[out:out + count] = cache.k[slot][first:first + count], cache.v[slot][first:first + count]
+    assert (keys.double().cpu().numpy() == want_k).all() and (vals.double().cpu().numpy() == want_v).all()
+    only = torch.full_like(vals, -5.0)
+    ops.kv_read(cache.view, i32(spans).T.contiguous(), None, only)
+    assert torch.equal(only, vals)
+
+
+def test_read_leaves_what_lies_outside_the_table(ops):
+    cache = Cache(ops, [20, 9], 2, 64, 16, seed=6)
+    keys = torch.full((40, 2, 64), -5.0, device=DEV)
+    # a slot too many, a negative one, a negative position, positions past the table's end
+    ops.kv_read(cache.view, i32([[2, -1, 0, 0], [0, 0, -3, 18], [5, 5, 5, 20], [0, 5, 10, 15]]), keys)
+    got = keys.double().cpu().numpy()
+    assert (got[:13] == -5).all() and (got[13:15] == cache.k[0][:2]).all() and (got[15:17] == cache.k[0][18:20]).all()
+    assert (got[15 + 14:] == -5).all(), "positions beyond the block table were read"
+
+
+def test_refusals(ops):
+    from axon_b200.kernels.lib import KernelError
+    cache = Cache(ops, [20], 2, 64, 16)
+    keys, spans = torch.zeros(4, 2, 64, device=DEV), i32([[0], [0], [4], [0]])
+    for bad, what in (((spans.long(), keys), "int32 spans"), ((spans[:3].contiguous(), keys), "spans"), ((spans, keys[:, :1].contiguous()), "keys as"),
+                      ((spans, None), "both"), ((spans, keys, torch.zeros(3, 2, 64, device=DEV)), "values as")):
+        with pytest.raises(ValueError, match=what):
+            ops.kv_read(cache.view, *bad)
+    with pytest.raises(TypeError, match="one dtype"):
+        ops.kv_read(cache.view, spans, keys, keys.to(torch.bfloat16))
+    with pytest.raises(TypeError, match="float16"):
+        ops.kv_read(cache.view, spans, keys.half())
+    with pytest.raises(ValueError, match="contiguous CUDA"):
+        ops.kv_read(cache.view, spans, torch.zeros(4, 2, 128, device=DEV)[..., :64])
+    plain = ops.KvView(torch.zeros(3, 1, 2, 2, 16, 64, device=DEV), cache.dev_table, 0, 16, 2, 64)
+    with pytest.raises(ValueError, match="quantised rows"):
+        ops.kv_read(plain, spans, keys)
+    qkv, pos = torch.zeros(4, 8 * 64, device=DEV), i32([0, 1, 2, 3])
+    q = torch.zeros(4, 4 * 64, device=DEV)
+    with pytest.raises(ValueError, match="for each row"):
+        ops.rope_kv_write(qkv, None, pos[:3].contiguous(), pos, q, cache.view, 4, 0)
+    with pytest.raises(ValueError, match="for each row"):
+        ops.rope_kv_write(qkv, None, pos, pos, q[:, :64].contiguous(), cache.view, 4, 0)
+    with pytest.raises(TypeError, match="int32"):
+        ops.rope_kv_write(qkv, None, pos.long(), pos, q, cache.view, 4, 0)
+    with pytest.raises(TypeError, match="float16"):
+        ops.rope_kv_write(qkv, None, pos, pos, q.half(), cache.view, 4, 0)
+    with pytest.raises(ValueError, match="rotation table"):
+        ops.rope_kv_write(qkv, torch.zeros(4, 16, 2, device=DEV), pos, pos, q, cache.view, 4, 64)
+    with pytest.raises(KernelError, match="rotated size"):
+        ops.rope_kv_write(qkv, torch.zeros(4, 64, 2, device=DEV), pos, pos, q, cache.view, 4, 128)
+    with pytest.raises(ValueError, match="queries"):
+        ops.attention_plain(q, cache.view, pos, pos, q[:, :64].contiguous(), 4, 0.1)
+    with pytest.raises(KernelError, match="over 2 kv heads"):
+        ops.attention_plain(torch.zeros(4, 3 * 64, device=DEV), cache.view, pos, pos, torch.zeros(4, 3 * 64, device=DEV), 3, 0.1)
+
+
+# -- attention --------------------------------------------------------------
+
+def attend(ops, cache, q_lens, heads, dtype, window=0, seed=9, scale=None, rt=None, precise=None, q=None):
+    """linear.attention for the last ``q_lens[s]`` tokens of each request; (out, context, q)."""
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import Runtime, StepContext
+    hd, vd = cache.hd, cache.v_dim
+    n = sum(q_lens)
+    if q is None:
+        q = (torch.randn(n, heads * hd, generator=torch.Generator().manual_seed(seed)) * 1.5).to(dtype).to(DEV)
+    starts = [sum(q_lens[:i]) for i in range(len(q_lens))]
+    pos = [p for l, k in zip(cache.lens, q_lens) for p in range(l - k, l)]
+    slot = [s for s, k in enumerate(q_lens) for _ in range(k)]
+    live = [s for s, k in enumerate(q_lens) if k]
+    seg = [live, [starts[s] for s in live], [q_lens[s] for s in live], [cache.lens[s] for s in live]]
+    rt = rt or Runtime(dtype, DEV, kv_bits=4)
+    ctx = StepContext(rt=rt, n_tokens=n, tokens=None, positions=i32(pos), token_slot=i32(slot), seg_slot=seg[0], seg_q_start=seg[1],
+                      seg_q_len=seg[2], seg_kv_len=seg[3], segments=i32(seg),
+                      unit_items=i32([[i, 0] for i in range(len(live))]) if all(k == 1 for k in seg[2]) else None)
+    out = torch.full((n + 2, heads * vd), -7.0, dtype=dtype, device=DEV)
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    linear.attention(q, cache.view, ctx, out[:n], heads, scale, precise=dtype == torch.float32 if precise is None else precise)
+    assert (out[n:] == -7.0).all(), "rows behind the last token were written"
+    return out[:n], ctx, q, pos, slot, scale
+
+
+def check_attention(ops, cache, q_lens, heads, dtype, window=0, weight_half=2.0 ** -11, **kw):
+    """Against float64, within a bound worked out for each number: a score is a sum of hd products in
+    32 bits (2^-23 a step: tensor cores cut sums), scaled (2^-22 of its size with the exponential's own error),
+    a weight is rounded to half its step (``weight_half``; none in the 32-bit model), sums over keys and the
+    output round again."""
+    out, ctx, q, pos, slot, scale = attend(ops, cache, q_lens, heads, dtype, window, **kw)
+    got = out.double().cpu().numpy().reshape(len(pos), heads, -1)
+    qd = q.double().cpu().numpy().reshape(len(pos), heads, -1)
+    group = heads // cache.kv_heads
+    pos, slot = np.array(pos), np.array(slot)
+    weight = 0.0 if dtype == torch.float32 else weight_half
+    for s in set(slot.tolist()):
+        rows = np.nonzero(slot == s)[0]
+        for h in range(heads):
+            want, mass, size = q4.attention(qd[rows, h], cache.k[s][:, h // group], cache.v[s][:, h // group], pos[rows], window, scale)
+            e_s = size * ((cache.hd + 4) * 2.0 ** -23 + 2.0 ** -22)
+            tol = mass * (weight + 2 * e_s[:, None] + 2.0 ** -20 + (cache.lens[s] + 8) * 2.0 ** -23) + 1.01 * HALF[dtype] * np.abs(want) + 1e-30
+            err = np.abs(got[rows, h] - want)
+            assert (err <= tol).all(), f"request {s} head {h}: worst error {float((err / tol).max()):.2f} of its bound"
+    return out, ctx
+
+
+LAYOUTS = [  # heads, kv heads, head size, page size
+    (4, 2, 16, 4), (3, 1, 32, 16), (5, 5, 48, 5), (2, 1, 256, 16), (28, 4, 128, 16), (12, 2, 128, 32), (6, 2, 64, 16), (8, 8, 128, 8),
+    (9, 1, 64, 4), (20, 1, 128, 64), (40, 1, 128, 16), (6, 2, 128, 48), (4, 4, 64, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd,ps", LAYOUTS)
+@pytest.mark.parametrize("window", [0, 1, 37])
+def test_single_tokens(ops, dtype, heads, kv_heads, hd, ps, window):
+    cache = Cache(ops, [1, 2, 15, 16, 17, 33, 70, 130, 257], kv_heads, hd, ps, window=window, seed=11)
+    check_attention(ops, cache, [1] * 9, heads, dtype, window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd,ps", LAYOUTS)
+@pytest.mark.parametrize("window", [0, 19])
+def test_portions(ops, dtype, heads, kv_heads, hd, ps, window):
+    """Portions of one to a few dozen tokens beside requests that have none in this step."""
+    cache = Cache(ops, [2, 40, 5, 64, 81, 33], kv_heads, hd, ps, window=window, seed=12)
+    check_attention(ops, cache, [2, 3, 0, 9, 1, 33], heads, dtype, window, weight_half=2.0 ** -8)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,ps,lens", [(28, 4, 128, 16, [5003]), (12, 2, 128, 16, [4096, 1, 777]), (6, 2, 64, 32, [3000, 2999]),
+                                                       (5, 5, 48, 16, [2500, 3])])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_long_contexts_in_shares(ops, heads, kv_heads, hd, ps, lens, window):
+    cache = Cache(ops, lens, kv_heads, hd, ps, window=window, seed=13, loud=1.0)
+    check_attention(ops, cache, [1] * len(lens), heads, torch.bfloat16, window)
+    check_attention(ops, cache, [min(l, 4) for l in lens], heads, torch.bfloat16, window, weight_half=2.0 ** -8)
+    check_attention(ops, cache, [1] * len(lens), heads, torch.float32, window)
+
+
+def test_what_is_not_finite_stays_with_who_sees_it(ops):
+    """A NaN key or value is NaN for the tokens that see it and for no others, in every head's own channels."""
+    for hd, heads, kv_heads in ((128, 6, 2), (64, 4, 4)):
+        for bad_key in (True, False):
+            cache = Cache(ops, [50, 50], kv_heads, hd, 16, seed=14)
+            page, i = int(cache.table[0, 40 // 16]), 40 % 16
+            place = cache.places[1 if bad_key else 3]
+            cache.pool[page, 1, place[0] + i * place[1]] = 0xFF          # kv head 0, first group, position 40 of request 0
+            for k in (1, 4):
+                out = attend(ops, cache, [k, k], heads, torch.bfloat16)[0].view(2, k, heads, hd)
+                group = heads // kv_heads
+                assert torch.isfinite(out[1]).all() and torch.isfinite(out[0, :, group:]).all()
+                nan = torch.isnan(out[0, :, :group])
+                assert nan.all() if bad_key else nan[..., :16].all() and not nan[..., 16:].any()
+    # tokens before the bad one, in the same portion
+    cache = Cache(ops, [44], 2, 128, 16, seed=14)
+    page, i = int(cache.table[0, 40 // 16]), 40 % 16
+    for which in (1, 3):
+        cache.pool[page, 1, cache.places[which][0] + i * cache.places[which][1]] = 0xFF
+        out = attend(ops, cache, [8], 2, torch.bfloat16)[0].view(8, 2, 128)
+        assert torch.isfinite(out[:4]).all() and torch.isnan(out[4:, 0, :16]).all() and torch.isfinite(out[:, 1]).all()
+
+
+def test_large_queries_and_keys(ops):
+    """Scores far apart: one key takes all the weight; and queries that overflow half precision."""
+    cache = Cache(ops, [90], 1, 128, 16, seed=15, loud=30.0)
+    q = (torch.randn(1, 4 * 128, generator=torch.Generator().manual_seed(1)) * torch.tensor([1e-6, 1.0, 300.0, 2e5]).repeat_interleave(128)).to(torch.bfloat16).to(DEV)
+    check_attention(ops, cache, [1], 4, torch.bfloat16, q=q)
+    check_attention(ops, cache, [1], 4, torch.float32, q=q.float())
+    check_attention(ops, cache, [1], 4, torch.bfloat16, q=torch.zeros_like(q))
+
+
+def test_one_plane_and_wider_values(ops):
+    for v_dim, planes in ((None, 1), (96, 2), (16, 2)):
+        cache = Cache(ops, [37, 70], 2, 64, 16, v_dim, planes, seed=16)
+        if planes == 1:
+            cache.v = cache.k
+        for dtype in DTYPES:
+            check_attention(ops, cache, [1, 3], 6, dtype)
+
+
+def test_the_same_call_gives_the_same_bits(ops):
+    for q_lens, dtype in (([1, 1, 1], torch.bfloat16), ([5, 1, 40], torch.bfloat16), ([1, 1, 1], torch.float32)):
+        cache = Cache(ops, [1500, 40, 300], 2, 128, 16, seed=17)
+        first = attend(ops, cache, q_lens, 14, dtype)[0].clone()
+        for _ in range(3):
+            assert torch.equal(attend(ops, cache, q_lens, 14, dtype)[0], first)
+
+
+def test_on_another_stream_and_in_a_graph(ops):
+    """Launches go to the current stream; a captured write and attention replays on new inputs."""
+    from axon_b200.parts.base import Runtime
+    rt = Runtime(torch.bfloat16, DEV, kv_bits=4)
+    heads, kv_heads, hd = 14, 2, 128
+    cache = Cache(ops, [700, 33], kv_heads, hd, 16, seed=18)
+    qkv = torch.randn(2, (heads + 2 * kv_heads) * hd, device=DEV)
+    pos, slot, q = i32([699, 32]), i32([0, 1]), torch.empty(2, heads * hd, dtype=torch.bfloat16, device=DEV)
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import StepContext
+    ctx = StepContext(rt=rt, n_tokens=2, tokens=None, positions=pos, token_slot=slot, seg_slot=[0, 1], seg_q_start=[0, 1], seg_q_len=[1, 1],
+                      seg_kv_len=[700, 33], segments=i32([[0, 1], [0, 1], [1, 1], [700, 33]]), unit_items=i32([[0, 0], [1, 0]]))
+    out = torch.empty(2, heads * hd, dtype=torch.bfloat16, device=DEV)
+
+    def run():
+        ops.rope_kv_write(qkv, None, pos, slot, q, cache.view, heads, 0)
+        linear.attention(q, cache.view, ctx, out, heads, 0.1)
+
+    run()
+    eager = out.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out.zero_()
+        run()
+        on_side = out.clone()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(on_side, eager)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for k in range(3):
+        qkv.copy_(torch.randn_like(qkv))
+        graph.replay()
+        replayed = out.clone()
+        run()
+        assert torch.equal(replayed, out)
+
+
+# -- the engine -------------------------------------------------------------
+
+def engine_for(folder, dtype, **kw):
+    from axon_b200.engine.build import build_engine
+    kw.setdefault("max_slots", 8)
+    kw.setdefault("max_tokens", 512)
+    return build_engine(folder, dtype=dtype, kv="q4", **kw)
+
+
+def logits_over_cached(cfg, w, tokens, cached):
+    """Float64 logits of a whole sequence whose layers attend over the given keys and values: what the
+    engine must answer from the cache it has, whichever side of a rounding border each value fell on."""
+    import plain_qwen2 as plain
+    H, hd = cfg["num_attention_heads"], cfg["head_dim"]
+    x = plain.embed(w["model.embed_tokens.weight"], tokens)
+    fresh = []
+    for l in range(cfg["num_hidden_layers"]):
+        p = f"model.layers.{l}."
+        h = plain.rms_norm(x, w[p + "input_layernorm.weight"], cfg["rms_norm_eps"])
+        a = p + "self_attn."
+        q = plain.linear(h, w[a + "q_proj.weight"], w[a + "q_proj.bias"]).view(len(tokens), H, hd)
+        k = plain.linear(h, w[a + "k_proj.weight"], w[a + "k_proj.bias"]).view(len(tokens), -1, hd)
+        v = plain.linear(h, w[a + "v_proj.weight"], w[a + "v_proj.bias"]).view(len(tokens), -1, hd)
+        pos = list(range(len(tokens)))
+        fresh.append((plain.rope_half(k, pos, cfg["rope_theta"]), v))
+        o = plain.causal_gqa_attention(plain.rope_half(q, pos, cfg["rope_theta"]), *cached[l])
+        x = x + plain.linear(o.reshape(len(tokens), H * hd), w[a + "o_proj.weight"])
+        h = plain.rms_norm(x, w[p + "post_attention_layernorm.weight"], cfg["rms_norm_eps"])
+        x = x + plain.swiglu_ffn(h, w[p + "mlp.gate_proj.weight"], w[p + "mlp.up_proj.weight"], w[p + "mlp.down_proj.weight"])
+    h = plain.rms_norm(x, w["model.norm.weight"], cfg["rms_norm_eps"])
+    head = w["model.embed_tokens.weight"] if cfg["tie_word_embeddings"] else w["lm_head.weight"]
+    return plain.linear(h, head), fresh
+
+
+#: of the largest logit: the engine's own tolerances (float rounding; activations of 8 bits between kernels)
+ENGINE_TOL = {"float32": 2e-5, "bfloat16": 3e-2}
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["A", "B", "C", "D"])
+@pytest.mark.parametrize("sizes", [[200], [5, 30, 3, 17, 2, 1, 33], [40, 1, 1, 1, 1, 1, 1, 1]])
+def test_engine(model_folders, name, dtype, sizes):
+    """Prompts whole, in portions and token by token: the logits of every place against float64 over the same
+    cache, and the cache against the float64 keys and values it was quantised from."""
+    import plain_qwen2 as plain
+    from axon_b200.engine.step import StepEntry
+    from test_engine_gpu import tokens_for
+    cfg, w = plain.read_model(model_folders[name])
+    engine = engine_for(model_folders[name], dtype, page_size=16, shuffle_seed=5)
+    lens = [1, 37, 100]
+    toks = [tokens_for(name, i, n) for i, n in enumerate(lens)]
+    slots = [engine.open_request() for _ in lens]
+    got = [[] for _ in lens]
+    fed, k = [0] * len(lens), 0
+    while any(f < n for f, n in zip(fed, lens)):
+        entries, who = [], []
+        for i, n in enumerate(lens):
+            size = min(sizes[(k + i) % len(sizes)], n - fed[i])
+            if size > 0:
+                entries.append(StepEntry(slots[i], toks[i][fed[i]:fed[i] + size], range(size)))
+                who.append((i, size))
+                fed[i] += size
+        rows = engine.step(entries).double().cpu()
+        for i, size in who:
+            got[i].append(rows[:size])
+            rows = rows[size:]
+        k += 1
+    for i, n in enumerate(lens):
+        cached = [tuple(t.double().cpu() for t in engine.cache.read(slots[i], l)) for l in range(cfg["num_hidden_layers"])]
+        want, fresh = logits_over_cached(cfg, w, toks[i], cached)
+        scale = float(want.abs().max())
+        err = float((torch.cat(got[i]) - want).abs().max())
+        assert err <= ENGINE_TOL[dtype] * scale, f"request {i}: {err / scale:.2e} of the largest logit"
+        for (k_c, v_c), (k_f, v_f) in zip(cached, fresh):
+            for c, f in ((k_c, k_f), (v_c, v_f)):
+                groups = f.unflatten(-1, (-1, 16))
+                # half a step of the group (at most 9/8 of its largest value over 7.5), and what the model's dtype moves the value by
+                room = groups.abs().amax(-1, keepdim=True) * (1.125 / 7.5 / 2) * (1 + 2 * ENGINE_TOL[dtype]) + ENGINE_TOL[dtype] * float(f.abs().max())
+                assert ((c.unflatten(-1, (-1, 16)) - groups).abs() <= room + 2.0 ** -18).all()
+    engine.check_device()
+    engine.cache.manager.check()
+
+
+def test_serving_with_a_quantised_cache(model_folders):
+    """Through the front door: more requests than slots and few pages (preemption), replayed graphs; alone or in a crowd a request's
+    greedy tokens come from the same numbers."""
+    import axon_b200 as axon
+    from test_engine_gpu import tokens_for
+    prompts = [tokens_for("C", i, 10 + 23 * i) for i in range(6)]
+    opts = axon.BackendOptions().max_ctx(256).kv("q4").dtype("float32").kv_tokens(320).parallel(3)
+    net = axon.Backend(axon.load(model_folders["C"]), opts)
+    outs = net.generate_batch(prompts, 24)
+    alone = axon.Backend(axon.load(model_folders["C"]), axon.BackendOptions().max_ctx(256).kv("q4").dtype("float32").parallel(1))
+    for p, o in zip(prompts, outs):
+        assert len(o) == 24
+        with alone.new_cache() as cache:
+            logits = alone.prefill_logits(p, 0, cache)
+            assert axon.generate(alone, cache, p, logits, axon.GenOpts.greedy(24)).ids == o
+    full = axon.Backend(axon.load(model_folders["C"]), axon.BackendOptions().max_ctx(256).dtype("float32"))
+    assert net.engine.cache.bytes_per_token() * 64 == full.engine.cache.bytes_per_token() * 9
+
+
+def test_reading_what_a_request_holds(model_folders):
+    from axon_b200.engine.build import build_engine
+    from axon_b200.engine.step import StepEntry
+    from test_engine_gpu import tokens_for
+    toks = tokens_for("B", 0, 50)
+    held = []
+    for kv in ("auto", "q4"):
+        e = build_engine(model_folders["B"], dtype="float32", kv=kv, max_slots=2, max_tokens=256, max_positions=128, page_size=8, shuffle_seed=2)
+        s = e.open_request()
+        e.step([StepEntry(s, toks, [])])
+        held.append(e.cache.read(s, 1))
+        k, v = e.cache.read(s, 1, first=7, count=20)
+        assert torch.equal(k, held[-1][0][7:27]) and torch.equal(v, held[-1][1][7:27])
+        for first, count in ((0, 51), (-1, 3), (50, 1)):
+            with pytest.raises(ValueError, match="holds positions"):
+                e.cache.read(s, 1, first=first, count=count)
+        with pytest.raises(ValueError, match="not open"):
+            e.cache.read(1 - s, 1)
+    assert held[0][0].shape == held[1][0].shape and held[1][0].dtype == torch.float32
+    # of layer 0 the two engines quantise the same numbers; of layer 1 the keys have moved by what layer 0's rounding did
+    assert float((held[0][0] - held[1][0]).abs().max()) < float(held[0][0].abs().max())
