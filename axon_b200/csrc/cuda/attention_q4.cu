@@ -19,16 +19,23 @@
 // A warp works alone: its own ring of shared memory, filled by bulk copies (one per 16-position page
 // and kv head: codes and steps of keys and values lie together) that one mbarrier per stage counts, its own running
 // maximum and sum.  The maximum lags: O is rescaled only when a score exceeds it by 2^8.  The warps of a CTA take
-// chunks of 32 keys in turn and are merged at the end; CTAs split a request's keys, and a second
-// kernel folds their shares in ascending order.
+// chunks of 32 keys in turn and are merged at the end.
+//
+// The grid is as many CTAs as fit at once, and the 16-key tiles of all (item, kv head) pairs, laid
+// end to end, are cut into one equal range for each: contexts of any lengths load the GPU evenly, and
+// nothing of the launch depends on them.  A CTA works through the pairs of its range; a pair that lies in one
+// range whole is written out, the pieces of the others go to scratch (at most two per CTA: the one
+// its range begins in and the one it ends in) and a second kernel folds them in ascending order.
 #include "kv_q4.cuh"
 #include "tcgen05.cuh"
+
+#include <type_traits>
 
 namespace axon {
 
 constexpr int QA_WARPS = 8, QA_THREADS = QA_WARPS * 32;
 constexpr int QA_KT = 2, QA_STAGES = 3;          // 16-key tiles per chunk, chunks in a warp's ring
-constexpr int QA_MAX_SPLITS = 64;
+constexpr int QA_LEAST = QA_WARPS * QA_KT;       // tiles below which a range is not cut further: one chunk for each warp
 constexpr float QA_LAZY = 8.f;                   // log2 units a score may exceed the running maximum
 
 struct QaParams {
@@ -37,10 +44,10 @@ struct QaParams {
     __nv_bfloat16* out;
     const int32_t* segments;     // [4][n_segments]: slot, q_start, q_len, kv_len
     const int32_t* items;        // [n_items][2]: segment, first row (token * group + head of the group); null: segment i, row 0
-    float* part_o;               // [item][kv head][split][row][HD], with several splits
+    float* part_o;               // [2 * CTA + (0: the pair its range begins in, 1: the one it ends in)][row][HD]
     float2* part_ml;             // the same without the last index: maximum (log2 units) and sum
     PagedQ4 kv;
-    int n_segments, heads, group, n_splits, window;
+    int n_segments, n_items, heads, group, ctas, window;
     int run;                     // positions of a tile that lie together in a page: gcd(page size, 16)
     float scale_log2;
 };
@@ -85,22 +92,37 @@ __device__ __forceinline__ uint32_t qa_mul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Two step bytes (in the low byte of each half) with the two addends that take 8 away from a code.
+// (w & mask) | magic in one instruction: with both as constants the compiler takes two, as an instruction holds one.
+__device__ __forceinline__ uint32_t qa_pick(uint32_t w, uint32_t mask, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+    return r;
+}
+// The exponents under which a code in bits 0-3 (8 + c / 128) and one in bits 4-7 (0.5 + c / 128) are read, in
+// registers the compiler cannot see through.
+struct QaMagic {
+    uint32_t low, high;
+    __device__ __forceinline__ QaMagic() {
+        asm volatile("mov.b32 %0, 0x48004800;" : "=r"(low));
+        asm volatile("mov.b32 %0, 0x38003800;" : "=r"(high));
+    }
+};
+// Two steps (their bytes << 7, one in each half) with the two addends that take 8 away from a code.
 struct QaStep {
     uint32_t s, low, high;       // the steps; -8.0625 s for nibbles in bits 0-3; -0.5625 s for nibbles in bits 4-7
     __device__ __forceinline__ explicit QaStep(uint32_t two) {
-        s = two << 7;
+        s = two;
         low = qa_mul2(s, 0xC808C808u);
         high = qa_mul2(s, 0xB880B880u);
     }
 };
 // The codes in bits 0-3, 4-7, 8-11 and 12-15 of both halves of w, times their steps / 128.
-__device__ __forceinline__ void qa_widen(uint32_t (&p)[4], uint32_t w, const QaStep& st) {
+__device__ __forceinline__ void qa_widen(uint32_t (&p)[4], uint32_t w, const QaStep& st, const QaMagic& magic) {
     const uint32_t v = w >> 8;
-    p[0] = qa_fma2((w & 0x000F000Fu) | 0x48004800u, st.s, st.low);
-    p[1] = qa_fma2((w & 0x00F000F0u) | 0x38003800u, st.s, st.high);
-    p[2] = qa_fma2((v & 0x000F000Fu) | 0x48004800u, st.s, st.low);
-    p[3] = qa_fma2((v & 0x00F000F0u) | 0x38003800u, st.s, st.high);
+    p[0] = qa_fma2(qa_pick(w, 0x000F000Fu, magic.low), st.s, st.low);
+    p[1] = qa_fma2(qa_pick(w, 0x00F000F0u, magic.high), st.s, st.high);
+    p[2] = qa_fma2(qa_pick(v, 0x000F000Fu, magic.low), st.s, st.low);
+    p[3] = qa_fma2(qa_pick(v, 0x00F000F0u, magic.high), st.s, st.high);
 }
 template <int N> __device__ __forceinline__ void qa_lds(uint32_t (&r)[N], const uint8_t* p) {
     if constexpr (N % 4 == 0) {
@@ -153,6 +175,65 @@ __device__ __forceinline__ float qa_load_query(uint32_t (&f)[HD / 16][2], const 
     return __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
+// An item's rows and the keys they see.
+struct QaItem {
+    int slot, q_start, row0, rows, pos0, pos_first, pos_last, kv_lo, kv_hi, tile0, tiles;
+    __device__ __forceinline__ QaItem(const QaParams& p, int item, int most_rows) {
+        const int seg = p.items ? p.items[2 * item] : item;
+        row0 = p.items ? p.items[2 * item + 1] : 0;
+        slot = p.segments[seg];
+        q_start = p.segments[p.n_segments + seg];
+        const int q_len = p.segments[2 * p.n_segments + seg], kv_len = p.segments[3 * p.n_segments + seg];
+        rows = min(most_rows, q_len * p.group - row0);
+        pos0 = kv_len - q_len;
+        pos_first = pos0 + row0 / p.group;
+        pos_last = pos0 + (row0 + rows - 1) / p.group;
+        kv_hi = pos_last + 1;
+        kv_lo = (p.window > 0 && pos_first - p.window + 1 > 0) ? pos_first - p.window + 1 : 0;
+        tile0 = kv_lo / 16;
+        tiles = rows > 0 ? max((kv_hi + 15) / 16 - tile0, 0) : 0;
+    }
+};
+// How the tiles of all pairs, laid end to end (items in order, the kv heads of each in order), fall to the
+// CTAs: `per` each.  Every warp works it out for itself, 32 items at a time.  (The launcher has seen to it that a full
+// block table counts in 32 bits.)
+struct QaRanges {
+    uint32_t total, per;
+    __device__ __forceinline__ QaRanges(const QaParams& p, int most_rows) {
+        total = before(p, p.n_items, most_rows);
+        per = max((uint32_t)QA_LEAST, (total + p.ctas - 1) / p.ctas);
+    }
+    // tiles of all pairs before `item`
+    static __device__ __forceinline__ uint32_t before(const QaParams& p, int item, int most_rows) {
+        uint32_t sum = 0;
+        for (int i = threadIdx.x & 31; i < item; i += 32) sum += QaItem(p, i, most_rows).tiles;
+        return __reduce_add_sync(0xffffffffu, sum) * p.kv.kv_heads;
+    }
+    // the item that tile f falls into, and the tiles before it
+    static __device__ __forceinline__ int find(const QaParams& p, uint32_t f, int most_rows, uint32_t* start) {
+        const int lane = threadIdx.x & 31;
+        uint32_t base = 0;
+        for (int i0 = 0; i0 < p.n_items; i0 += 32) {
+            const uint32_t n = i0 + lane < p.n_items ? QaItem(p, i0 + lane, most_rows).tiles * p.kv.kv_heads : 0;
+            uint32_t upto = n;                                     // of this item and those before it in the 32
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t x = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, base + upto > f);
+            if (past) {
+                const int who = __ffs(past) - 1;
+                *start = base + __shfl_sync(0xffffffffu, upto - n, who);
+                return i0 + who;
+            }
+            base += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        *start = base;
+        return p.n_items;
+    }
+};
+
 template <int HD, int NT>
 __global__ void __launch_bounds__(QA_THREADS, (NT == 1 && HD <= 128) ? 2 : 1)
 attention_q4_kernel(const QaParams p) {
@@ -174,19 +255,30 @@ attention_q4_kernel(const QaParams p) {
     __syncwarp();
     pdl_wait();
 
-    const int item = blockIdx.x, kvh = blockIdx.y, split = blockIdx.z;
-    const int seg = p.items ? p.items[2 * item] : item, row0 = p.items ? p.items[2 * item + 1] : 0;
-    const int slot = p.segments[seg], q_start = p.segments[p.n_segments + seg];
-    const int q_len = p.segments[2 * p.n_segments + seg], kv_len = p.segments[3 * p.n_segments + seg];
-    const int rows = min(8 * NT, q_len * p.group - row0);
-    const int pos_first = kv_len - q_len + row0 / p.group, pos_last = kv_len - q_len + (row0 + rows - 1) / p.group;
-    const int kv_hi = pos_last + 1, kv_lo = (p.window > 0 && pos_first - p.window + 1 > 0) ? pos_first - p.window + 1 : 0;
-    int tile0, tile1;
+    constexpr int R = 8 * NT;
+    uint32_t f, f1, start;
+    int item;
     {
-        const int first = kv_lo / 16, n = (kv_hi + 15) / 16 - first, per = (n + p.n_splits - 1) / p.n_splits;
-        tile0 = first + split * per;
-        tile1 = min(first + n, tile0 + per);
+        const QaRanges all(p, R);
+        if (blockIdx.x > (all.total - 1) / all.per || all.total == 0) return;
+        f = blockIdx.x * all.per;
+        f1 = f + min(all.per, all.total - f);
+        item = QaRanges::find(p, f, R, &start);
     }
+    const uint32_t f_begin = f;
+    const QaMagic magic;
+    int at = 0;                                                    // the stage of the warp's ring that it reads next,
+    uint32_t phase = 0;                                            // and its barrier's phase
+    while (f < f1) {
+    const QaItem it(p, item, R);
+    if (it.tiles == 0) {                                           // (an empty segment: nothing to read or to write)
+        if (++item >= p.n_items) return;
+        continue;
+    }
+    const int kvh = (int)((f - start) / it.tiles), off = (int)((f - start) % it.tiles);
+    const int rows = it.rows, pos_first = it.pos_first, pos_last = it.pos_last, row0 = it.row0, q_start = it.q_start;
+    const int kv_lo = it.kv_lo, kv_hi = it.kv_hi;
+    const int tile0 = it.tile0 + off, tile1 = tile0 + (int)min((uint32_t)(it.tiles - off), f1 - f);
 
     // ---- copies.  A lane owns one piece of a chunk: with pages of 16 positions a whole tile, else a run of
     // one of its four parts.
@@ -198,7 +290,7 @@ attention_q4_kernel(const QaParams p) {
     const uint32_t my_dst = my_tile * T::BYTES + (whole ? 0 : (part & 1 ? T::KC : 0) + (part & 2 ? T::KC + T::KS : 0) + key_off * row_bytes);
     const uint8_t* const my_src = p.pool + p.kv.entry_offset + (long long)kvh * p.kv.record +
         (whole || part == 0 ? 0 : part == 1 ? p.kv.k_steps : part == 2 ? p.kv.v_codes : p.kv.v_steps);
-    const int32_t* const table = p.kv.block_table + (long long)slot * p.kv.table_stride;
+    const int32_t* const table = p.kv.block_table + (long long)it.slot * p.kv.table_stride;
     const int last_page = (kv_hi - 1) / p.kv.page_size;
     auto chunk_tile = [&](int j) { return tile0 + (warp + j * QA_WARPS) * QA_KT; };
     auto my_page = [&](int j) {                                   // the table entry of this lane's piece of its warp's j-th chunk
@@ -206,15 +298,15 @@ attention_q4_kernel(const QaParams p) {
         if (my_tile >= QA_KT || tile >= tile1) return 0;
         return (int)table[whole ? tile : min((tile * 16 + key_off) / p.kv.page_size, last_page)];
     };
-    auto request = [&](int j, int entry) {
+    auto request = [&](int j, int entry, int stage) {
         const int first = chunk_tile(j), n = min(QA_KT, tile1 - first);
         if (n <= 0) return;
-        const uint32_t bar = bars + 8 * (j % QA_STAGES);
+        const uint32_t bar = bars + 8 * stage;
         if (lane == 0) mbar_expect_tx(bar, n * T::BYTES);
         __syncwarp();
         if (my_tile < n) {
             const int in_page = whole ? 0 : ((first + my_tile) * 16 + key_off) % p.kv.page_size;
-            qa_bulk_load(ring_addr + (j % QA_STAGES) * (QA_KT * T::BYTES) + my_dst,
+            qa_bulk_load(ring_addr + stage * (QA_KT * T::BYTES) + my_dst,
                          my_src + (long long)p.kv.page(entry) * p.kv.page_stride + (long long)in_page * row_bytes, my_bytes, bar);
         }
     };
@@ -225,7 +317,7 @@ attention_q4_kernel(const QaParams p) {
         for (int j = 0; j < QA_STAGES; ++j) e[j] = my_page(j);
         next_entry = my_page(QA_STAGES);
 #pragma unroll
-        for (int j = 0; j < QA_STAGES; ++j) request(j, e[j]);
+        for (int j = 0; j < QA_STAGES; ++j) request(j, e[j], at + j < QA_STAGES ? at + j : at + j - QA_STAGES);
     }
 
     // ---- queries as B fragments, and the factor that brings a row's scores to log2 units
@@ -266,15 +358,11 @@ attention_q4_kernel(const QaParams p) {
         l[n][0] = l[n][1] = 0.f;
     }
     // the position of the query row in column c of row tile n (rows past the last: the last token's)
-    auto row_pos = [&](int n, int c) { return kv_len - q_len + (row0 + min(8 * n + 2 * t + c, rows - 1)) / p.group; };
+    auto row_pos = [&](int n, int c) { return it.pos0 + (row0 + min(8 * n + 2 * t + c, rows - 1)) / p.group; };
 
-    for (int j = 0;; ++j) {
-        const int first = chunk_tile(j), n_tiles = min(QA_KT, tile1 - first);
-        if (n_tiles <= 0) break;
-        const uint8_t* const stage = ring + (j % QA_STAGES) * (QA_KT * T::BYTES);
-        if (!mbar_wait(bars + 8 * (j % QA_STAGES), (j / QA_STAGES) & 1, 0))
-            mbar_wait(bars + 8 * (j % QA_STAGES), (j / QA_STAGES) & 1, 0);      // its copies must not outlive the CTA
-
+    // One chunk: EDGE when it may be short or hold keys that not every row sees.
+    auto chunk = [&](auto edge, int first, int n_tiles, const uint8_t* stage) {
+        constexpr bool EDGE = decltype(edge)::value;
         float s[QA_KT][NT][4];
         float top[NT][2];
 #pragma unroll
@@ -284,8 +372,8 @@ attention_q4_kernel(const QaParams p) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s[i][n][c] = i < n_tiles ? 0.f : -INFINITY;
-            if (i >= n_tiles) continue;
+                for (int c = 0; c < 4; ++c) s[i][n][c] = !EDGE || i < n_tiles ? 0.f : -INFINITY;
+            if (EDGE && i >= n_tiles) continue;
             const uint8_t* const tile = stage + i * T::BYTES;
             uint32_t wa[KW], wb[KW];                               // this thread's codes of keys g and g + 8
             qa_lds(wa, tile + g * (HD / 2) + t * (HD / 8));
@@ -293,10 +381,10 @@ attention_q4_kernel(const QaParams p) {
             const uint8_t* const st = tile + T::KC + g * (HD / 16) + t * KG;
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
-                const QaStep sa(st[w / 2] * 0x00010001u), sb(st[8 * (HD / 16) + w / 2] * 0x00010001u);
+                const QaStep sa(st[w / 2] * 0x00800080u), sb(st[8 * (HD / 16) + w / 2] * 0x00800080u);
                 uint32_t a[4], b[4];
-                qa_widen(a, wa[w], sa);
-                qa_widen(b, wb[w], sb);
+                qa_widen(a, wa[w], sa, magic);
+                qa_widen(b, wb[w], sb, magic);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     uint2 q0, q1;
@@ -307,12 +395,11 @@ attention_q4_kernel(const QaParams p) {
                 }
             }
             const int key0 = (first + i) * 16;
-            const bool partly = key0 + 15 > pos_first || (p.window > 0 && key0 <= pos_last - p.window);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) s[i][n][c] *= factor[n][c & 1];
-                if (partly) {
+                if (EDGE) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int key = key0 + g + (c >> 1) * 8, pos = row_pos(n, c & 1);
@@ -346,7 +433,7 @@ attention_q4_kernel(const QaParams p) {
         uint32_t pf[QA_KT][NT][2];                                 // weights as B fragments
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float m0 = m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.f : m[n][1];
+            const float m0 = EDGE && m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = EDGE && m[n][1] == -INFINITY ? 0.f : m[n][1];
 #pragma unroll
             for (int i = 0; i < QA_KT; ++i) {
                 const float p0 = qa_ex2(s[i][n][0] - m0), p1 = qa_ex2(s[i][n][1] - m1), p2 = qa_ex2(s[i][n][2] - m0), p3 = qa_ex2(s[i][n][3] - m1);
@@ -358,52 +445,49 @@ attention_q4_kernel(const QaParams p) {
         }
 #pragma unroll
         for (int i = 0; i < QA_KT; ++i) {
-            if (i >= n_tiles) continue;
+            if (EDGE && i >= n_tiles) continue;
             const uint8_t* const tile = stage + i * T::BYTES + T::KC + T::KS;
             const int key0 = (first + i) * 16;
-            const bool partly = key0 + 15 > pos_first || (p.window > 0 && key0 <= pos_last - p.window);
             uint32_t w4[4][VW];                                    // codes of keys 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
             for (int k = 0; k < 4; ++k) qa_lds(w4[k], tile + (2 * t + (k & 1) + (k >> 1) * 8) * (HD / 2) + g * (HD / 16));
-            uint32_t nan_keys[(VW + 1) / 2];
 #pragma unroll
-            for (int v = 0; v < VW; ++v) {
+            for (int u = 0; u < (VW + 1) / 2; ++u) {               // groups of 16 channels (of 8, the half of one, at head size 64)
                 uint32_t by[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) by[k] = tile[T::KC + (2 * t + (k & 1) + (k >> 1) * 8) * (HD / 16) + (g * (HD / 8) + 8 * v) / 16];
-                if (partly) {
+                for (int k = 0; k < 4; ++k) by[k] = tile[T::KC + (2 * t + (k & 1) + (k >> 1) * 8) * (HD / 16) + (g * (HD / 8)) / 16 + u];
+                uint32_t nan_keys = 0;
+                if (EDGE) {
                     // keys that no row sees may hold anything, and a NaN that some rows see must not reach the others (0 * NaN
                     // is NaN): both count as zero here, and the rows that see a NaN get theirs below
-                    if (v % 2 == 0) nan_keys[v / 2] = 0;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        const int at = 2 * t + (k & 1) + (k >> 1) * 8;
-                        const bool in = key0 + at >= kv_lo && key0 + at < kv_hi;
-                        if (in && by[k] == Q4_NAN) nan_keys[v / 2] |= 1u << at;
+                        const int key = 2 * t + (k & 1) + (k >> 1) * 8;
+                        const bool in = key0 + key >= kv_lo && key0 + key < kv_hi;
+                        if (in && by[k] == Q4_NAN) nan_keys |= 1u << key;
                         if (!in || by[k] == Q4_NAN) by[k] = 0;
                     }
                 }
-                const QaStep s01(by[0] | by[1] << 16), s89(by[2] | by[3] << 16);
+                const QaStep s01(by[0] * 0x80u + by[1] * 0x800000u), s89(by[2] * 0x80u + by[3] * 0x800000u);
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {             // codes 0-3 and 4-7 of the words
-                    const uint32_t sel = half ? 0x7632u : 0x5410u;
-                    uint32_t a[4], b[4];
-                    qa_widen(a, __byte_perm(w4[0][v], w4[1][v], sel), s01);
-                    qa_widen(b, __byte_perm(w4[2][v], w4[3][v], sel), s89);
+                for (int v = 2 * u; v < VW && v < 2 * u + 2; ++v) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        qa_mma(o[4 * v + 2 * half][n], a[0], a[1], b[0], b[1], pf[i][n][0], pf[i][n][1]);
-                        qa_mma(o[4 * v + 2 * half + 1][n], a[2], a[3], b[2], b[3], pf[i][n][0], pf[i][n][1]);
+                    for (int half = 0; half < 2; ++half) {         // codes 0-3 and 4-7 of the words
+                        const uint32_t sel = half ? 0x7632u : 0x5410u;
+                        uint32_t a[4], b[4];
+                        qa_widen(a, __byte_perm(w4[0][v], w4[1][v], sel), s01, magic);
+                        qa_widen(b, __byte_perm(w4[2][v], w4[3][v], sel), s89, magic);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            qa_mma(o[4 * v + 2 * half][n], a[0], a[1], b[0], b[1], pf[i][n][0], pf[i][n][1]);
+                            qa_mma(o[4 * v + 2 * half + 1][n], a[2], a[3], b[2], b[3], pf[i][n][0], pf[i][n][1]);
+                        }
                     }
                 }
-            }
-            if (partly) {
-#pragma unroll
-                for (int v = 0; v < (VW + 1) / 2; ++v) {
-                    uint32_t bad = nan_keys[v];
-                    bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
-                    bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
-                    if (bad == 0) continue;
+                if (EDGE) {
+                    nan_keys |= __shfl_xor_sync(0xffffffffu, nan_keys, 1);
+                    nan_keys |= __shfl_xor_sync(0xffffffffu, nan_keys, 2);
+                    if (nan_keys == 0) continue;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -411,17 +495,28 @@ attention_q4_kernel(const QaParams p) {
                             const int pos = row_pos(n, c);
                             bool sees = false;
                             for (int k = 0; k < 16; ++k)
-                                sees = sees || ((bad >> k & 1) && key0 + k <= pos && (p.window <= 0 || key0 + k > pos - p.window));
+                                sees = sees || ((nan_keys >> k & 1) && key0 + k <= pos && (p.window <= 0 || key0 + k > pos - p.window));
                             if (!sees) continue;
 #pragma unroll
-                            for (int k = 0; k < (VW == 1 ? 4 : 8); ++k) o[8 * v + k][n][c] = o[8 * v + k][n][c + 2] = __int_as_float(0x7fc00000);
+                            for (int k = 0; k < (VW == 1 ? 4 : 8); ++k) o[8 * u + k][n][c] = o[8 * u + k][n][c + 2] = __int_as_float(0x7fc00000);
                         }
                 }
             }
         }
+    };
+    for (int j = 0;; ++j) {
+        const int first = chunk_tile(j), n_tiles = min(QA_KT, tile1 - first);
+        if (n_tiles <= 0) break;
+        const uint8_t* const stage = ring + at * (QA_KT * T::BYTES);
+        if (!mbar_wait(bars + 8 * at, phase, 0)) mbar_wait(bars + 8 * at, phase, 0);      // its copies must not outlive the CTA
+        if (n_tiles < QA_KT || (first + QA_KT) * 16 - 1 > pos_first || (p.window > 0 && first * 16 <= pos_last - p.window))
+            chunk(std::true_type(), first, n_tiles, stage);
+        else
+            chunk(std::false_type(), first, QA_KT, stage);
         __syncwarp();                                              // every lane is done with the stage
-        request(j + QA_STAGES, next_entry);
+        request(j + QA_STAGES, next_entry, at);
         next_entry = my_page(j + QA_STAGES + 1);
+        if (++at == QA_STAGES) { at = 0; phase ^= 1; }
     }
 
     // ---- the warps' results side by side in shared memory (the rings are free), merged by all threads
@@ -434,7 +529,6 @@ attention_q4_kernel(const QaParams p) {
             l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
         }
     __syncthreads();
-    constexpr int R = 8 * NT;
     float* const mo = reinterpret_cast<float*>(qa_smem);                       // [warp][row][PITCH]
     float2* const ml = reinterpret_cast<float2*>(mo + QA_WARPS * R * T::PITCH);  // [warp][row]
 #pragma unroll
@@ -448,7 +542,8 @@ attention_q4_kernel(const QaParams p) {
             if (g == 0) ml[warp * R + r] = make_float2(m[n][c], l[n][c]);
         }
     __syncthreads();
-    const long long part0 = (((long long)item * gridDim.y + kvh) * p.n_splits + split) * R;
+    const bool whole_pair = off == 0 && tile1 - tile0 == it.tiles;
+    const long long part0 = (2ll * blockIdx.x + (off == 0 || f > f_begin ? 1 : 0)) * R;
     for (int e = threadIdx.x; e < rows * (HD / 4); e += QA_THREADS) {
         const int r = e / (HD / 4), d = e % (HD / 4) * 4;
         float top = -INFINITY;
@@ -465,7 +560,7 @@ attention_q4_kernel(const QaParams p) {
             sum = fmaf(x.y, f, sum);
             acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
         }
-        if (p.n_splits > 1) {
+        if (!whole_pair) {
             *reinterpret_cast<float4*>(p.part_o + (part0 + r) * HD + d) = acc;
             if (d == 0) p.part_ml[part0 + r] = make_float2(top, sum);
         } else {
@@ -476,109 +571,137 @@ attention_q4_kernel(const QaParams p) {
                 make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
         }
     }
+    f += tile1 - tile0;
+    if (f >= start + it.tiles * p.kv.kv_heads) { start += it.tiles * p.kv.kv_heads; ++item; }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next pair's copies overwrite what was merged here
+    __syncthreads();
+    }
 }
 
-// The shares of each (item, kv head, row), folded in ascending order.  The first eight shares are asked for
-// before their weights are known.
+// The pieces of each pair that fell to several CTAs, folded in ascending order.  GROUPS 1: a CTA per pair, a thread
+// for four channels of a row (many pairs, few pieces each).  GROUPS > 1: a CTA per pair and row, whose
+// threads take every GROUPS-th piece and are added up in shared memory (few pairs, many pieces).
 constexpr int QA_FOLD_THREADS = 256;
-template <int HD, int NT>
+template <int HD, int NT, int GROUPS>
 __global__ void __launch_bounds__(QA_FOLD_THREADS) attention_q4_fold_kernel(const QaParams p) {
     constexpr int R = 8 * NT, V = HD / 4, S = 8;
-    __shared__ float wm[QA_MAX_SPLITS * R], wl[QA_MAX_SPLITS * R];
+    __shared__ float4 sums[GROUPS > 1 ? QA_FOLD_THREADS : 1];
+    __shared__ float parts[GROUPS > 1 ? GROUPS : 1];
     pdl_launch_dependents();
     pdl_wait();
-    const int item = blockIdx.x, kvh = blockIdx.y;
-    const int seg = p.items ? p.items[2 * item] : item, row0 = p.items ? p.items[2 * item + 1] : 0;
-    const int q_start = p.segments[p.n_segments + seg], q_len = p.segments[2 * p.n_segments + seg];
-    const int rows = min(R, q_len * p.group - row0);
-    const long long base = ((long long)item * gridDim.y + kvh) * p.n_splits * R;
-    const float4* const po = reinterpret_cast<const float4*>(p.part_o) + base * V;
-    for (int e = threadIdx.x; e < p.n_splits * R; e += QA_FOLD_THREADS) {
-        if (e % R >= rows) continue;                               // rows past the last are not written
-        const float2 x = __ldcg(p.part_ml + base + e);
-        wm[e] = x.x;
-        wl[e] = x.y;
-    }
-    __syncthreads();
-    if (threadIdx.x < rows) {
-        const int r = threadIdx.x;
+    const int item = blockIdx.x / p.kv.kv_heads, kvh = blockIdx.x % p.kv.kv_heads;
+    const QaItem it(p, item, R);
+    const QaRanges all(p, R);
+    const uint32_t begin = QaRanges::before(p, item, R) + kvh * it.tiles;
+    const int c0 = (int)(begin / all.per), c1 = (int)((begin + it.tiles - 1) / all.per);
+    if (c0 == c1 || it.tiles == 0) return;                         // written whole
+    const int group = GROUPS > 1 ? threadIdx.x / V : 0;
+    for (int e = GROUPS > 1 ? threadIdx.x % V + blockIdx.y * V : threadIdx.x; e < it.rows * V; e += GROUPS > 1 ? R * V : QA_FOLD_THREADS) {
+        const int r = e / V, d = e % V;
         float top = -INFINITY, sum = 0.f;
-        for (int s = 0; s < p.n_splits; ++s) top = fmaxf(top, wm[s * R + r]);
-        const float use = top == -INFINITY ? 0.f : top;
-        for (int s = 0; s < p.n_splits; ++s) {
-            const float f = qa_ex2(wm[s * R + r] - use);
-            sum = fmaf(wl[s * R + r], f, sum);
-            wm[s * R + r] = f;
-        }
-        wl[r] = 128.f / sum;
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < rows * V; e += QA_FOLD_THREADS) {
-        const int r = e / V, d = e % V * 4;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s0 = 0; s0 < p.n_splits; s0 += S) {
+        for (int s0 = c0 + group; s0 <= c1; s0 += S * GROUPS) {
+            float2 ml[S];
             float4 v[S];
 #pragma unroll
-            for (int q = 0; q < S; ++q)
-                v[q] = s0 + q < p.n_splits ? __ldcg(po + (long long)(s0 + q) * R * V + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int q = 0; q < S; ++q) {
+                const int c = s0 + q * GROUPS;
+                // the pair begins in c0's range, or lies before all of the others'
+                const long long at = (2ll * c + (c == c0 ? 1 : 0)) * R + r;
+                ml[q] = c <= c1 ? __ldcg(p.part_ml + at) : make_float2(-INFINITY, 0.f);
+                v[q] = c <= c1 ? __ldcg(reinterpret_cast<const float4*>(p.part_o) + at * V + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float m = top;
+#pragma unroll
+            for (int q = 0; q < S; ++q) m = fmaxf(m, ml[q].x);
+            const float use = m == -INFINITY ? 0.f : m, f = qa_ex2(top - use);
+            top = m;
+            sum *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
 #pragma unroll
             for (int q = 0; q < S; ++q) {
-                const float f = s0 + q < p.n_splits ? wm[(s0 + q) * R + r] : 0.f;
-                acc.x = fmaf(v[q].x, f, acc.x); acc.y = fmaf(v[q].y, f, acc.y); acc.z = fmaf(v[q].z, f, acc.z); acc.w = fmaf(v[q].w, f, acc.w);
+                const float w = qa_ex2(ml[q].x - use);
+                sum = fmaf(ml[q].y, w, sum);
+                acc.x = fmaf(v[q].x, w, acc.x); acc.y = fmaf(v[q].y, w, acc.y); acc.z = fmaf(v[q].z, w, acc.z); acc.w = fmaf(v[q].w, w, acc.w);
             }
         }
-        const float inv = wl[r];
-        const int row = row0 + r, tok = q_start + row / p.group, head = kvh * p.group + row % p.group;
+        if constexpr (GROUPS > 1) {
+            // (one row per CTA: all threads are here)
+            __shared__ float tops[GROUPS];
+            sums[threadIdx.x] = acc;
+            if (d == 0) { tops[group] = top; parts[group] = sum; }
+            __syncthreads();
+            if (group > 0) return;
+            float m = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < GROUPS; ++k) m = fmaxf(m, tops[k]);
+            const float use = m == -INFINITY ? 0.f : m;
+            sum = 0.f;
+            acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < GROUPS; ++k) {
+                const float w = qa_ex2(tops[k] - use);
+                const float4 v = sums[k * V + d];
+                sum = fmaf(parts[k], w, sum);
+                acc.x = fmaf(v.x, w, acc.x); acc.y = fmaf(v.y, w, acc.y); acc.z = fmaf(v.z, w, acc.z); acc.w = fmaf(v.w, w, acc.w);
+            }
+        }
+        const float inv = 128.f / sum;
+        const int row = it.row0 + r, tok = it.q_start + row / p.group, head = kvh * p.group + row % p.group;
         const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), b = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(p.out + ((long long)tok * p.heads + head) * HD + d) =
+        *reinterpret_cast<uint2*>(p.out + ((long long)tok * p.heads + head) * HD + 4 * d) =
             make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
 }
 
 template <int HD, int NT>
-static int launch_q4(const QaParams& p, int n_items, cudaStream_t stream) {
-    constexpr int smem = QaTile<HD>::smem(NT);
+static int launch_q4(const QaParams& p, cudaStream_t stream) {
+    constexpr int smem = QaTile<HD>::smem(NT), groups = QA_FOLD_THREADS / (HD / 4);
     static_assert(smem <= 226 * 1024, "the rings do not fit shared memory");
     if (int st = ensure_dynamic_smem<attention_q4_kernel<HD, NT>>(smem, "axon_attention_q4")) return st;
-    launch_pdl(attention_q4_kernel<HD, NT>, dim3(n_items, p.kv.kv_heads, p.n_splits), dim3(QA_THREADS), smem, stream, p);
+    launch_pdl(attention_q4_kernel<HD, NT>, dim3(p.ctas), dim3(QA_THREADS), smem, stream, p);
     if (int st = launch_status("axon_attention_q4")) return st;
-    if (p.n_splits > 1) {
-        launch_pdl(attention_q4_fold_kernel<HD, NT>, dim3(n_items, p.kv.kv_heads), dim3(QA_FOLD_THREADS), 0, stream, p);
-        return launch_status("axon_attention_q4 fold");
-    }
-    return AXON_OK;
+    const int pairs = p.n_items * p.kv.kv_heads;
+    // a pair is cut into at most ctas / pairs + 2 pieces if all are alike; with few pairs there are many
+    if (pairs * 4 < p.ctas)
+        launch_pdl(attention_q4_fold_kernel<HD, NT, groups>, dim3(pairs, 8 * NT), dim3(QA_FOLD_THREADS), 0, stream, p);
+    else
+        launch_pdl(attention_q4_fold_kernel<HD, NT, 1>, dim3(pairs), dim3(QA_FOLD_THREADS), 0, stream, p);
+    return launch_status("axon_attention_q4 fold");
 }
 
 }  // namespace axon
 
 using namespace axon;
 
+// How many CTAs an attention launch has (two fit an SM with one tile of 8 rows, up to head size 128).
+AXON_API int axon_attention_q4_ctas(int head_dim, int row_tiles) { return (row_tiles == 1 && head_dim <= 128 ? 2 : 1) * 148; }
+
 // Attention of `n_items` tiles of up to 8 * row_tiles query rows (row_tiles 1, 2 or 4; at head size 256 1 or 2).  items null:
-// item i is segment i, whose rows all fit one tile.  With several splits scratch holds
-// n_items * kv_heads * splits * 8 * row_tiles * (head_dim + 2) floats.
+// item i is segment i, whose rows all fit one tile.  scratch: 2 * ctas * 8 * row_tiles * (head_dim + 2) floats.
 AXON_API int axon_attention_q4(const void* q, const void* pool, void* out, const int32_t* segments, int n_segments,
                                const int32_t* items, int n_items, const AxonKvLayout* layout, int heads, float scale, int window,
-                               int row_tiles, int n_splits, float* scratch, long long scratch_floats, cudaStream_t stream) {
+                               int row_tiles, float* scratch, long long scratch_floats, cudaStream_t stream) {
     if (n_items <= 0) return AXON_OK;
     QaParams p;
     if (int st = to_q4(layout, pool, "axon_attention_q4", &p.kv)) return st;
     const int hd = p.kv.hd;
     if (p.kv.planes != 2 || p.kv.vd != hd) { set_error("axon_attention_q4: takes caches with key and value planes of one width"); return AXON_BAD_ARGUMENT; }
     if (heads < 1 || heads % p.kv.kv_heads) { set_error("axon_attention_q4: %d heads over %d kv heads", heads, p.kv.kv_heads); return AXON_BAD_ARGUMENT; }
-    if (n_splits < 1 || n_splits > QA_MAX_SPLITS || p.kv.kv_heads > 65535) { set_error("axon_attention_q4: bad split count %d (1..%d)", n_splits, QA_MAX_SPLITS); return AXON_BAD_ARGUMENT; }
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)scratch) & 15) { set_error("axon_attention_q4: operands must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
+    if ((double)n_items * p.kv.kv_heads * ((double)p.kv.table_stride * p.kv.page_size / 16 + 1) > 2147483647.0) { set_error("axon_attention_q4: %d items of %d kv heads at up to %d pages are too many", n_items, p.kv.kv_heads, p.kv.table_stride); return AXON_BAD_ARGUMENT; }
     p.run = 1;
     while (p.run < 16 && p.kv.page_size % (2 * p.run) == 0) p.run *= 2;
     // a copy moves whole 16 bytes, and a lane each must do for the pieces of a chunk
     if (p.run * hd / 16 % 16 || QA_KT * (p.kv.page_size == 16 ? 1 : 64 / p.run) > 32) { set_error("axon_attention_q4: pages of %d positions of %d values do not fall into pieces it can copy", p.kv.page_size, hd); return AXON_BAD_ARGUMENT; }
-    const long long per = (long long)n_items * p.kv.kv_heads * n_splits * 8 * row_tiles;
-    if (n_splits > 1 && (scratch == nullptr || scratch_floats < per * (hd + 2))) { set_error("axon_attention_q4: %d key shares need %lld floats of scratch", n_splits, per * (hd + 2)); return AXON_BAD_ARGUMENT; }
+    p.ctas = axon_attention_q4_ctas(hd, row_tiles);
+    const long long rows = 2ll * p.ctas * 8 * row_tiles;
+    if (scratch == nullptr || scratch_floats < rows * (hd + 2)) { set_error("axon_attention_q4: needs %lld floats of scratch", rows * (hd + 2)); return AXON_BAD_ARGUMENT; }
     p.q = (const __nv_bfloat16*)q; p.pool = (const uint8_t*)pool; p.out = (__nv_bfloat16*)out;
     p.segments = segments; p.items = items;
-    p.part_o = scratch; p.part_ml = scratch ? reinterpret_cast<float2*>(scratch + per * hd) : nullptr;
-    p.n_segments = n_segments; p.heads = heads; p.group = heads / p.kv.kv_heads; p.n_splits = n_splits; p.window = window;
+    p.part_o = scratch; p.part_ml = reinterpret_cast<float2*>(scratch + rows * hd);
+    p.n_segments = n_segments; p.n_items = n_items; p.heads = heads; p.group = heads / p.kv.kv_heads; p.window = window;
     p.scale_log2 = scale * 1.4426950408889634f;
-#define AXON_Q4_CASE(HD, NT) if (hd == HD && row_tiles == NT) return launch_q4<HD, NT>(p, n_items, stream)
+#define AXON_Q4_CASE(HD, NT) if (hd == HD && row_tiles == NT) return launch_q4<HD, NT>(p, stream)
     AXON_Q4_CASE(64, 1); AXON_Q4_CASE(64, 2); AXON_Q4_CASE(64, 4);
     AXON_Q4_CASE(128, 1); AXON_Q4_CASE(128, 2); AXON_Q4_CASE(128, 4);
     AXON_Q4_CASE(256, 1); AXON_Q4_CASE(256, 2);

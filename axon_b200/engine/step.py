@@ -81,6 +81,7 @@ class Engine:
 
     def __init__(self, model: DecoderModel, cache: PagedCache, max_step_tokens: int = 8192):
         self.model, self.cache, self.rt = model, cache, model.rt
+        self.rt.kv_page_size = cache.page_size
         self.max_step_tokens = max_step_tokens
         self._staging: List[torch.Tensor] = []
         self._events: List[Optional[torch.cuda.Event]] = []

@@ -367,28 +367,13 @@ def q4_plain_splits(ctx, heads: int, kv_heads: int, window: int) -> int:
     return max(1, min(-(-keys // Q4_PLAIN_KEYS), Q4_PLAIN_CTAS // max(ctas, 1)))
 
 
-Q4_MAX_SPLITS = 64
-#: row tiles of 8 that the kernel holds at once, by head size, and 16-key tiles that the eight warps of a CTA take in a turn
+#: row tiles of 8 that the kernel holds at once, by head size
 Q4_ROW_TILES = {64: 4, 128: 4, 256: 2}
-Q4_TURN_TILES = 16
 
 
 def _q4_row_tiles(rows: int, hd: int) -> int:
     """Row tiles of 8 for segments of up to ``rows`` query rows: 1, 2 or 4."""
     return next((n for n in (1, 2, 4) if 8 * n >= rows or n == Q4_ROW_TILES[hd]))
-
-
-def _q4_splits(pairs: int, keys: int, row_tiles: int) -> int:
-    """Into how many shares to cut the keys of each of ``pairs`` (item, kv head), the longest of which sees
-    ``keys``: the cheapest by turns of the longest share, a little per share for the fold and its kernel."""
-    tiles = -(-keys // 16)
-    most = max(1, min(-(-tiles // 2), Q4_MAX_SPLITS, (2 if row_tiles == 1 else 1) * SM_COUNT // max(pairs, 1)))
-    best, best_cost = 1, -(-tiles // Q4_TURN_TILES)
-    for s in range(2, most + 1):
-        cost = -(--(-tiles // s) // Q4_TURN_TILES) + 0.1 * s + 2.0
-        if cost < best_cost - 1e-9:
-            best, best_cost = s, cost
-    return best
 
 
 def _q4_items(ctx, group: int, hd: int):
@@ -408,29 +393,26 @@ def _q4_items(ctx, group: int, hd: int):
     return got
 
 
-def _q4_takes(kv, heads: int) -> bool:
-    return (kv.head_dim in Q4_ROW_TILES and kv.planes == 2 and kv.v_dim == kv.head_dim and heads % kv.kv_heads == 0
-            and kv.page_size % 4 == 0)
+def _q4_takes(hd: int, page_size: int) -> bool:
+    return hd in Q4_ROW_TILES and page_size % 4 == 0
 
 
 def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
     """Tensor-core attention over a 4-bit cache; refuses head sizes other than 64, 128 and 256, pages of a
     number of positions that is no multiple of 4, and dtypes other than bfloat16."""
-    if not ENABLED["attention_q4"] or ctx.segments is None or not _q4_takes(kv, heads):
+    if not ENABLED["attention_q4"] or ctx.segments is None or not _q4_takes(kv.head_dim, kv.page_size):
+        return False
+    if kv.planes != 2 or kv.v_dim != kv.head_dim or heads % kv.kv_heads:
         return False
     if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or not q.is_contiguous() or not out.is_contiguous():
         return False
-    group = heads // kv.kv_heads
-    nt, n_items, items = _q4_items(ctx, group, kv.head_dim)
-    keys = min(ctx.max_kv_len, kv.window + ctx.max_q_len - 1) if kv.window else ctx.max_kv_len
-    splits = _q4_splits(n_items * kv.kv_heads, keys, nt)
-    scratch, floats = None, 0
-    if splits > 1:
-        floats = n_items * kv.kv_heads * splits * 8 * nt * (kv.head_dim + 2)
-        scratch = ctx.rt.buffer("q4_scratch", (floats,), torch.float32)
-    check(lib.cuda().axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
-                                       None if items is None else items.data_ptr(), n_items, kv._ref, heads, float(scale),
-                                       int(kv.window), nt, splits, None if scratch is None else scratch.data_ptr(), floats, _stream()))
+    nt, n_items, items = _q4_items(ctx, heads // kv.kv_heads, kv.head_dim)
+    cu = lib.cuda()
+    floats = 2 * cu.axon_attention_q4_ctas(kv.head_dim, nt) * 8 * nt * (kv.head_dim + 2)
+    scratch = ctx.rt.buffer(f"q4_scratch_{kv.head_dim}_{nt}", (floats,), torch.float32)
+    check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
+                               None if items is None else items.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
+                               nt, scratch.data_ptr(), floats, _stream()))
     return True
 
 
@@ -440,11 +422,8 @@ def attention_q4_status() -> int:
 
 
 def q4_graph_key(ctx, heads: int, kv_heads: int, head_dim: int, window: int, precise: bool):
-    """What the 4-bit attention's launches take from the host beside the batch shape."""
-    keys = min(ctx.max_kv_len, window + ctx.max_q_len - 1) if window else ctx.max_kv_len
-    splits = 0
-    if not precise and head_dim in Q4_ROW_TILES:
-        group = heads // kv_heads
-        nt = _q4_row_tiles(ctx.max_q_len * group, head_dim)
-        splits = _q4_splits(sum(-(-n * group // (8 * nt)) for n in ctx.seg_q_len) * kv_heads, keys, nt)
-    return (("q4", q4_plain_splits(ctx, heads, kv_heads, window), splits),)
+    """What the 4-bit attention's launches take from the host beside the batch shape: nothing of the
+    tensor-core kernel's (it divides its work on the device), the share count of the plain one's."""
+    if not precise and ENABLED["attention_q4"] and _q4_takes(head_dim, ctx.rt.kv_page_size):
+        return ()
+    return (("q4_plain", q4_plain_splits(ctx, heads, kv_heads, window)),)

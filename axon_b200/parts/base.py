@@ -50,6 +50,8 @@ class Runtime:
             raise ValueError(f"cache rows have the model's dtype (0) or 4 bits a value, not {kv_bits}")
         #: bits of a cached value (0: the model's dtype) in the caches of parts that take them (``Part.kv_bits``)
         self.kv_bits = kv_bits
+        #: positions per cache page (the engine sets it)
+        self.kv_page_size = 0
         #: the true 32-bit path: plain FFMA kernels everywhere
         self.precise = dtype == torch.float32
         self._buffers: Dict[str, torch.Tensor] = {}
