@@ -16,25 +16,26 @@
 // Halves rather than bfloat16 because the weights P then keep 11 bits; queries are scaled by a power of two
 // per row to the range of halves (exact, but for elements 2^-24 below the row's largest).
 //
-// A warp works alone: its own ring of shared memory, filled by bulk copies (one per 16-position page
-// and kv head: codes and steps of keys and values lie together) that one mbarrier per stage counts, its own running
+// A warp works alone: its own ring of shared memory, filled by asynchronous copies of 16 bytes (with pages of 16
+// positions a kv head's codes and steps of keys and values are one run of 18 HD bytes), its own running
 // maximum and sum.  The maximum lags: O is rescaled only when a score exceeds it by 2^8.  The warps of a CTA take
-// chunks of 32 keys in turn and are merged at the end.
+// chunks of 32 keys in turn and are merged at the end.  (Bulk copies counted by mbarriers were measured first: a
+// copy's uniform operands cost the issuing warp some 30 instructions, these 5 a tile.)
 //
 // The grid is as many CTAs as fit at once, and the 16-key tiles of all (item, kv head) pairs, laid
 // end to end, are cut into one equal range for each: contexts of any lengths load the GPU evenly, and
-// nothing of the launch depends on them.  A CTA works through the pairs of its range; a pair that lies in one
-// range whole is written out, the pieces of the others go to scratch (at most two per CTA: the one
-// its range begins in and the one it ends in) and a second kernel folds them in ascending order.
+// nothing of the launch depends on them.  A CTA works through the pairs of its range, asking for the next pair's
+// keys before it merges the warps' results of the last.  A pair that lies in one range whole is written out; the pieces
+// of the others go to scratch (at most two per CTA: the one its range begins in and the one it ends in), and the
+// CTA whose piece arrives last folds them in ascending order, so results do not depend on the order of arrival.
 #include "kv_q4.cuh"
-#include "tcgen05.cuh"
 
 #include <type_traits>
 
 namespace axon {
 
 constexpr int QA_WARPS = 8, QA_THREADS = QA_WARPS * 32;
-constexpr int QA_KT = 2, QA_STAGES = 3;          // 16-key tiles per chunk, chunks in a warp's ring
+constexpr int QA_KT = 2, QA_STAGES = 2;          // 16-key tiles per chunk, chunks in a warp's ring
 constexpr int QA_LEAST = QA_WARPS * QA_KT;       // tiles below which a range is not cut further: one chunk for each warp
 constexpr float QA_LAZY = 8.f;                   // log2 units a score may exceed the running maximum
 
@@ -46,29 +47,34 @@ struct QaParams {
     const int32_t* items;        // [n_items][2]: segment, first row (token * group + head of the group); null: segment i, row 0
     float* part_o;               // [2 * CTA + (0: the pair its range begins in, 1: the one it ends in)][row][HD]
     float2* part_ml;             // the same without the last index: maximum (log2 units) and sum
+    unsigned int* arrived;       // [CTA]: pieces written of the pair that begins in the CTA's range and ends in another's; zero between launches
     PagedQ4 kv;
     int n_segments, n_items, heads, group, ctas, window;
-    int run;                     // positions of a tile that lie together in a page: gcd(page size, 16)
     float scale_log2;
 };
 
 template <int HD> struct QaTile {
     static constexpr int KC = 8 * HD, KS = HD, BYTES = 2 * (KC + KS);      // codes and steps of 16 keys; a tile with its values
+    static constexpr int PIECES = BYTES / 16, LANE_PIECES = (QA_KT * PIECES + 31) / 32;   // 16-byte pieces of a tile; of a chunk per lane
     static constexpr int RING = QA_WARPS * QA_STAGES * QA_KT * BYTES;
     static constexpr int PITCH = HD + 8;                                    // floats between rows of the merge buffer
     static constexpr int merge(int nt) { return QA_WARPS * 8 * nt * (PITCH + 2) * 4; }
     static constexpr int queries(int nt) { return nt > 1 ? HD / 16 * nt * 32 * 8 + 8 * nt * 4 : 0; }
-    static constexpr int area(int nt) { return RING > merge(nt) ? RING : merge(nt); }
-    static constexpr int smem(int nt) { return area(nt) + queries(nt); }
+    static constexpr int smem(int nt) { return RING + merge(nt) + queries(nt); }
 };
 
-__device__ __forceinline__ void qa_bulk_load(uint32_t smem, const void* gmem, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem), "l"(gmem), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void qa_copy16(uint32_t smem, const void* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
+__device__ __forceinline__ void qa_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void qa_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void qa_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void qa_mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t qa_transpose(uint32_t x) {
     uint32_t y;
@@ -140,9 +146,10 @@ template <int N> __device__ __forceinline__ void qa_lds(uint32_t (&r)[N], const 
 }
 
 // One row's share of a query fragment: the HD / 4 channels of this thread (lane % 4) of the row, scaled by
-// 2^-e so that the row's largest element lies in [1, 2), as the B operand's registers.  Returns 2^e.
+// 2^-e so that the row's largest element lies in [1, 2), and by -1 for a negative scale, as the B operand's
+// registers.  Returns the factor that brings scores to log2 units (keys carry a 1 / 128), which is not negative.
 template <int HD>
-__device__ __forceinline__ float qa_load_query(uint32_t (&f)[HD / 16][2], const __nv_bfloat16* row, int t, bool live) {
+__device__ __forceinline__ float qa_load_query(uint32_t (&f)[HD / 16][2], const __nv_bfloat16* row, int t, bool live, float scale_log2) {
     constexpr int W = HD / 32;
     uint4 raw[W];
     uint32_t top = 0;
@@ -159,7 +166,7 @@ __device__ __forceinline__ float qa_load_query(uint32_t (&f)[HD / 16][2], const 
     int e = (int)(top >> 7) - 127;
     if (top == 0 || top >= 0x7f80u) e = 0;
     e = max(e, -126);                             // (2^126 is the largest power that brings subnormals up)
-    const float down = e > 126 ? 5.877471754111438e-39f : __uint_as_float((uint32_t)(127 - e) << 23);
+    const float down = copysignf(e > 126 ? 5.877471754111438e-39f : __uint_as_float((uint32_t)(127 - e) << 23), scale_log2);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
         const uint32_t u[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
@@ -172,7 +179,7 @@ __device__ __forceinline__ float qa_load_query(uint32_t (&f)[HD / 16][2], const 
         f[2 * w][0] = qa_pack(x[0], x[4]); f[2 * w][1] = qa_pack(x[1], x[5]);
         f[2 * w + 1][0] = qa_pack(x[2], x[6]); f[2 * w + 1][1] = qa_pack(x[3], x[7]);
     }
-    return __uint_as_float((uint32_t)(127 + e) << 23);
+    return __uint_as_float((uint32_t)(127 + e) << 23) * fabsf(scale_log2) * 128.f;
 }
 
 // An item's rows and the keys they see.
@@ -200,14 +207,17 @@ struct QaItem {
 struct QaRanges {
     uint32_t total, per;
     __device__ __forceinline__ QaRanges(const QaParams& p, int most_rows) {
-        total = before(p, p.n_items, most_rows);
-        per = max((uint32_t)QA_LEAST, (total + p.ctas - 1) / p.ctas);
-    }
-    // tiles of all pairs before `item`
-    static __device__ __forceinline__ uint32_t before(const QaParams& p, int item, int most_rows) {
-        uint32_t sum = 0;
-        for (int i = threadIdx.x & 31; i < item; i += 32) sum += QaItem(p, i, most_rows).tiles;
-        return __reduce_add_sync(0xffffffffu, sum) * p.kv.kv_heads;
+        uint32_t sum = 0, longest = 0;
+        for (int i = threadIdx.x & 31; i < p.n_items; i += 32) {
+            const uint32_t n = QaItem(p, i, most_rows).tiles;
+            sum += n;
+            longest = max(longest, n);
+        }
+        total = __reduce_add_sync(0xffffffffu, sum) * p.kv.kv_heads;
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        // one CTA folds a pair's pieces: with few long pairs, as long a range (a turn of 16 tiles takes about 0.9 us) as the
+        // fold of as many pieces (0.05 us each) would take, which is about the square root of a pair's tiles
+        per = max(max((uint32_t)QA_LEAST, (uint32_t)sqrtf((float)longest)), (total + p.ctas - 1) / p.ctas);
     }
     // the item that tile f falls into, and the tiles before it
     static __device__ __forceinline__ int find(const QaParams& p, uint32_t f, int most_rows, uint32_t* start) {
@@ -234,114 +244,138 @@ struct QaRanges {
     }
 };
 
-template <int HD, int NT>
+template <int HD, int NT, bool WHOLE>
 __global__ void __launch_bounds__(QA_THREADS, (NT == 1 && HD <= 128) ? 2 : 1)
 attention_q4_kernel(const QaParams p) {
     using T = QaTile<HD>;
     constexpr int KW = HD / 32, VW = HD / 64, MT = HD / 16;      // words of a key row and of a value row per thread; 16-channel tiles of O
     constexpr int KG = HD / 64;                                   // groups (steps) of a key row per thread
+    constexpr int R = 8 * NT;
     extern __shared__ __align__(128) uint8_t qa_smem[];
-    __shared__ __align__(8) uint64_t qa_bars[QA_WARPS * QA_STAGES];
-    pdl_launch_dependents();
+    __shared__ unsigned int last;
+    float* const mo = reinterpret_cast<float*>(qa_smem + T::RING);                // [warp][row][PITCH] results of the warps
+    float2* const ml = reinterpret_cast<float2*>(mo + QA_WARPS * R * T::PITCH);   // [warp][row]
+    uint2* const q_smem = reinterpret_cast<uint2*>(qa_smem + T::RING + T::merge(NT));         // [HD / 16][NT][lane], several row tiles
+    float* const f_smem = reinterpret_cast<float*>(q_smem + HD / 16 * NT * 32);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t* const ring = qa_smem + warp * (QA_STAGES * QA_KT * T::BYTES);
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-    const uint32_t bars = (uint32_t)__cvta_generic_to_shared(qa_bars + warp * QA_STAGES);
-    if (lane == 0) {
-        for (int s = 0; s < QA_STAGES; ++s) mbar_init(bars + 8 * s, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    __syncwarp();
+    pdl_launch_dependents();
     pdl_wait();
 
-    constexpr int R = 8 * NT;
-    uint32_t f, f1, start;
+    uint32_t f, f1, start, per;
     int item;
     {
         const QaRanges all(p, R);
-        if (blockIdx.x > (all.total - 1) / all.per || all.total == 0) return;
-        f = blockIdx.x * all.per;
-        f1 = f + min(all.per, all.total - f);
+        if (all.total == 0 || blockIdx.x > (all.total - 1) / all.per) return;
+        per = all.per;
+        f = blockIdx.x * per;
+        f1 = f + min(per, all.total - f);
         item = QaRanges::find(p, f, R, &start);
     }
     const uint32_t f_begin = f;
     const QaMagic magic;
-    int at = 0;                                                    // the stage of the warp's ring that it reads next,
-    uint32_t phase = 0;                                            // and its barrier's phase
-    while (f < f1) {
-    const QaItem it(p, item, R);
-    if (it.tiles == 0) {                                           // (an empty segment: nothing to read or to write)
-        if (++item >= p.n_items) return;
-        continue;
-    }
-    const int kvh = (int)((f - start) / it.tiles), off = (int)((f - start) % it.tiles);
-    const int rows = it.rows, pos_first = it.pos_first, pos_last = it.pos_last, row0 = it.row0, q_start = it.q_start;
-    const int kv_lo = it.kv_lo, kv_hi = it.kv_hi;
-    const int tile0 = it.tile0 + off, tile1 = tile0 + (int)min((uint32_t)(it.tiles - off), f1 - f);
 
-    // ---- copies.  A lane owns one piece of a chunk: with pages of 16 positions a whole tile, else a run of
-    // one of its four parts.
-    const bool whole = p.kv.page_size == 16;
-    const int pieces = whole ? 1 : 64 / p.run;                    // of a tile
-    const int my_tile = lane / pieces, sub = lane % pieces, part = sub & 3, key_off = whole ? 0 : (sub >> 2) * p.run;
-    const int row_bytes = (part & 1) ? HD / 16 : HD / 2;
-    const uint32_t my_bytes = whole ? T::BYTES : p.run * row_bytes;
-    const uint32_t my_dst = my_tile * T::BYTES + (whole ? 0 : (part & 1 ? T::KC : 0) + (part & 2 ? T::KC + T::KS : 0) + key_off * row_bytes);
-    const uint8_t* const my_src = p.pool + p.kv.entry_offset + (long long)kvh * p.kv.record +
-        (whole || part == 0 ? 0 : part == 1 ? p.kv.k_steps : part == 2 ? p.kv.v_codes : p.kv.v_steps);
-    const int32_t* const table = p.kv.block_table + (long long)it.slot * p.kv.table_stride;
-    const int last_page = (kv_hi - 1) / p.kv.page_size;
+    // ---- copies: piece i of a chunk (of QA_KT * PIECES) is lane i % 32's
+    const int ps = p.kv.page_size;
+    const uint8_t* head_src;                                       // the pair's record in page 0
+    const int32_t* table;
+    int tile0, tile1, last_page;
     auto chunk_tile = [&](int j) { return tile0 + (warp + j * QA_WARPS) * QA_KT; };
-    auto my_page = [&](int j) {                                   // the table entry of this lane's piece of its warp's j-th chunk
-        const int tile = chunk_tile(j) + my_tile;
-        if (my_tile >= QA_KT || tile >= tile1) return 0;
-        return (int)table[whole ? tile : min((tile * 16 + key_off) / p.kv.page_size, last_page)];
+    struct Pages { int e[QA_KT]; };
+    auto pages = [&](int j) {                                     // table entries of the first positions of a chunk's tiles
+        Pages x;
+        const int first = chunk_tile(j);
+#pragma unroll
+        for (int i = 0; i < QA_KT; ++i) x.e[i] = first + i < tile1 ? table[WHOLE ? first + i : (first + i) * 16 / ps] : 0;
+        return x;
     };
-    auto request = [&](int j, int entry, int stage) {
+    auto request = [&](int j, const Pages& x, int stage) {
         const int first = chunk_tile(j), n = min(QA_KT, tile1 - first);
-        if (n <= 0) return;
-        const uint32_t bar = bars + 8 * stage;
-        if (lane == 0) mbar_expect_tx(bar, n * T::BYTES);
-        __syncwarp();
-        if (my_tile < n) {
-            const int in_page = whole ? 0 : ((first + my_tile) * 16 + key_off) % p.kv.page_size;
-            qa_bulk_load(ring_addr + stage * (QA_KT * T::BYTES) + my_dst,
-                         my_src + (long long)p.kv.page(entry) * p.kv.page_stride + (long long)in_page * row_bytes, my_bytes, bar);
+        if (n > 0) {
+            const uint32_t dst = ring_addr + stage * (QA_KT * T::BYTES) + lane * 16;
+            const int pieces = n * T::PIECES;
+            if constexpr (WHOLE) {
+                const uint8_t* src[QA_KT];
+#pragma unroll
+                for (int i = 0; i < QA_KT; ++i) src[i] = head_src + (long long)p.kv.page(x.e[i]) * p.kv.page_stride + lane * 16 - i * T::BYTES;
+                auto copy = [&](int k) {
+                    const uint8_t* from = src[0];
+#pragma unroll
+                    for (int i = 1; i < QA_KT; ++i) if (32 * k + lane >= i * T::PIECES) from = src[i];
+                    qa_copy16(dst + k * 512, from + k * 512);
+                };
+                if (n == QA_KT && QA_KT * T::PIECES % 32 == 0) {
+#pragma unroll
+                    for (int k = 0; k < T::LANE_PIECES; ++k) copy(k);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < T::LANE_PIECES; ++k) if (32 * k + lane < pieces) copy(k);
+                }
+            } else {
+                // a tile's four parts lie apart, and with pages that are no multiple of 16 positions its keys do too
+                const bool together = ps % 16 == 0;
+#pragma unroll
+                for (int k = 0; k < T::LANE_PIECES; ++k) {
+                    const int i = 32 * k + lane, tile = i / T::PIECES, in_tile = i % T::PIECES * 16;      // (bytes)
+                    if (i >= pieces) continue;
+                    const int half = in_tile / (T::KC + T::KS), in_half = in_tile % (T::KC + T::KS), steps = in_half >= T::KC;
+                    const int in_part = in_half - (steps ? T::KC : 0), row = steps ? HD / 16 : HD / 2;
+                    const int key = in_part / row, pos = (first + tile) * 16 + key;
+                    const int lp = min(pos / ps, last_page), in_page = pos % ps;      // (past the last page: some row of it, hidden later)
+                    const int entry = !together ? table[lp] : tile == 0 ? x.e[0] : x.e[1];
+                    const int part = half ? (steps ? p.kv.v_steps : p.kv.v_codes) : (steps ? p.kv.k_steps : 0);
+                    qa_copy16(dst + k * 512, head_src + (long long)p.kv.page(entry) * p.kv.page_stride + part + in_page * row + in_part % row);
+                }
+            }
         }
+        qa_copy_commit();
     };
-    int next_entry;
-    {
-        int e[QA_STAGES];
+    Pages next;
+    auto begin_pair = [&](const QaItem& it, int kvh, int off) {   // asks for the first keys of a pair's piece
+        tile0 = it.tile0 + off;
+        tile1 = tile0 + (int)min((uint32_t)(it.tiles - off), f1 - f);
+        head_src = p.pool + p.kv.entry_offset + (long long)kvh * p.kv.record;
+        table = p.kv.block_table + (long long)it.slot * p.kv.table_stride;
+        last_page = (it.kv_hi - 1) / ps;
+        Pages x[QA_STAGES];
 #pragma unroll
-        for (int j = 0; j < QA_STAGES; ++j) e[j] = my_page(j);
-        next_entry = my_page(QA_STAGES);
+        for (int j = 0; j < QA_STAGES; ++j) x[j] = pages(j);
+        next = pages(QA_STAGES);
 #pragma unroll
-        for (int j = 0; j < QA_STAGES; ++j) request(j, e[j], at + j < QA_STAGES ? at + j : at + j - QA_STAGES);
-    }
+        for (int j = 0; j < QA_STAGES; ++j) request(j, x[j], j);
+    };
 
     // ---- queries as B fragments, and the factor that brings a row's scores to log2 units
     uint32_t qf[NT == 1 ? HD / 16 : 1][2];
-    uint2* const q_smem = reinterpret_cast<uint2*>(qa_smem + T::area(NT));                    // [HD / 16][NT][lane]
-    float* const f_smem = reinterpret_cast<float*>(qa_smem + T::area(NT) + HD / 16 * NT * 32 * 8);
     float factor[NT][2];
-    auto query_row = [&](int r) {
-        const int row = row0 + r, tok = q_start + row / p.group, head = kvh * p.group + row % p.group;
-        return p.q + ((long long)tok * p.heads + head) * HD;
-    };
-    if constexpr (NT == 1) {
-        const float f = qa_load_query<HD>(qf, query_row(g < rows ? g : 0), t, g < rows) * p.scale_log2 * 128.f;
-        factor[0][0] = __shfl_sync(0xffffffffu, f, 8 * t);
-        factor[0][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);
-    } else {
-        if (warp < NT) {
-            uint32_t f[HD / 16][2];
+    auto load_queries = [&](const QaItem& it, int kvh) {
+        auto query_row = [&](int r) {
+            const int row = it.row0 + (r < it.rows ? r : 0), tok = it.q_start + row / p.group, head = kvh * p.group + row % p.group;
+            return p.q + ((long long)tok * p.heads + head) * HD;
+        };
+        if constexpr (NT == 1) {
+            const float x = qa_load_query<HD>(qf, query_row(g), t, g < it.rows, p.scale_log2);
+            factor[0][0] = __shfl_sync(0xffffffffu, x, 8 * t);
+            factor[0][1] = __shfl_sync(0xffffffffu, x, 8 * t + 4);
+        } else if (warp < NT) {                                    // (read back after the next barrier)
+            uint32_t x[HD / 16][2];
             const int r = 8 * warp + g;
-            const float scale = qa_load_query<HD>(f, query_row(r < rows ? r : 0), t, r < rows) * p.scale_log2 * 128.f;
+            const float scale = qa_load_query<HD>(x, query_row(r), t, r < it.rows, p.scale_log2);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) q_smem[(k * NT + warp) * 32 + lane] = make_uint2(f[k][0], f[k][1]);
+            for (int k = 0; k < HD / 16; ++k) q_smem[(k * NT + warp) * 32 + lane] = make_uint2(x[k][0], x[k][1]);
             if (t == 0) f_smem[r] = scale;
         }
+    };
+
+    QaItem it(p, item, R);
+    int kvh = (int)((f - start) / it.tiles), off = (int)((f - start) % it.tiles);
+    begin_pair(it, kvh, off);
+    load_queries(it, kvh);
+    for (;;) {
+    const int rows = it.rows, pos_first = it.pos_first, pos_last = it.pos_last, row0 = it.row0, q_start = it.q_start;
+    const int kv_lo = it.kv_lo, kv_hi = it.kv_hi;
+    if constexpr (NT > 1) {
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NT; ++n) { factor[n][0] = f_smem[8 * n + 2 * t]; factor[n][1] = f_smem[8 * n + 2 * t + 1]; }
@@ -360,21 +394,14 @@ attention_q4_kernel(const QaParams p) {
     // the position of the query row in column c of row tile n (rows past the last: the last token's)
     auto row_pos = [&](int n, int c) { return it.pos0 + (row0 + min(8 * n + 2 * t + c, rows - 1)) / p.group; };
 
-    // One chunk: EDGE when it may be short or hold keys that not every row sees.
-    auto chunk = [&](auto edge, int first, int n_tiles, const uint8_t* stage) {
+    // the tiles of this piece that every row sees whole: [clear0, clear1)
+    const int clear0 = p.window > 0 ? max(pos_last - p.window + 16, 0) / 16 : 0, clear1 = min(tile1, (pos_first + 1) / 16);
+    // One tile; EDGE when it may hold keys that not every row sees.
+    auto fold = [&](auto edge, int key0, const uint8_t* tile) {
         constexpr bool EDGE = decltype(edge)::value;
-        float s[QA_KT][NT][4];
-        float top[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < QA_KT; ++i) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) s[i][n][c] = !EDGE || i < n_tiles ? 0.f : -INFINITY;
-            if (EDGE && i >= n_tiles) continue;
-            const uint8_t* const tile = stage + i * T::BYTES;
+        float s[NT][4];
+        {
+            float s2[NT][4];                                       // two sums, so that products do not wait for one another
             uint32_t wa[KW], wb[KW];                               // this thread's codes of keys g and g + 8
             qa_lds(wa, tile + g * (HD / 2) + t * (HD / 8));
             qa_lds(wb, tile + (g + 8) * (HD / 2) + t * (HD / 8));
@@ -390,29 +417,39 @@ attention_q4_kernel(const QaParams p) {
                     uint2 q0, q1;
                     if constexpr (NT == 1) { q0 = make_uint2(qf[2 * w][0], qf[2 * w][1]); q1 = make_uint2(qf[2 * w + 1][0], qf[2 * w + 1][1]); }
                     else { q0 = q_smem[(2 * w * NT + n) * 32 + lane]; q1 = q_smem[((2 * w + 1) * NT + n) * 32 + lane]; }
-                    qa_mma(s[i][n], a[0], b[0], a[1], b[1], q0.x, q0.y);
-                    qa_mma(s[i][n], a[2], b[2], a[3], b[3], q1.x, q1.y);
-                }
-            }
-            const int key0 = (first + i) * 16;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) s[i][n][c] *= factor[n][c & 1];
-                if (EDGE) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int key = key0 + g + (c >> 1) * 8, pos = row_pos(n, c & 1);
-                        if (key > pos || (p.window > 0 && key <= pos - p.window)) s[i][n][c] = -INFINITY;
+                    if (w == 0) {
+                        qa_mma_first(s[n], a[0], b[0], a[1], b[1], q0.x, q0.y);
+                        qa_mma_first(s2[n], a[2], b[2], a[3], b[3], q1.x, q1.y);
+                    } else {
+                        qa_mma(s[n], a[0], b[0], a[1], b[1], q0.x, q0.y);
+                        qa_mma(s2[n], a[2], b[2], a[3], b[3], q1.x, q1.y);
                     }
                 }
-                top[n][0] = fmaxf(top[n][0], fmaxf(s[i][n][0], s[i][n][2]));
-                top[n][1] = fmaxf(top[n][1], fmaxf(s[i][n][1], s[i][n][3]));
             }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[n][c] += s2[n][c];
         }
+        // scores in log2 units are s * factor; an edge tile's are multiplied out before the mask (0 * infinity is NaN)
+        float top[NT][2];
         bool grew = false;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) grew = grew || top[n][0] > m[n][0] + QA_LAZY || top[n][1] > m[n][1] + QA_LAZY;
+        for (int n = 0; n < NT; ++n) {
+            if (EDGE) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int key = key0 + g + (c >> 1) * 8, pos = row_pos(n, c & 1);
+                    s[n][c] *= factor[n][c & 1];
+                    if (key > pos || (p.window > 0 && key <= pos - p.window)) s[n][c] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                top[n][c] = fmaxf(s[n][c], s[n][c + 2]) * (EDGE ? 1.f : factor[n][c]);
+                grew = grew || top[n][c] > m[n][c] + QA_LAZY;
+            }
+        }
         if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -430,64 +467,61 @@ attention_q4_kernel(const QaParams p) {
                     for (int k = 0; k < MT; ++k) { o[k][n][c] *= f; o[k][n][c + 2] *= f; }
                 }
         }
-        uint32_t pf[QA_KT][NT][2];                                 // weights as B fragments
+        uint32_t pf[NT][2];                                        // weights as B fragments
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float m0 = EDGE && m[n][0] == -INFINITY ? 0.f : m[n][0], m1 = EDGE && m[n][1] == -INFINITY ? 0.f : m[n][1];
+            float w[4];
 #pragma unroll
-            for (int i = 0; i < QA_KT; ++i) {
-                const float p0 = qa_ex2(s[i][n][0] - m0), p1 = qa_ex2(s[i][n][1] - m1), p2 = qa_ex2(s[i][n][2] - m0), p3 = qa_ex2(s[i][n][3] - m1);
-                l[n][0] += p0 + p2;
-                l[n][1] += p1 + p3;
-                pf[i][n][0] = qa_transpose(qa_pack(p0, p1));
-                pf[i][n][1] = qa_transpose(qa_pack(p2, p3));
+            for (int c = 0; c < 4; ++c) {
+                const float m_c = EDGE && m[n][c & 1] == -INFINITY ? 0.f : m[n][c & 1];
+                w[c] = qa_ex2(EDGE ? s[n][c] - m_c : fmaf(s[n][c], factor[n][c & 1], -m_c));
             }
+            l[n][0] += w[0] + w[2];
+            l[n][1] += w[1] + w[3];
+            pf[n][0] = qa_transpose(qa_pack(w[0], w[1]));
+            pf[n][1] = qa_transpose(qa_pack(w[2], w[3]));
         }
+        const uint8_t* const vt = tile + T::KC + T::KS;
+        uint32_t w4[4][VW];                                        // codes of keys 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-        for (int i = 0; i < QA_KT; ++i) {
-            if (EDGE && i >= n_tiles) continue;
-            const uint8_t* const tile = stage + i * T::BYTES + T::KC + T::KS;
-            const int key0 = (first + i) * 16;
-            uint32_t w4[4][VW];                                    // codes of keys 2t, 2t + 1, 2t + 8, 2t + 9
+        for (int k = 0; k < 4; ++k) qa_lds(w4[k], vt + (2 * t + (k & 1) + (k >> 1) * 8) * (HD / 2) + g * (HD / 16));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) qa_lds(w4[k], tile + (2 * t + (k & 1) + (k >> 1) * 8) * (HD / 2) + g * (HD / 16));
+        for (int u = 0; u < (VW + 1) / 2; ++u) {                   // groups of 16 channels (of 8, the half of one, at head size 64)
+            uint32_t by[4];
 #pragma unroll
-            for (int u = 0; u < (VW + 1) / 2; ++u) {               // groups of 16 channels (of 8, the half of one, at head size 64)
-                uint32_t by[4];
+            for (int k = 0; k < 4; ++k) by[k] = vt[T::KC + (2 * t + (k & 1) + (k >> 1) * 8) * (HD / 16) + (g * (HD / 8)) / 16 + u];
+            uint32_t nan_keys = 0;
+            if (EDGE) {
+                // keys that no row sees may hold anything, and a NaN that some rows see must not reach the others (0 * NaN
+                // is NaN): both count as zero here, and the rows that see a NaN get theirs below
 #pragma unroll
-                for (int k = 0; k < 4; ++k) by[k] = tile[T::KC + (2 * t + (k & 1) + (k >> 1) * 8) * (HD / 16) + (g * (HD / 8)) / 16 + u];
-                uint32_t nan_keys = 0;
-                if (EDGE) {
-                    // keys that no row sees may hold anything, and a NaN that some rows see must not reach the others (0 * NaN
-                    // is NaN): both count as zero here, and the rows that see a NaN get theirs below
+                for (int k = 0; k < 4; ++k) {
+                    const int key = 2 * t + (k & 1) + (k >> 1) * 8;
+                    const bool in = key0 + key >= kv_lo && key0 + key < kv_hi;
+                    if (in && by[k] == Q4_NAN) nan_keys |= 1u << key;
+                    if (!in || by[k] == Q4_NAN) by[k] = 0;
+                }
+            }
+            const QaStep s01(by[0] * 0x80u + by[1] * 0x800000u), s89(by[2] * 0x80u + by[3] * 0x800000u);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int key = 2 * t + (k & 1) + (k >> 1) * 8;
-                        const bool in = key0 + key >= kv_lo && key0 + key < kv_hi;
-                        if (in && by[k] == Q4_NAN) nan_keys |= 1u << key;
-                        if (!in || by[k] == Q4_NAN) by[k] = 0;
+            for (int v = 2 * u; v < VW && v < 2 * u + 2; ++v) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {             // codes 0-3 and 4-7 of the words
+                    const uint32_t sel = half ? 0x7632u : 0x5410u;
+                    uint32_t a[4], b[4];
+                    qa_widen(a, __byte_perm(w4[0][v], w4[1][v], sel), s01, magic);
+                    qa_widen(b, __byte_perm(w4[2][v], w4[3][v], sel), s89, magic);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        qa_mma(o[4 * v + 2 * half][n], a[0], a[1], b[0], b[1], pf[n][0], pf[n][1]);
+                        qa_mma(o[4 * v + 2 * half + 1][n], a[2], a[3], b[2], b[3], pf[n][0], pf[n][1]);
                     }
                 }
-                const QaStep s01(by[0] * 0x80u + by[1] * 0x800000u), s89(by[2] * 0x80u + by[3] * 0x800000u);
-#pragma unroll
-                for (int v = 2 * u; v < VW && v < 2 * u + 2; ++v) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {         // codes 0-3 and 4-7 of the words
-                        const uint32_t sel = half ? 0x7632u : 0x5410u;
-                        uint32_t a[4], b[4];
-                        qa_widen(a, __byte_perm(w4[0][v], w4[1][v], sel), s01, magic);
-                        qa_widen(b, __byte_perm(w4[2][v], w4[3][v], sel), s89, magic);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            qa_mma(o[4 * v + 2 * half][n], a[0], a[1], b[0], b[1], pf[i][n][0], pf[i][n][1]);
-                            qa_mma(o[4 * v + 2 * half + 1][n], a[2], a[3], b[2], b[3], pf[i][n][0], pf[i][n][1]);
-                        }
-                    }
-                }
-                if (EDGE) {
-                    nan_keys |= __shfl_xor_sync(0xffffffffu, nan_keys, 1);
-                    nan_keys |= __shfl_xor_sync(0xffffffffu, nan_keys, 2);
-                    if (nan_keys == 0) continue;
+            }
+            if (EDGE) {
+                nan_keys |= __shfl_xor_sync(0xffffffffu, nan_keys, 1);
+                nan_keys |= __shfl_xor_sync(0xffffffffu, nan_keys, 2);
+                if (nan_keys != 0) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -504,22 +538,30 @@ attention_q4_kernel(const QaParams p) {
             }
         }
     };
-    for (int j = 0;; ++j) {
-        const int first = chunk_tile(j), n_tiles = min(QA_KT, tile1 - first);
+    // Chunks that every row sees whole go through a loop of their own: joined with the masked code behind one
+    // branch, the compiler moved the accumulators from register to register every tile.
+    for (int j = 0, stage = 0;;) {
+        auto take = [&](auto edge, int n_tiles) {
+            qa_copy_wait<QA_STAGES - 1>();
+            __syncwarp();                                          // every lane's pieces are there
+            const int first = chunk_tile(j);
+#pragma unroll 1
+            for (int i = 0; i < n_tiles; ++i) fold(edge, (first + i) * 16, ring + (stage * QA_KT + i) * T::BYTES);
+            __syncwarp();                                          // every lane is done with the stage
+            request(j + QA_STAGES, next, stage);
+            next = pages(j + QA_STAGES + 1);
+            ++j;
+            if (++stage == QA_STAGES) stage = 0;
+        };
+        while (chunk_tile(j) >= clear0 && chunk_tile(j) + QA_KT <= clear1) take(std::false_type(), QA_KT);
+        const int n_tiles = min(QA_KT, tile1 - chunk_tile(j));
         if (n_tiles <= 0) break;
-        const uint8_t* const stage = ring + at * (QA_KT * T::BYTES);
-        if (!mbar_wait(bars + 8 * at, phase, 0)) mbar_wait(bars + 8 * at, phase, 0);      // its copies must not outlive the CTA
-        if (n_tiles < QA_KT || (first + QA_KT) * 16 - 1 > pos_first || (p.window > 0 && first * 16 <= pos_last - p.window))
-            chunk(std::true_type(), first, n_tiles, stage);
-        else
-            chunk(std::false_type(), first, QA_KT, stage);
-        __syncwarp();                                              // every lane is done with the stage
-        request(j + QA_STAGES, next_entry, at);
-        next_entry = my_page(j + QA_STAGES + 1);
-        if (++at == QA_STAGES) { at = 0; phase ^= 1; }
+        take(std::true_type(), n_tiles);
     }
+    qa_copy_wait<0>();
 
-    // ---- the warps' results side by side in shared memory (the rings are free), merged by all threads
+    // ---- the warps' results side by side in shared memory, merged by all threads; the next pair's keys and
+    // queries are on their way meanwhile
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -527,14 +569,6 @@ attention_q4_kernel(const QaParams p) {
             l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 4);
             l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 8);
             l[n][c] += __shfl_xor_sync(0xffffffffu, l[n][c], 16);
-        }
-    __syncthreads();
-    float* const mo = reinterpret_cast<float*>(qa_smem);                       // [warp][row][PITCH]
-    float2* const ml = reinterpret_cast<float2*>(mo + QA_WARPS * R * T::PITCH);  // [warp][row]
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
             const int r = 8 * n + 2 * t + c;
             float* const dst = mo + (warp * R + r) * T::PITCH + g * (HD / 8);
 #pragma unroll
@@ -542,8 +576,27 @@ attention_q4_kernel(const QaParams p) {
             if (g == 0) ml[warp * R + r] = make_float2(m[n][c], l[n][c]);
         }
     __syncthreads();
-    const bool whole_pair = off == 0 && tile1 - tile0 == it.tiles;
-    const long long part0 = (2ll * blockIdx.x + (off == 0 || f > f_begin ? 1 : 0)) * R;
+    const bool whole_pair = off == 0 && tile1 - tile0 == it.tiles, began_here = off == 0 || f > f_begin;
+    const uint32_t pair_begin = f - off;
+    const int pair_tiles = it.tiles, head0 = kvh * p.group;
+    f += tile1 - tile0;
+    if (f < f1) {
+        // (the range goes on: the pair ended, the next one is another head of the item or the next item that has tiles)
+        if (++kvh == p.kv.kv_heads) {
+            kvh = 0;
+            do { ++item; it = QaItem(p, min(item, p.n_items - 1), R); } while (it.tiles == 0 && item < p.n_items);
+        }
+        off = 0;
+        begin_pair(it, kvh, off);
+        load_queries(it, kvh);
+    }
+    auto write_out = [&](int r, int d, const float4& acc, float sum) {
+        const float inv = 128.f / sum;                             // (values carry a 1 / 128, as keys do)
+        const int row = row0 + r, tok = q_start + row / p.group, head = head0 + row % p.group;
+        const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), b = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(p.out + ((long long)tok * p.heads + head) * HD + d) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    };
     for (int e = threadIdx.x; e < rows * (HD / 4); e += QA_THREADS) {
         const int r = e / (HD / 4), d = e % (HD / 4) * 4;
         float top = -INFINITY;
@@ -555,118 +608,79 @@ attention_q4_kernel(const QaParams p) {
 #pragma unroll
         for (int w = 0; w < QA_WARPS; ++w) {
             const float2 x = ml[w * R + r];
-            const float f = qa_ex2(x.x - use);
+            const float wt = qa_ex2(x.x - use);
             const float4 v = *reinterpret_cast<const float4*>(mo + (w * R + r) * T::PITCH + d);
-            sum = fmaf(x.y, f, sum);
-            acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+            sum = fmaf(x.y, wt, sum);
+            acc.x = fmaf(v.x, wt, acc.x); acc.y = fmaf(v.y, wt, acc.y); acc.z = fmaf(v.z, wt, acc.z); acc.w = fmaf(v.w, wt, acc.w);
         }
-        if (!whole_pair) {
-            *reinterpret_cast<float4*>(p.part_o + (part0 + r) * HD + d) = acc;
-            if (d == 0) p.part_ml[part0 + r] = make_float2(top, sum);
-        } else {
-            const float inv = 128.f / sum;                         // (values carry a 1 / 128, as keys do)
-            const int row = row0 + r, tok = q_start + row / p.group, head = kvh * p.group + row % p.group;
-            const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), b = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-            *reinterpret_cast<uint2*>(p.out + ((long long)tok * p.heads + head) * HD + d) =
-                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        if (whole_pair) write_out(r, d, acc, sum);
+        else {
+            const long long at = (2ll * blockIdx.x + began_here) * R + r;
+            __stcg(reinterpret_cast<float4*>(p.part_o + at * HD + d), acc);
+            if (d == 0) __stcg(p.part_ml + at, make_float2(top, sum));
         }
     }
-    f += tile1 - tile0;
-    if (f >= start + it.tiles * p.kv.kv_heads) { start += it.tiles * p.kv.kv_heads; ++item; }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the next pair's copies overwrite what was merged here
-    __syncthreads();
+    if (!whole_pair) {
+        const int c0 = (int)(pair_begin / per), c1 = (int)((pair_begin + pair_tiles - 1) / per);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            last = atomicAdd(p.arrived + c0, 1u) == (unsigned)(c1 - c0);
+            if (last) p.arrived[c0] = 0;                           // ready for the next launch
+        }
+        __syncthreads();
+        if (last) {
+            __threadfence();
+            constexpr int S = 8;                                   // pieces asked for together
+            for (int e = threadIdx.x; e < rows * (HD / 4); e += QA_THREADS) {
+                const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+                float top = -INFINITY, sum = 0.f;
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int s0 = c0; s0 <= c1; s0 += S) {
+                    float2 x[S];
+                    float4 v[S];
+#pragma unroll
+                    for (int q = 0; q < S; ++q) {
+                        const int c = s0 + q;
+                        // the pair begins in c0's range, and before all of the others'
+                        const long long at = (2ll * c + (c == c0)) * R + r;
+                        x[q] = c <= c1 ? __ldcg(p.part_ml + at) : make_float2(-INFINITY, 0.f);
+                        v[q] = c <= c1 ? __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                    float up = top;
+#pragma unroll
+                    for (int q = 0; q < S; ++q) up = fmaxf(up, x[q].x);
+                    const float use = up == -INFINITY ? 0.f : up, was = qa_ex2(top - use);
+                    top = up;
+                    sum *= was; acc.x *= was; acc.y *= was; acc.z *= was; acc.w *= was;
+#pragma unroll
+                    for (int q = 0; q < S; ++q) {
+                        const float wt = qa_ex2(x[q].x - use);
+                        sum = fmaf(x[q].y, wt, sum);
+                        acc.x = fmaf(v[q].x, wt, acc.x); acc.y = fmaf(v[q].y, wt, acc.y); acc.z = fmaf(v[q].z, wt, acc.z); acc.w = fmaf(v[q].w, wt, acc.w);
+                    }
+                }
+                write_out(r, d, acc, sum);
+            }
+        }
     }
-}
-
-// The pieces of each pair that fell to several CTAs, folded in ascending order.  GROUPS 1: a CTA per pair, a thread
-// for four channels of a row (many pairs, few pieces each).  GROUPS > 1: a CTA per pair and row, whose
-// threads take every GROUPS-th piece and are added up in shared memory (few pairs, many pieces).
-constexpr int QA_FOLD_THREADS = 256;
-template <int HD, int NT, int GROUPS>
-__global__ void __launch_bounds__(QA_FOLD_THREADS) attention_q4_fold_kernel(const QaParams p) {
-    constexpr int R = 8 * NT, V = HD / 4, S = 8;
-    __shared__ float4 sums[GROUPS > 1 ? QA_FOLD_THREADS : 1];
-    __shared__ float parts[GROUPS > 1 ? GROUPS : 1];
-    pdl_launch_dependents();
-    pdl_wait();
-    const int item = blockIdx.x / p.kv.kv_heads, kvh = blockIdx.x % p.kv.kv_heads;
-    const QaItem it(p, item, R);
-    const QaRanges all(p, R);
-    const uint32_t begin = QaRanges::before(p, item, R) + kvh * it.tiles;
-    const int c0 = (int)(begin / all.per), c1 = (int)((begin + it.tiles - 1) / all.per);
-    if (c0 == c1 || it.tiles == 0) return;                         // written whole
-    const int group = GROUPS > 1 ? threadIdx.x / V : 0;
-    for (int e = GROUPS > 1 ? threadIdx.x % V + blockIdx.y * V : threadIdx.x; e < it.rows * V; e += GROUPS > 1 ? R * V : QA_FOLD_THREADS) {
-        const int r = e / V, d = e % V;
-        float top = -INFINITY, sum = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s0 = c0 + group; s0 <= c1; s0 += S * GROUPS) {
-            float2 ml[S];
-            float4 v[S];
-#pragma unroll
-            for (int q = 0; q < S; ++q) {
-                const int c = s0 + q * GROUPS;
-                // the pair begins in c0's range, or lies before all of the others'
-                const long long at = (2ll * c + (c == c0 ? 1 : 0)) * R + r;
-                ml[q] = c <= c1 ? __ldcg(p.part_ml + at) : make_float2(-INFINITY, 0.f);
-                v[q] = c <= c1 ? __ldcg(reinterpret_cast<const float4*>(p.part_o) + at * V + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            float m = top;
-#pragma unroll
-            for (int q = 0; q < S; ++q) m = fmaxf(m, ml[q].x);
-            const float use = m == -INFINITY ? 0.f : m, f = qa_ex2(top - use);
-            top = m;
-            sum *= f; acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-#pragma unroll
-            for (int q = 0; q < S; ++q) {
-                const float w = qa_ex2(ml[q].x - use);
-                sum = fmaf(ml[q].y, w, sum);
-                acc.x = fmaf(v[q].x, w, acc.x); acc.y = fmaf(v[q].y, w, acc.y); acc.z = fmaf(v[q].z, w, acc.z); acc.w = fmaf(v[q].w, w, acc.w);
-            }
-        }
-        if constexpr (GROUPS > 1) {
-            // (one row per CTA: all threads are here)
-            __shared__ float tops[GROUPS];
-            sums[threadIdx.x] = acc;
-            if (d == 0) { tops[group] = top; parts[group] = sum; }
-            __syncthreads();
-            if (group > 0) return;
-            float m = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < GROUPS; ++k) m = fmaxf(m, tops[k]);
-            const float use = m == -INFINITY ? 0.f : m;
-            sum = 0.f;
-            acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < GROUPS; ++k) {
-                const float w = qa_ex2(tops[k] - use);
-                const float4 v = sums[k * V + d];
-                sum = fmaf(parts[k], w, sum);
-                acc.x = fmaf(v.x, w, acc.x); acc.y = fmaf(v.y, w, acc.y); acc.z = fmaf(v.z, w, acc.z); acc.w = fmaf(v.w, w, acc.w);
-            }
-        }
-        const float inv = 128.f / sum;
-        const int row = it.row0 + r, tok = it.q_start + row / p.group, head = kvh * p.group + row % p.group;
-        const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), b = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-        *reinterpret_cast<uint2*>(p.out + ((long long)tok * p.heads + head) * HD + 4 * d) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    if (f >= f1) break;
+    __syncthreads();                                               // the next pair's results overwrite what was merged here
     }
 }
 
 template <int HD, int NT>
 static int launch_q4(const QaParams& p, cudaStream_t stream) {
-    constexpr int smem = QaTile<HD>::smem(NT), groups = QA_FOLD_THREADS / (HD / 4);
+    constexpr int smem = QaTile<HD>::smem(NT);
     static_assert(smem <= 226 * 1024, "the rings do not fit shared memory");
-    if (int st = ensure_dynamic_smem<attention_q4_kernel<HD, NT>>(smem, "axon_attention_q4")) return st;
-    launch_pdl(attention_q4_kernel<HD, NT>, dim3(p.ctas), dim3(QA_THREADS), smem, stream, p);
-    if (int st = launch_status("axon_attention_q4")) return st;
-    const int pairs = p.n_items * p.kv.kv_heads;
-    // a pair is cut into at most ctas / pairs + 2 pieces if all are alike; with few pairs there are many
-    if (pairs * 4 < p.ctas)
-        launch_pdl(attention_q4_fold_kernel<HD, NT, groups>, dim3(pairs, 8 * NT), dim3(QA_FOLD_THREADS), 0, stream, p);
-    else
-        launch_pdl(attention_q4_fold_kernel<HD, NT, 1>, dim3(pairs), dim3(QA_FOLD_THREADS), 0, stream, p);
-    return launch_status("axon_attention_q4 fold");
+    if (p.kv.page_size == 16) {
+        if (int st = ensure_dynamic_smem<attention_q4_kernel<HD, NT, true>>(smem, "axon_attention_q4")) return st;
+        launch_pdl(attention_q4_kernel<HD, NT, true>, dim3(p.ctas), dim3(QA_THREADS), smem, stream, p);
+    } else {
+        if (int st = ensure_dynamic_smem<attention_q4_kernel<HD, NT, false>>(smem, "axon_attention_q4")) return st;
+        launch_pdl(attention_q4_kernel<HD, NT, false>, dim3(p.ctas), dim3(QA_THREADS), smem, stream, p);
+    }
+    return launch_status("axon_attention_q4");
 }
 
 }  // namespace axon
@@ -676,8 +690,9 @@ using namespace axon;
 // How many CTAs an attention launch has (two fit an SM with one tile of 8 rows, up to head size 128).
 AXON_API int axon_attention_q4_ctas(int head_dim, int row_tiles) { return (row_tiles == 1 && head_dim <= 128 ? 2 : 1) * 148; }
 
-// Attention of `n_items` tiles of up to 8 * row_tiles query rows (row_tiles 1, 2 or 4; at head size 256 1 or 2).  items null:
-// item i is segment i, whose rows all fit one tile.  scratch: 2 * ctas * 8 * row_tiles * (head_dim + 2) floats.
+// Attention of `n_items` tiles of up to 8 * row_tiles query rows (row_tiles 1, 2 or 4; at head size 256 1).  items null:
+// item i is segment i, whose rows all fit one tile.  scratch: 2 * ctas * 8 * row_tiles * (head_dim + 2) + ctas floats, zeroed once:
+// launches leave the last ctas of them zero.
 AXON_API int axon_attention_q4(const void* q, const void* pool, void* out, const int32_t* segments, int n_segments,
                                const int32_t* items, int n_items, const AxonKvLayout* layout, int heads, float scale, int window,
                                int row_tiles, float* scratch, long long scratch_floats, cudaStream_t stream) {
@@ -689,29 +704,22 @@ AXON_API int axon_attention_q4(const void* q, const void* pool, void* out, const
     if (heads < 1 || heads % p.kv.kv_heads) { set_error("axon_attention_q4: %d heads over %d kv heads", heads, p.kv.kv_heads); return AXON_BAD_ARGUMENT; }
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)scratch) & 15) { set_error("axon_attention_q4: operands must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
     if ((double)n_items * p.kv.kv_heads * ((double)p.kv.table_stride * p.kv.page_size / 16 + 1) > 2147483647.0) { set_error("axon_attention_q4: %d items of %d kv heads at up to %d pages are too many", n_items, p.kv.kv_heads, p.kv.table_stride); return AXON_BAD_ARGUMENT; }
-    p.run = 1;
-    while (p.run < 16 && p.kv.page_size % (2 * p.run) == 0) p.run *= 2;
-    // a copy moves whole 16 bytes, and a lane each must do for the pieces of a chunk
-    if (p.run * hd / 16 % 16 || QA_KT * (p.kv.page_size == 16 ? 1 : 64 / p.run) > 32) { set_error("axon_attention_q4: pages of %d positions of %d values do not fall into pieces it can copy", p.kv.page_size, hd); return AXON_BAD_ARGUMENT; }
+    // a copy moves 16 bytes: at head size 64 the steps of four positions, which have to lie in one page
+    if (p.kv.page_size % (hd >= 256 ? 1 : 256 / hd)) { set_error("axon_attention_q4: pages of %d positions of %d values do not fall into pieces it can copy", p.kv.page_size, hd); return AXON_BAD_ARGUMENT; }
     p.ctas = axon_attention_q4_ctas(hd, row_tiles);
     const long long rows = 2ll * p.ctas * 8 * row_tiles;
-    if (scratch == nullptr || scratch_floats < rows * (hd + 2)) { set_error("axon_attention_q4: needs %lld floats of scratch", rows * (hd + 2)); return AXON_BAD_ARGUMENT; }
+    if (scratch == nullptr || scratch_floats < rows * (hd + 2) + p.ctas) { set_error("axon_attention_q4: needs %lld floats of zeroed scratch", rows * (hd + 2) + p.ctas); return AXON_BAD_ARGUMENT; }
     p.q = (const __nv_bfloat16*)q; p.pool = (const uint8_t*)pool; p.out = (__nv_bfloat16*)out;
     p.segments = segments; p.items = items;
     p.part_o = scratch; p.part_ml = reinterpret_cast<float2*>(scratch + rows * hd);
+    p.arrived = reinterpret_cast<unsigned int*>(scratch + rows * (hd + 2));
     p.n_segments = n_segments; p.n_items = n_items; p.heads = heads; p.group = heads / p.kv.kv_heads; p.window = window;
     p.scale_log2 = scale * 1.4426950408889634f;
 #define AXON_Q4_CASE(HD, NT) if (hd == HD && row_tiles == NT) return launch_q4<HD, NT>(p, stream)
     AXON_Q4_CASE(64, 1); AXON_Q4_CASE(64, 2); AXON_Q4_CASE(64, 4);
     AXON_Q4_CASE(128, 1); AXON_Q4_CASE(128, 2); AXON_Q4_CASE(128, 4);
-    AXON_Q4_CASE(256, 1); AXON_Q4_CASE(256, 2);
+    AXON_Q4_CASE(256, 1);
 #undef AXON_Q4_CASE
     set_error("axon_attention_q4: no kernel for head size %d with %d tiles of 8 rows", hd, row_tiles);
     return AXON_BAD_ARGUMENT;
-}
-
-AXON_API int axon_attention_q4_status() {
-    unsigned int v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_tc_error, sizeof v) != cudaSuccess) return -1;
-    return (int)v;
 }

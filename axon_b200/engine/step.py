@@ -314,8 +314,7 @@ class Engine:
         if self.rt.precise:
             return
         from ..kernels import fast
-        for what, status in (("product", fast.gemm_tc_status()), ("attention", fast.attention_tc_status()),
-                             ("4-bit attention", fast.attention_q4_status())):
+        for what, status in (("product", fast.gemm_tc_status()), ("attention", fast.attention_tc_status())):
             if status:
                 raise DeviceFault(f"a tensor-core {what} kernel gave up waiting (status {status}: 1 + the role that "
                                   "waited: 0 loads, 1 MMA, 2 epilogue; 100: misaligned shared memory)")

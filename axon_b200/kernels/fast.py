@@ -368,7 +368,7 @@ def q4_plain_splits(ctx, heads: int, kv_heads: int, window: int) -> int:
 
 
 #: row tiles of 8 that the kernel holds at once, by head size
-Q4_ROW_TILES = {64: 4, 128: 4, 256: 2}
+Q4_ROW_TILES = {64: 4, 128: 4, 256: 1}
 
 
 def _q4_row_tiles(rows: int, hd: int) -> int:
@@ -394,12 +394,13 @@ def _q4_items(ctx, group: int, hd: int):
 
 
 def _q4_takes(hd: int, page_size: int) -> bool:
-    return hd in Q4_ROW_TILES and page_size % 4 == 0
+    return hd in Q4_ROW_TILES and page_size % max(1, 256 // hd) == 0
 
 
 def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
-    """Tensor-core attention over a 4-bit cache; refuses head sizes other than 64, 128 and 256, pages of a
-    number of positions that is no multiple of 4, and dtypes other than bfloat16."""
+    """Tensor-core attention over a 4-bit cache; refuses head sizes other than 64, 128 and 256, dtypes
+    other than bfloat16, and pages whose 16-byte pieces of steps would straddle them (a multiple of 4 positions
+    is needed at head size 64, of 2 at 128)."""
     if not ENABLED["attention_q4"] or ctx.segments is None or not _q4_takes(kv.head_dim, kv.page_size):
         return False
     if kv.planes != 2 or kv.v_dim != kv.head_dim or heads % kv.kv_heads:
@@ -408,17 +409,13 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
         return False
     nt, n_items, items = _q4_items(ctx, heads // kv.kv_heads, kv.head_dim)
     cu = lib.cuda()
-    floats = 2 * cu.axon_attention_q4_ctas(kv.head_dim, nt) * 8 * nt * (kv.head_dim + 2)
-    scratch = ctx.rt.buffer(f"q4_scratch_{kv.head_dim}_{nt}", (floats,), torch.float32)
+    ctas = cu.axon_attention_q4_ctas(kv.head_dim, nt)
+    floats = 2 * ctas * 8 * nt * (kv.head_dim + 2) + ctas
+    scratch = ctx.rt.zeroed_buffer(f"q4_scratch_{kv.head_dim}_{nt}", (floats,), torch.float32)
     check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
                                None if items is None else items.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
                                nt, scratch.data_ptr(), floats, _stream()))
     return True
-
-
-def attention_q4_status() -> int:
-    """0 when no 4-bit attention ever gave up on a wait (synchronises the device)."""
-    return lib.cuda().axon_attention_q4_status()
 
 
 def q4_graph_key(ctx, heads: int, kv_heads: int, head_dim: int, window: int, precise: bool):

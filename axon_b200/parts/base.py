@@ -75,6 +75,14 @@ class Runtime:
             self._buffers[name] = buf
         return buf[:n].view(shape)
 
+    def zeroed_buffer(self, name: str, shape: Tuple[int, ...], dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """A scratch buffer that is zero when it is first handed out (its users leave zero what must be)."""
+        before = self._buffers.get(name)
+        buf = self.buffer(name, shape, dtype)
+        if self._buffers[name] is not before:
+            self._buffers[name].zero_()
+        return buf
+
     def upload_i32(self, name: str, values) -> torch.Tensor:
         """Host integers (a work list, say) as a device tensor.  The same list under the same name
         is uploaded once and kept, so steps of a shape seen before copy nothing, and a CUDA graph
