@@ -36,7 +36,10 @@ namespace axon {
 
 constexpr int QA_WARPS = 8, QA_THREADS = QA_WARPS * 32;
 constexpr int QA_KT = 2, QA_STAGES = 2;          // 16-key tiles per chunk, chunks in a warp's ring
-constexpr int QA_LEAST = QA_WARPS * QA_KT;       // tiles below which a range is not cut further: one chunk for each warp
+// A pair counts as its tiles and so many more when ranges are cut: what starting on it and merging the warps'
+// results cost the CTA, in tiles (with none, CTAs that met a dozen short requests finished last: see the launch bench of ragged contexts).
+constexpr int QA_PAIR_COST = 8;
+constexpr int QA_LEAST = QA_WARPS * QA_KT;       // the shortest range: one chunk for each warp
 constexpr float QA_LAZY = 8.f;                   // log2 units a score may exceed the running maximum
 
 struct QaParams {
@@ -99,9 +102,9 @@ __device__ __forceinline__ uint32_t qa_mul2(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 // (w & mask) | magic in one instruction: with both as constants the compiler takes two, as an instruction holds one.
-__device__ __forceinline__ uint32_t qa_pick(uint32_t w, uint32_t mask, uint32_t magic) {
+template <uint32_t MASK> __device__ __forceinline__ uint32_t qa_pick(uint32_t w, uint32_t magic) {
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));
     return r;
 }
 // The exponents under which a code in bits 0-3 (8 + c / 128) and one in bits 4-7 (0.5 + c / 128) are read, in
@@ -125,10 +128,10 @@ struct QaStep {
 // The codes in bits 0-3, 4-7, 8-11 and 12-15 of both halves of w, times their steps / 128.
 __device__ __forceinline__ void qa_widen(uint32_t (&p)[4], uint32_t w, const QaStep& st, const QaMagic& magic) {
     const uint32_t v = w >> 8;
-    p[0] = qa_fma2(qa_pick(w, 0x000F000Fu, magic.low), st.s, st.low);
-    p[1] = qa_fma2(qa_pick(w, 0x00F000F0u, magic.high), st.s, st.high);
-    p[2] = qa_fma2(qa_pick(v, 0x000F000Fu, magic.low), st.s, st.low);
-    p[3] = qa_fma2(qa_pick(v, 0x00F000F0u, magic.high), st.s, st.high);
+    p[0] = qa_fma2(qa_pick<0x000F000Fu>(w, magic.low), st.s, st.low);
+    p[1] = qa_fma2(qa_pick<0x00F000F0u>(w, magic.high), st.s, st.high);
+    p[2] = qa_fma2(qa_pick<0x000F000Fu>(v, magic.low), st.s, st.low);
+    p[3] = qa_fma2(qa_pick<0x00F000F0u>(v, magic.high), st.s, st.high);
 }
 template <int N> __device__ __forceinline__ void qa_lds(uint32_t (&r)[N], const uint8_t* p) {
     if constexpr (N % 4 == 0) {
@@ -149,13 +152,11 @@ template <int N> __device__ __forceinline__ void qa_lds(uint32_t (&r)[N], const 
 // 2^-e so that the row's largest element lies in [1, 2), and by -1 for a negative scale, as the B operand's
 // registers.  Returns the factor that brings scores to log2 units (keys carry a 1 / 128), which is not negative.
 template <int HD>
-__device__ __forceinline__ float qa_load_query(uint32_t (&f)[HD / 16][2], const __nv_bfloat16* row, int t, bool live, float scale_log2) {
+__device__ __forceinline__ float qa_query(uint32_t (&f)[HD / 16][2], const uint4 (&raw)[HD / 32], float scale_log2) {
     constexpr int W = HD / 32;
-    uint4 raw[W];
     uint32_t top = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-        raw[w] = live ? reinterpret_cast<const uint4*>(row + t * (HD / 4))[w] : make_uint4(0, 0, 0, 0);
         const uint32_t u[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = max(top, max(u[i] & 0x7fffu, (u[i] >> 16) & 0x7fffu));
@@ -193,38 +194,68 @@ struct QaItem {
         const int q_len = p.segments[2 * p.n_segments + seg], kv_len = p.segments[3 * p.n_segments + seg];
         rows = min(most_rows, q_len * p.group - row0);
         pos0 = kv_len - q_len;
-        pos_first = pos0 + row0 / p.group;
-        pos_last = pos0 + (row0 + rows - 1) / p.group;
+        pos_first = pos0;
+        pos_last = kv_len - 1;
+        if (p.items) {                                             // a part of a segment's rows
+            pos_first = pos0 + row0 / p.group;
+            pos_last = pos0 + (row0 + rows - 1) / p.group;
+        }
         kv_hi = pos_last + 1;
         kv_lo = (p.window > 0 && pos_first - p.window + 1 > 0) ? pos_first - p.window + 1 : 0;
         tile0 = kv_lo / 16;
         tiles = rows > 0 ? max((kv_hi + 15) / 16 - tile0, 0) : 0;
     }
 };
-// How the tiles of all pairs, laid end to end (items in order, the kv heads of each in order), fall to the
-// CTAs: `per` each.  Every warp works it out for itself, 32 items at a time.  (The launcher has seen to it that a full
-// block table counts in 32 bits.)
-struct QaRanges {
-    uint32_t total, per;
-    __device__ __forceinline__ QaRanges(const QaParams& p, int most_rows) {
-        uint32_t sum = 0, longest = 0;
-        for (int i = threadIdx.x & 31; i < p.n_items; i += 32) {
+// How all pairs, laid end to end (items in order, the kv heads of each in order), fall to the CTAs: a range
+// of `per` places each.  Where the pairs cut into pieces of equal length that start at their beginnings make no more
+// pieces than there are CTAs, a pair's tiles are padded to whole ranges, so that no CTA has two pieces; else pairs follow one
+// another without gaps but for `cost` places before each.  Every warp works it out for itself, 32 items at a
+// time.  (The launcher has seen to it that full block tables count in 32 bits.)
+struct QaPlan {
+    uint32_t total, per, cost;
+    bool padded;
+    // what a pair of `tiles` takes: its cost, then its tiles
+    __device__ __forceinline__ uint32_t weight(uint32_t tiles) const {
+        return tiles == 0 ? 0 : padded ? (tiles + per - 1) / per * per : tiles + cost;
+    }
+    __device__ __forceinline__ uint32_t sum(const QaParams& p, int most_rows, uint32_t mine) const {
+        const int lane = threadIdx.x & 31;
+        uint32_t x = weight(mine);                                 // (the first 32 items' tiles are in registers)
+        for (int i = lane + 32; i < p.n_items; i += 32) x += weight(QaItem(p, i, most_rows).tiles);
+        return __reduce_add_sync(0xffffffffu, x) * p.kv.kv_heads;
+    }
+    // `item`: the one that this CTA's range begins in, `start`: where its first pair begins
+    __device__ __forceinline__ QaPlan(const QaParams& p, int most_rows, int* item, uint32_t* start) {
+        const int lane = threadIdx.x & 31;
+        const uint32_t mine = lane < p.n_items ? QaItem(p, lane, most_rows).tiles : 0;
+        uint32_t tiles = mine, longest = mine;
+        for (int i = lane + 32; i < p.n_items; i += 32) {
             const uint32_t n = QaItem(p, i, most_rows).tiles;
-            sum += n;
+            tiles += n;
             longest = max(longest, n);
         }
-        total = __reduce_add_sync(0xffffffffu, sum) * p.kv.kv_heads;
+        tiles = __reduce_add_sync(0xffffffffu, tiles) * p.kv.kv_heads;
         longest = __reduce_max_sync(0xffffffffu, longest);
         // one CTA folds a pair's pieces: with few long pairs, as long a range (a turn of 16 tiles takes about 0.9 us) as the
         // fold of as many pieces (0.05 us each) would take, which is about the square root of a pair's tiles
-        per = max(max((uint32_t)QA_LEAST, (uint32_t)sqrtf((float)longest)), (total + p.ctas - 1) / p.ctas);
-    }
-    // the item that tile f falls into, and the tiles before it
-    static __device__ __forceinline__ int find(const QaParams& p, uint32_t f, int most_rows, uint32_t* start) {
-        const int lane = threadIdx.x & 31;
+        const uint32_t least = max((uint32_t)QA_LEAST, (uint32_t)sqrtf((float)longest));
+        const uint32_t even = (tiles + p.ctas - 1) / p.ctas;
+        padded = true;
+        cost = 0;
+        per = (max(least, even) + QA_LEAST - 1) / QA_LEAST * QA_LEAST;
+        total = sum(p, most_rows, mine);
+        if (total > p.ctas * per) {
+            padded = false;
+            cost = QA_PAIR_COST;
+            total = sum(p, most_rows, mine);
+            per = max(least, (total + p.ctas - 1) / p.ctas);
+        }
+        // the item of this CTA's first place
+        const uint32_t f = blockIdx.x * per;
         uint32_t base = 0;
+        *item = p.n_items;
         for (int i0 = 0; i0 < p.n_items; i0 += 32) {
-            const uint32_t n = i0 + lane < p.n_items ? QaItem(p, i0 + lane, most_rows).tiles * p.kv.kv_heads : 0;
+            const uint32_t n = (i0 == 0 ? weight(mine) : i0 + lane < p.n_items ? weight(QaItem(p, i0 + lane, most_rows).tiles) : 0) * p.kv.kv_heads;
             uint32_t upto = n;                                     // of this item and those before it in the 32
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -235,15 +266,15 @@ struct QaRanges {
             if (past) {
                 const int who = __ffs(past) - 1;
                 *start = base + __shfl_sync(0xffffffffu, upto - n, who);
-                return i0 + who;
+                *item = i0 + who;
+                break;
             }
             base += __shfl_sync(0xffffffffu, upto, 31);
         }
-        *start = base;
-        return p.n_items;
     }
 };
 
+// WHOLE: pages of 16 positions, table entries not checked (a check may store, which keeps the copies behind it apart).
 template <int HD, int NT, bool WHOLE>
 __global__ void __launch_bounds__(QA_THREADS, (NT == 1 && HD <= 128) ? 2 : 1)
 attention_q4_kernel(const QaParams p) {
@@ -263,17 +294,12 @@ attention_q4_kernel(const QaParams p) {
     pdl_launch_dependents();
     pdl_wait();
 
-    uint32_t f, f1, start, per;
     int item;
-    {
-        const QaRanges all(p, R);
-        if (all.total == 0 || blockIdx.x > (all.total - 1) / all.per) return;
-        per = all.per;
-        f = blockIdx.x * per;
-        f1 = f + min(per, all.total - f);
-        item = QaRanges::find(p, f, R, &start);
-    }
-    const uint32_t f_begin = f;
+    uint32_t start;
+    const QaPlan plan(p, R, &item, &start);
+    if (item >= p.n_items) return;                                 // (nothing left for this CTA)
+    uint32_t f = blockIdx.x * plan.per;
+    const uint32_t f1 = f + min(plan.per, plan.total - f), per = plan.per;
     const QaMagic magic;
 
     // ---- copies: piece i of a chunk (of QA_KT * PIECES) is lane i % 32's
@@ -281,24 +307,23 @@ attention_q4_kernel(const QaParams p) {
     const uint8_t* head_src;                                       // the pair's record in page 0
     const int32_t* table;
     int tile0, tile1, last_page;
-    auto chunk_tile = [&](int j) { return tile0 + (warp + j * QA_WARPS) * QA_KT; };
+    constexpr int TURN = QA_WARPS * QA_KT;                         // tiles between two chunks of a warp
     struct Pages { int e[QA_KT]; };
-    auto pages = [&](int j) {                                     // table entries of the first positions of a chunk's tiles
+    auto pages = [&](int first) {                                 // table entries of the first positions of the tiles of the chunk at `first`
         Pages x;
-        const int first = chunk_tile(j);
 #pragma unroll
         for (int i = 0; i < QA_KT; ++i) x.e[i] = first + i < tile1 ? table[WHOLE ? first + i : (first + i) * 16 / ps] : 0;
         return x;
     };
-    auto request = [&](int j, const Pages& x, int stage) {
-        const int first = chunk_tile(j), n = min(QA_KT, tile1 - first);
+    auto request = [&](int first, const Pages& x, int stage) {
+        const int n = min(QA_KT, tile1 - first);
         if (n > 0) {
             const uint32_t dst = ring_addr + stage * (QA_KT * T::BYTES) + lane * 16;
             const int pieces = n * T::PIECES;
             if constexpr (WHOLE) {
                 const uint8_t* src[QA_KT];
 #pragma unroll
-                for (int i = 0; i < QA_KT; ++i) src[i] = head_src + (long long)p.kv.page(x.e[i]) * p.kv.page_stride + lane * 16 - i * T::BYTES;
+                for (int i = 0; i < QA_KT; ++i) src[i] = head_src + (long long)x.e[i] * p.kv.page_stride + lane * 16 - i * T::BYTES;
                 auto copy = [&](int k) {
                     const uint8_t* from = src[0];
 #pragma unroll
@@ -332,46 +357,76 @@ attention_q4_kernel(const QaParams p) {
         qa_copy_commit();
     };
     Pages next;
-    auto begin_pair = [&](const QaItem& it, int kvh, int off) {   // asks for the first keys of a pair's piece
-        tile0 = it.tile0 + off;
-        tile1 = tile0 + (int)min((uint32_t)(it.tiles - off), f1 - f);
+    QaItem it(p, item, R);
+    int off = 0;
+    uint32_t pair_weight = plan.weight(it.tiles);                  // (not zero: the plan gives an item that has tiles)
+    int kvh = (int)((f - start) / pair_weight);
+    uint32_t pair_begin = start + kvh * pair_weight;
+    // The next piece of the range: tiles off .. of the pair (it, kvh), f moved to its end; false when there is none.
+    auto advance = [&]() {
+        while (f < f1) {
+            const uint32_t from = f - pair_begin, to = min(pair_weight, f1 - pair_begin);      // within the pair
+            if (from >= pair_weight) {
+                pair_begin += pair_weight;
+                if (++kvh == p.kv.kv_heads) {
+                    kvh = 0;
+                    do { ++item; it = QaItem(p, min(item, p.n_items - 1), R); } while (it.tiles == 0 && item < p.n_items);
+                    if (item >= p.n_items) return false;
+                    pair_weight = plan.weight(it.tiles);
+                }
+                continue;
+            }
+            f = pair_begin + to;
+            if (to <= plan.cost) return false;                     // the range ends before the pair's first tile
+            off = max((int)(from - plan.cost), 0);
+            tile0 = it.tile0 + off;
+            tile1 = it.tile0 + min((int)(to - plan.cost), it.tiles);
+            return true;
+        }
+        return false;
+    };
+    // ---- a pair's piece begins: table entries, then this thread's share of the queries, are asked for, then the
+    // first keys; while they come queries become B fragments, with the factors that bring rows' scores to log2 units
+    uint32_t qf[NT == 1 ? HD / 16 : 1][2];
+    float factor[NT][2];
+    auto begin_pair = [&]() {
         head_src = p.pool + p.kv.entry_offset + (long long)kvh * p.kv.record;
         table = p.kv.block_table + (long long)it.slot * p.kv.table_stride;
         last_page = (it.kv_hi - 1) / ps;
         Pages x[QA_STAGES];
 #pragma unroll
-        for (int j = 0; j < QA_STAGES; ++j) x[j] = pages(j);
-        next = pages(QA_STAGES);
+        for (int j = 0; j < QA_STAGES; ++j) x[j] = pages(tile0 + warp * QA_KT + j * TURN);
+        next = pages(tile0 + warp * QA_KT + QA_STAGES * TURN);
+        const int r = NT == 1 ? g : 8 * warp + g, row = it.row0 + r;
+        const bool mine = NT == 1 || warp < NT, live = mine && r < it.rows;
+        uint4 raw[HD / 32];
+        if (live) {
+            const int ahead = row < p.group ? 0 : row / p.group;   // tokens of the segment before the row's
+            const uint4* const src = reinterpret_cast<const uint4*>(
+                p.q + ((long long)(it.q_start + ahead) * p.heads + kvh * p.group + row - ahead * p.group) * HD + t * (HD / 4));
 #pragma unroll
-        for (int j = 0; j < QA_STAGES; ++j) request(j, x[j], j);
-    };
-
-    // ---- queries as B fragments, and the factor that brings a row's scores to log2 units
-    uint32_t qf[NT == 1 ? HD / 16 : 1][2];
-    float factor[NT][2];
-    auto load_queries = [&](const QaItem& it, int kvh) {
-        auto query_row = [&](int r) {
-            const int row = it.row0 + (r < it.rows ? r : 0), tok = it.q_start + row / p.group, head = kvh * p.group + row % p.group;
-            return p.q + ((long long)tok * p.heads + head) * HD;
-        };
+            for (int w = 0; w < HD / 32; ++w) raw[w] = src[w];
+        } else {
+#pragma unroll
+            for (int w = 0; w < HD / 32; ++w) raw[w] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < QA_STAGES; ++j) request(tile0 + warp * QA_KT + j * TURN, x[j], j);
         if constexpr (NT == 1) {
-            const float x = qa_load_query<HD>(qf, query_row(g), t, g < it.rows, p.scale_log2);
-            factor[0][0] = __shfl_sync(0xffffffffu, x, 8 * t);
-            factor[0][1] = __shfl_sync(0xffffffffu, x, 8 * t + 4);
-        } else if (warp < NT) {                                    // (read back after the next barrier)
-            uint32_t x[HD / 16][2];
-            const int r = 8 * warp + g;
-            const float scale = qa_load_query<HD>(x, query_row(r), t, r < it.rows, p.scale_log2);
+            const float scale = qa_query<HD>(qf, raw, p.scale_log2);
+            factor[0][0] = __shfl_sync(0xffffffffu, scale, 8 * t);
+            factor[0][1] = __shfl_sync(0xffffffffu, scale, 8 * t + 4);
+        } else if (mine) {                                         // (read back after the next barrier)
+            uint32_t frag[HD / 16][2];
+            const float scale = qa_query<HD>(frag, raw, p.scale_log2);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) q_smem[(k * NT + warp) * 32 + lane] = make_uint2(x[k][0], x[k][1]);
+            for (int k = 0; k < HD / 16; ++k) q_smem[(k * NT + warp) * 32 + lane] = make_uint2(frag[k][0], frag[k][1]);
             if (t == 0) f_smem[r] = scale;
         }
     };
 
-    QaItem it(p, item, R);
-    int kvh = (int)((f - start) / it.tiles), off = (int)((f - start) % it.tiles);
-    begin_pair(it, kvh, off);
-    load_queries(it, kvh);
+    if (!advance()) return;
+    begin_pair();
     for (;;) {
     const int rows = it.rows, pos_first = it.pos_first, pos_last = it.pos_last, row0 = it.row0, q_start = it.q_start;
     const int kv_lo = it.kv_lo, kv_hi = it.kv_hi;
@@ -540,21 +595,20 @@ attention_q4_kernel(const QaParams p) {
     };
     // Chunks that every row sees whole go through a loop of their own: joined with the masked code behind one
     // branch, the compiler moved the accumulators from register to register every tile.
-    for (int j = 0, stage = 0;;) {
+    for (int at = tile0 + warp * QA_KT, stage = 0;;) {
         auto take = [&](auto edge, int n_tiles) {
             qa_copy_wait<QA_STAGES - 1>();
             __syncwarp();                                          // every lane's pieces are there
-            const int first = chunk_tile(j);
 #pragma unroll 1
-            for (int i = 0; i < n_tiles; ++i) fold(edge, (first + i) * 16, ring + (stage * QA_KT + i) * T::BYTES);
+            for (int i = 0; i < n_tiles; ++i) fold(edge, (at + i) * 16, ring + (stage * QA_KT + i) * T::BYTES);
             __syncwarp();                                          // every lane is done with the stage
-            request(j + QA_STAGES, next, stage);
-            next = pages(j + QA_STAGES + 1);
-            ++j;
+            request(at + QA_STAGES * TURN, next, stage);
+            next = pages(at + (QA_STAGES + 1) * TURN);
+            at += TURN;
             if (++stage == QA_STAGES) stage = 0;
         };
-        while (chunk_tile(j) >= clear0 && chunk_tile(j) + QA_KT <= clear1) take(std::false_type(), QA_KT);
-        const int n_tiles = min(QA_KT, tile1 - chunk_tile(j));
+        while (at >= clear0 && at + QA_KT <= clear1) take(std::false_type(), QA_KT);
+        const int n_tiles = min(QA_KT, tile1 - at);
         if (n_tiles <= 0) break;
         take(std::true_type(), n_tiles);
     }
@@ -576,23 +630,14 @@ attention_q4_kernel(const QaParams p) {
             if (g == 0) ml[warp * R + r] = make_float2(m[n][c], l[n][c]);
         }
     __syncthreads();
-    const bool whole_pair = off == 0 && tile1 - tile0 == it.tiles, began_here = off == 0 || f > f_begin;
-    const uint32_t pair_begin = f - off;
-    const int pair_tiles = it.tiles, head0 = kvh * p.group;
-    f += tile1 - tile0;
-    if (f < f1) {
-        // (the range goes on: the pair ended, the next one is another head of the item or the next item that has tiles)
-        if (++kvh == p.kv.kv_heads) {
-            kvh = 0;
-            do { ++item; it = QaItem(p, min(item, p.n_items - 1), R); } while (it.tiles == 0 && item < p.n_items);
-        }
-        off = 0;
-        begin_pair(it, kvh, off);
-        load_queries(it, kvh);
-    }
+    const bool whole_pair = off == 0 && tile1 - tile0 == it.tiles, began_here = off == 0;
+    const uint32_t first_place = pair_begin + plan.cost, last_place = first_place + it.tiles - 1;      // of the pair's tiles
+    const int head0 = kvh * p.group;
+    const bool more = advance();
+    if (more) begin_pair();
     auto write_out = [&](int r, int d, const float4& acc, float sum) {
         const float inv = 128.f / sum;                             // (values carry a 1 / 128, as keys do)
-        const int row = row0 + r, tok = q_start + row / p.group, head = head0 + row % p.group;
+        const int row = row0 + r, ahead = row < p.group ? 0 : row / p.group, tok = q_start + ahead, head = head0 + row - ahead * p.group;
         const __nv_bfloat162 a = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), b = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
         *reinterpret_cast<uint2*>(p.out + ((long long)tok * p.heads + head) * HD + d) =
             make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
@@ -621,16 +666,16 @@ attention_q4_kernel(const QaParams p) {
         }
     }
     if (!whole_pair) {
-        const int c0 = (int)(pair_begin / per), c1 = (int)((pair_begin + pair_tiles - 1) / per);
-        __threadfence();
-        __syncthreads();
+        const int c0 = (int)(first_place / per), c1 = (int)(last_place / per);
+        __syncthreads();                                           // (every thread's share is written; one fence covers them)
         if (threadIdx.x == 0) {
+            __threadfence();
             last = atomicAdd(p.arrived + c0, 1u) == (unsigned)(c1 - c0);
             if (last) p.arrived[c0] = 0;                           // ready for the next launch
+            __threadfence();
         }
         __syncthreads();
         if (last) {
-            __threadfence();
             constexpr int S = 8;                                   // pieces asked for together
             for (int e = threadIdx.x; e < rows * (HD / 4); e += QA_THREADS) {
                 const int r = e / (HD / 4), d = e % (HD / 4) * 4;
@@ -664,7 +709,7 @@ attention_q4_kernel(const QaParams p) {
             }
         }
     }
-    if (f >= f1) break;
+    if (!more) break;
     __syncthreads();                                               // the next pair's results overwrite what was merged here
     }
 }
@@ -673,7 +718,7 @@ template <int HD, int NT>
 static int launch_q4(const QaParams& p, cudaStream_t stream) {
     constexpr int smem = QaTile<HD>::smem(NT);
     static_assert(smem <= 226 * 1024, "the rings do not fit shared memory");
-    if (p.kv.page_size == 16) {
+    if (p.kv.page_size == 16 && p.kv.fault == nullptr) {
         if (int st = ensure_dynamic_smem<attention_q4_kernel<HD, NT, true>>(smem, "axon_attention_q4")) return st;
         launch_pdl(attention_q4_kernel<HD, NT, true>, dim3(p.ctas), dim3(QA_THREADS), smem, stream, p);
     } else {
