@@ -108,43 +108,123 @@ rope_kv_write_q4_kernel(const float* __restrict__ qkv, const float2* __restrict_
     }
 }
 
+// The same for the common layout (pairs (i, i + hd / 2) over the whole head, hd % 32 == 0, keys and values of one
+// width, 16-byte aligned operands): a thread owns four channels of each half of a row, so that nothing is read twice
+// and the groups of both halves are again four neighbouring lanes.  Bound by memory: 2,048 tokens at 28 + 4 + 4 heads of 128 move
+// 57 MB.
+template <typename T>
+__device__ __forceinline__ void q4_store4(T* dst, const float (&x)[4]);
+template <>
+__device__ __forceinline__ void q4_store4<float>(float* dst, const float (&x)[4]) {
+    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+}
+template <>
+__device__ __forceinline__ void q4_store4<__nv_bfloat16>(__nv_bfloat16* dst, const float (&x)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+constexpr int Q4_WRITE_THREADS = 192;
+template <typename T>
+__global__ void __launch_bounds__(Q4_WRITE_THREADS)
+rope_kv_write_q4_vec_kernel(const float* __restrict__ qkv, const float2* __restrict__ table, const int32_t* __restrict__ positions,
+                            const int32_t* __restrict__ token_slot, T* __restrict__ q_out, uint8_t* __restrict__ pool, PagedQ4 kv,
+                            int heads, int write_kv, SplitFold fold) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int t = blockIdx.x, half = kv.hd / 2, lanes = half / 4;                  // threads of a row
+    const int items = (heads + (write_kv ? 2 * kv.kv_heads : 0)) * lanes;
+    const float* row = qkv + (long long)t * ((heads + 2 * kv.kv_heads) * kv.hd);
+    const int pos = positions[t], lp = pos / kv.page_size, in_page = pos - lp * kv.page_size;
+    const long long page = write_kv ? kv.record_at(token_slot[t], lp, 0) : 0;
+    // (the items of a row are a multiple of four, so the lanes of a group are all here or all beyond the last item)
+    for (int it = blockIdx.y * Q4_WRITE_THREADS + threadIdx.x; it < items; it += gridDim.y * Q4_WRITE_THREADS) {
+        const int h = it / lanes, i0 = (it - h * lanes) * 4, col = h * kv.hd;
+        const float4 a4 = q4_load4(row, fold, t, col + i0), b4 = q4_load4(row, fold, t, col + half + i0);
+        float a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+        if (h < heads + kv.kv_heads) {
+            const float4 w01 = *reinterpret_cast<const float4*>(table + (long long)t * half + i0), w23 = *reinterpret_cast<const float4*>(table + (long long)t * half + i0 + 2);
+            const float c[4] = {w01.x, w01.z, w23.x, w23.z}, s[4] = {w01.y, w01.w, w23.y, w23.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = a[j], y = b[j];
+                a[j] = __fsub_rn(__fmul_rn(x, c[j]), __fmul_rn(y, s[j]));
+                b[j] = __fadd_rn(__fmul_rn(x, s[j]), __fmul_rn(y, c[j]));
+            }
+        }
+        if (h < heads) {
+            T* dst = q_out + (long long)t * (heads * kv.hd) + col + i0;
+            q4_store4<T>(dst, a);
+            q4_store4<T>(dst + half, b);
+            continue;
+        }
+        const bool is_v = h >= heads + kv.kv_heads;
+        uint8_t* rec = pool + page + (long long)(is_v ? h - heads - kv.kv_heads : h - heads) * kv.record;
+        uint8_t* codes = rec + (is_v ? kv.v_codes : 0) + (long long)in_page * (kv.hd / 2) + i0 / 2;
+        uint8_t* steps = rec + (is_v ? kv.v_steps : kv.k_steps) + (long long)in_page * (kv.hd / Q4_GROUP) + i0 / Q4_GROUP;
+        const unsigned group = 0xFu << (threadIdx.x & 28);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const float* x = part ? b : a;
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(group, top, 1));
+            top = max(top, __shfl_xor_sync(group, top, 2));
+            const int byte = q4_step_byte(top);
+            const float inv = q4_inverse(byte);
+            uint32_t two = 0x8888u;
+            if (byte != Q4_NAN) two = q4_code(x[0], inv) | q4_code(x[1], inv) << 4 | q4_code(x[2], inv) << 8 | q4_code(x[3], inv) << 12;
+            *reinterpret_cast<uint16_t*>(codes + part * (half / 2)) = (uint16_t)two;
+            if ((threadIdx.x & 3) == 0) steps[part * (half / Q4_GROUP)] = (uint8_t)byte;
+        }
+    }
+}
+
 // Positions back as rows of T.  A CTA owns up to 32 consecutive rows of the output: its first
-// threads find each row's span and page once, then all threads turn words of eight codes into
-// eight values, neighbouring threads along a row and then along positions, which is how both sides lie in
-// memory.  Output row r of plane p and kv head h starts at
+// threads find each row's span and page once, then every thread takes one word of eight codes of a row through all heads
+// and both planes, several loads at a time; neighbouring threads go along a row and then along positions,
+// which is how both sides lie in memory.  Output row r of plane p and kv head h starts at
 //   (r / block) * block_stride + (r % block) * row_stride + h * head_stride.
+// Bound by the bytes written, 3.6 times those read in bfloat16.
 struct Q4Out {
     void *k, *v;
     long long block_stride, row_stride, head_stride;
     int block;
 };
 template <typename T>
-__device__ __forceinline__ void q4_store8(T* dst, uint32_t word, float s);
+__device__ __forceinline__ void q4_store8(T* dst, uint32_t word, int byte);
 template <>
-__device__ __forceinline__ void q4_store8<float>(float* dst, uint32_t word, float s) {
+__device__ __forceinline__ void q4_store8<float>(float* dst, uint32_t word, int byte) {
+    const float s = q4_step(byte);
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = q4_digit(word, i) * s;
     reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
     reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
+// In bfloat16 a code in the last four bits of 128 + code, and one fused multiply-add that takes 136 s away: (c - 8) s
+// has seven significant bits and 136 s eight, so nothing is rounded.
 template <>
-__device__ __forceinline__ void q4_store8<__nv_bfloat16>(__nv_bfloat16* dst, uint32_t word, float s) {
-    uint32_t o[4];
+__device__ __forceinline__ void q4_store8<__nv_bfloat16>(__nv_bfloat16* dst, uint32_t word, int byte) {
+    const __nv_bfloat162 s = __float2bfloat162_rn(q4_step(byte)), less = __hmul2(s, __float2bfloat162_rn(-136.f));
+    uint32_t v[4];                                             // codes (i, i + 4)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        __nv_bfloat162 b = __floats2bfloat162_rn(q4_digit(word, 2 * i) * s, q4_digit(word, 2 * i + 1) * s);
-        o[i] = *reinterpret_cast<uint32_t*>(&b);
+        const uint32_t c = ((word >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+        const __nv_bfloat162 x = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&c), s, less);
+        v[i] = *reinterpret_cast<const uint32_t*>(&x);
     }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                                                __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632));
 }
 
-constexpr int Q4_READ_ROWS = 32, Q4_READ_THREADS = 256;
+constexpr int Q4_READ_ROWS = 32, Q4_READ_THREADS = 256, Q4_READ_BATCH = 4;      // (threads: for one plane, or half for each of two)
+// `pad`: the rows from a span's end up to the next multiple of `pad` of its rows hold zeros.
 template <typename T>
 __global__ void __launch_bounds__(Q4_READ_THREADS)
 kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* __restrict__ spans, int n_spans, int n_slots,
-                  long long n_rows, int rows_per_cta, Q4Out out) {
-    __shared__ long long rec[Q4_READ_ROWS];                    // the row's record of kv head 0, or -1: not written
+                  long long n_rows, int rows_per_cta, int pad, Q4Out out) {
+    __shared__ long long rec[Q4_READ_ROWS];                    // the row's record of kv head 0; -1: not written, -2: zeros
     __shared__ int at[Q4_READ_ROWS];                           // its place in the page
     pdl_launch_dependents();
     pdl_wait();
@@ -154,11 +234,12 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* _
         long long where = -1;
         int in_page = 0;
         for (int s = 0; s < n_spans && r < n_rows; ++s) {
-            const long long i = r - spans[3 * n_spans + s];
-            if (i < 0 || i >= spans[2 * n_spans + s]) continue;
+            const long long i = r - spans[3 * n_spans + s], count = spans[2 * n_spans + s];
+            if (i < 0 || i >= (count + pad - 1) / pad * pad) continue;
             const int slot = spans[s];
             const long long pos = spans[n_spans + s] + i, lp = pos / kv.page_size;
-            if (slot >= 0 && slot < n_slots && pos >= 0 && lp < kv.table_stride) {
+            if (i >= count) where = -2;
+            else if (slot >= 0 && slot < n_slots && pos >= 0 && lp < kv.table_stride) {
                 where = kv.record_at(slot, (int)lp, 0);
                 in_page = (int)(pos - lp * kv.page_size);
             }
@@ -168,19 +249,36 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* _
         at[threadIdx.x] = in_page;
     }
     __syncthreads();
-    const int kw = kv.hd / 8, vw = kv.vd / 8;                  // words of a row
-    const int k_items = out.k ? kv.kv_heads * rows_per_cta * kw : 0, v_items = out.v ? kv.kv_heads * rows_per_cta * vw : 0;
-    for (int i = threadIdx.x; i < k_items + v_items; i += Q4_READ_THREADS) {
-        const bool is_v = i >= k_items;
-        const int words = is_v ? vw : kw, j = is_v ? i - k_items : i;
-        const int w = j % words, r = j / words % rows_per_cta, h = j / words / rows_per_cta;
-        if (rec[r] < 0) continue;
-        const uint8_t* from = pool + rec[r] + (long long)h * kv.record;
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(from + (is_v ? kv.v_codes : 0) + ((long long)at[r] * words + w) * 4);
-        const float s = q4_step(from[(is_v ? kv.v_steps : kv.k_steps) + (long long)at[r] * (words / 2) + w / 2]);
-        const long long row = r0 + r;
-        T* dst = (T*)(is_v ? out.v : out.k) + row / out.block * out.block_stride + row % out.block * out.row_stride + h * out.head_stride + w * 8;
-        q4_store8<T>(dst, word, s);
+    // with both planes to write the first half of the threads takes keys, the second values
+    const bool both = out.k != nullptr && out.v != nullptr, is_v = both ? threadIdx.x >= Q4_READ_THREADS / 2 : out.v != nullptr;
+    const int threads = both ? Q4_READ_THREADS / 2 : Q4_READ_THREADS, tid = both ? threadIdx.x % (Q4_READ_THREADS / 2) : threadIdx.x;
+    T* const base = (T*)(is_v ? out.v : out.k);
+    const int words = (is_v ? kv.vd : kv.hd) / 8, codes = is_v ? kv.v_codes : 0, steps = is_v ? kv.v_steps : kv.k_steps;
+    const int r_step = max(threads / words, 1);
+    for (int i = tid; i < (threads / words > 0 ? r_step * words : words); i += threads) {      // (a row of more words than threads: several of them)
+        const int w = i % words;
+        for (int r = i / words; r < rows_per_cta; r += r_step) {
+            if (rec[r] == -1) continue;
+            const bool held = rec[r] >= 0;
+            const uint8_t* from = pool + (held ? rec[r] : 0);
+            const uint8_t* const word_at = from + codes + ((long long)at[r] * words + w) * 4;
+            const uint8_t* const step_at = from + steps + (long long)at[r] * (words / 2) + w / 2;
+            const long long row = r0 + r;
+            T* dst = base + row / out.block * out.block_stride + row % out.block * out.row_stride + w * 8;
+            for (int h0 = 0; h0 < kv.kv_heads; h0 += Q4_READ_BATCH) {
+                uint32_t word[Q4_READ_BATCH];
+                int byte[Q4_READ_BATCH];
+#pragma unroll
+                for (int k = 0; k < Q4_READ_BATCH; ++k) {
+                    const bool there = held && h0 + k < kv.kv_heads;
+                    word[k] = there ? *reinterpret_cast<const uint32_t*>(word_at + (long long)(h0 + k) * kv.record) : 0x88888888u;
+                    byte[k] = there ? step_at[(long long)(h0 + k) * kv.record] : 0;
+                }
+#pragma unroll
+                for (int k = 0; k < Q4_READ_BATCH; ++k)
+                    if (h0 + k < kv.kv_heads) q4_store8<T>(dst + (h0 + k) * out.head_stride, word[k], byte[k]);
+            }
+        }
     }
 }
 
@@ -384,6 +482,17 @@ AXON_API int axon_rope_kv_write_q4(const float* qkv, const float* table, const i
     if (rot % 2 || rot > kv.hd || rot < 0) { set_error("axon_rope_kv_write_q4: rotated size %d must be even and at most the head size %d", rot, kv.hd); return AXON_BAD_ARGUMENT; }
     if (dtype != AXON_Q4_F32 && dtype != AXON_Q4_BF16) { set_error("axon_rope_kv_write_q4: unknown dtype %d", dtype); return AXON_BAD_ARGUMENT; }
     const SplitFold fold{partial, partial ? bias : nullptr, splits, ntok};
+    if (table != nullptr && !adjacent && rot == kv.hd && kv.hd % 32 == 0 && kv.planes == 2 && kv.vd == kv.hd &&
+        (((uintptr_t)qkv | (uintptr_t)table | (uintptr_t)partial | (uintptr_t)bias | (uintptr_t)q_out) & 15) == 0) {
+        const int items = (heads + (write_kv ? 2 * kv.kv_heads : 0)) * (kv.hd / 8);
+        // few tokens: a CTA per 192 of a token's items; many: a CTA per token
+        const dim3 vgrid(n, n >= 4 * 148 ? 1 : (items + Q4_WRITE_THREADS - 1) / Q4_WRITE_THREADS);
+        if (dtype == AXON_Q4_F32)
+            launch_pdl(rope_kv_write_q4_vec_kernel<float>, vgrid, dim3(Q4_WRITE_THREADS), 0, stream, qkv, (const float2*)table, positions, token_slot, (float*)q_out, (uint8_t*)pool, kv, heads, write_kv, fold);
+        else
+            launch_pdl(rope_kv_write_q4_vec_kernel<__nv_bfloat16>, vgrid, dim3(Q4_WRITE_THREADS), 0, stream, qkv, (const float2*)table, positions, token_slot, (__nv_bfloat16*)q_out, (uint8_t*)pool, kv, heads, write_kv, fold);
+        return launch_status("axon_rope_kv_write_q4");
+    }
     const int rows = heads + kv.planes * kv.kv_heads;
     const dim3 grid(n, (rows + 7) / 8);
     const bool vec = rot % 8 == 0 && (((uintptr_t)qkv | (uintptr_t)table | (uintptr_t)partial | (uintptr_t)bias) & 15) == 0;
@@ -392,6 +501,20 @@ AXON_API int axon_rope_kv_write_q4(const float* qkv, const float* table, const i
     else { if (vec) AXON_Q4_WRITE(__nv_bfloat16, true); else AXON_Q4_WRITE(__nv_bfloat16, false); }
 #undef AXON_Q4_WRITE
     return launch_status("axon_rope_kv_write_q4");
+}
+
+static int kv_read_launch(const void* pool, const PagedQ4& kv, const int32_t* spans, int n_spans, int n_slots, int dtype, long long n_rows,
+                          int pad, const Q4Out& out, cudaStream_t stream) {
+    int rows = Q4_READ_ROWS;
+    while (rows > 1 && (n_rows + rows - 1) / rows < 2 * 148) rows /= 2;      // few rows: more CTAs rather than longer ones
+    const long long ctas = (n_rows + rows - 1) / rows;
+    if (ctas > 0x7fffffffLL) { set_error("axon_kv_read_q4: %lld rows are too many", n_rows); return AXON_BAD_ARGUMENT; }
+    if (dtype == AXON_Q4_F32)
+        launch_pdl(kv_read_q4_kernel<float>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, pad, out);
+    else if (dtype == AXON_Q4_BF16)
+        launch_pdl(kv_read_q4_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, pad, out);
+    else { set_error("axon_kv_read_q4: unknown dtype %d", dtype); return AXON_BAD_ARGUMENT; }
+    return launch_status("axon_kv_read_q4");
 }
 
 // Output rows 0 .. n_rows - 1 ([kv_heads][width] each) from the spans [4][n_spans]: slot, first
@@ -403,23 +526,61 @@ AXON_API int axon_kv_read_q4(const void* pool, const AxonKvLayout* layout, const
     PagedQ4 kv;
     if (int st = to_q4(layout, pool, "axon_kv_read_q4", &kv)) return st;
     if (((uintptr_t)keys | (uintptr_t)values) & 15) { set_error("axon_kv_read_q4: outputs must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
-    if (dtype != AXON_Q4_F32 && dtype != AXON_Q4_BF16) { set_error("axon_kv_read_q4: unknown dtype %d", dtype); return AXON_BAD_ARGUMENT; }
-    if (values != nullptr && keys != nullptr && kv.vd != kv.hd) {
-        // the two planes have strides of their own: one launch each
-        if (int st = axon_kv_read_q4(pool, layout, spans, n_spans, n_slots, keys, nullptr, dtype, n_rows, stream)) return st;
-        return axon_kv_read_q4(pool, layout, spans, n_spans, n_slots, nullptr, values, dtype, n_rows, stream);
+    // planes of different widths have strides of their own: one launch each
+    const bool apart = keys != nullptr && values != nullptr && kv.vd != kv.hd;
+    for (int part = 0; part < (apart ? 2 : 1); ++part) {
+        void* const k = apart && part ? nullptr : keys;
+        void* const v = apart && !part ? nullptr : values;
+        const long long width = k != nullptr ? kv.hd : kv.vd;
+        const Q4Out out{k, v, kv.kv_heads * width, 0, width, 1};
+        if (int st = kv_read_launch(pool, kv, spans, n_spans, n_slots, dtype, n_rows, 1, out, stream)) return st;
     }
-    const long long width = values != nullptr ? kv.vd : kv.hd;
-    const Q4Out out{keys, values, kv.kv_heads * width, 0, width, 1};
-    int rows = Q4_READ_ROWS;
-    while (rows > 1 && (n_rows + rows - 1) / rows < 2 * 148) rows /= 2;      // few rows: more CTAs rather than longer ones
-    const long long ctas = (n_rows + rows - 1) / rows;
-    if (ctas > 0x7fffffffLL) { set_error("axon_kv_read_q4: %lld rows are too many", n_rows); return AXON_BAD_ARGUMENT; }
-    if (dtype == AXON_Q4_F32)
-        launch_pdl(kv_read_q4_kernel<float>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, out);
-    else
-        launch_pdl(kv_read_q4_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, out);
-    return launch_status("axon_kv_read_q4");
+    return AXON_OK;
+}
+
+// Tables for a prompt's attention over read-back keys.  For each of the n_long segments named in `which`: a span (see
+// axon_kv_read_q4) of the positions that its rows see, from a multiple of 64 on; its place in a pool of pages of 64
+// positions, one after another; and its segment as the attention kernels take it, counted from the span's first
+// position, with row i of `table` [n_long][stride] as its block table.  What `pages` or `stride` do not hold is left out (the
+// host sizes both from the same lengths).
+__global__ void q4_prompt_plan_kernel(const int32_t* __restrict__ segments, int n_segments, const int32_t* __restrict__ which, int n_long,
+                                      int window, int pages, int stride, int32_t* __restrict__ spans, int32_t* __restrict__ seg_out,
+                                      int32_t* __restrict__ table) {
+    pdl_launch_dependents();
+    pdl_wait();
+    int base = 0;
+    for (int i = 0; i < n_long; ++i) {
+        const int s = which[i], q_len = segments[2 * n_segments + s], kv_len = segments[3 * n_segments + s];
+        const int lo = window > 0 ? max(kv_len - q_len - window + 1, 0) / 64 * 64 : 0;
+        const int n = min(min((kv_len - lo + 63) / 64, stride), pages - base);
+        if (threadIdx.x == 0) {
+            spans[i] = segments[s]; spans[n_long + i] = lo; spans[2 * n_long + i] = min(kv_len - lo, n * 64); spans[3 * n_long + i] = base * 64;
+            seg_out[i] = i; seg_out[n_long + i] = segments[n_segments + s]; seg_out[2 * n_long + i] = q_len; seg_out[3 * n_long + i] = min(kv_len - lo, n * 64);
+        }
+        for (int j = threadIdx.x; j < stride; j += blockDim.x) table[(long long)i * stride + j] = min(base + j, pages - 1);
+        base += n;
+    }
+}
+AXON_API int axon_q4_prompt_plan(const int32_t* segments, int n_segments, const int32_t* which, int n_long, int window, int pages, int stride,
+                                 int32_t* spans, int32_t* seg_out, int32_t* table, cudaStream_t stream) {
+    if (n_long <= 0) return AXON_OK;
+    if (pages < 1 || stride < 1) { set_error("axon_q4_prompt_plan: no room (%d pages, %d per request)", pages, stride); return AXON_BAD_ARGUMENT; }
+    launch_pdl(q4_prompt_plan_kernel, dim3(1), dim3(256), 0, stream, segments, n_segments, which, n_long, window, pages, stride, spans, seg_out, table);
+    return launch_status("axon_q4_prompt_plan");
+}
+
+// The positions of the plan's spans into its pool of pages [pages][2][kv_heads][64][head_dim]; rows behind a span's end in
+// its last page are zeros.
+AXON_API int axon_kv_read_q4_pages(const void* pool, const AxonKvLayout* layout, const int32_t* spans, int n_spans, int n_slots,
+                                   void* pages_out, int dtype, int pages, cudaStream_t stream) {
+    if (pages <= 0 || n_spans <= 0) return AXON_OK;
+    PagedQ4 kv;
+    if (int st = to_q4(layout, pool, "axon_kv_read_q4_pages", &kv)) return st;
+    if (kv.planes != 2 || kv.vd != kv.hd) { set_error("axon_kv_read_q4_pages: takes caches with key and value planes of one width"); return AXON_BAD_ARGUMENT; }
+    if ((uintptr_t)pages_out & 15) { set_error("axon_kv_read_q4_pages: outputs must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
+    const long long plane = (long long)kv.kv_heads * 64 * kv.hd;
+    const Q4Out out{pages_out, (uint8_t*)pages_out + plane * (dtype == AXON_Q4_F32 ? 4 : 2), 2 * plane, kv.hd, 64ll * kv.hd, 64};
+    return kv_read_launch(pool, kv, spans, n_spans, n_slots, dtype, 64ll * pages, 64, out, stream);
 }
 
 // Floats of scratch that axon_attention_q4_plain needs for its key shares (0 for one share).

@@ -60,6 +60,14 @@ def step_workspace_bytes(hidden_size: int, vocab_size: int, max_step_tokens: int
     return max_step_tokens * hidden_size * 64 + 4 * vocab_size * max(max_slots, 1)
 
 
+def quantised_workspace_bytes(needs, max_slots: int, max_positions: int) -> int:
+    """What prompts over a quantised cache take beside it: the bfloat16 pages that their keys and values are read back into."""
+    from ..kernels.fast import Q4_PROMPT_POSITIONS
+    widest = max((n.elements_per_token for entry in needs for n in entry.values() if getattr(n, "bits", 0)), default=0)
+    positions = min(max_slots * max_positions, max(max_positions, Q4_PROMPT_POSITIONS))
+    return 2 * widest * positions * 9 // 8
+
+
 def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] = None,
                  seed: Optional[int] = None, dtype: Union[str, torch.dtype] = "bfloat16",
                  device: Union[str, torch.device] = "cuda:0", page_size: int = 16,
@@ -102,7 +110,8 @@ def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] 
             free, _ = torch.cuda.mem_get_info(dev)
             max_tokens = plan_pool_tokens(free, bytes_per_token(model.needs, dt, page_size), page_size, max_slots, max_positions,
                                           step_workspace_bytes(spec.hidden_size, spec.vocab_size,
-                                                               min(max_step_tokens, max_slots * max_positions), max_slots))
+                                                               min(max_step_tokens, max_slots * max_positions), max_slots)
+                                          + quantised_workspace_bytes(model.needs, max_slots, max_positions))
             if max_tokens < page_size:
                 raise RuntimeError(f"{free >> 20} MiB are free on {dev} once the weights are placed: no room for a cache pool")
         if check_tables is None:

@@ -376,20 +376,86 @@ def _q4_row_tiles(rows: int, hd: int) -> int:
     return next((n for n in (1, 2, 4) if 8 * n >= rows or n == Q4_ROW_TILES[hd]))
 
 
-def _q4_items(ctx, group: int, hd: int):
-    """The step's work for the 4-bit attention, cached per step: tiles of query rows (token * group + head) of each segment."""
-    key = ("q4_items", group, hd)
+#: segments with more query rows (tokens x heads of a group) than this attend over keys and values read back into
+#: bfloat16 pages; the 4-bit kernel, which widens the keys anew for every 32 rows, takes the others
+Q4_SHORT_ROWS = 256
+#: positions that are read back at a time (of several requests; one request is never cut)
+Q4_PROMPT_POSITIONS = 1 << 18
+
+
+def _q4_is_long(n: int, group: int, hd: int) -> bool:
+    return hd in FA_HEAD_DIMS and n * group > Q4_SHORT_ROWS
+
+
+def _q4_any_long(ctx, group: int, hd: int) -> bool:
+    return _q4_is_long(ctx.max_q_len, group, hd)
+
+
+def _q4_bucket(n: int) -> int:
+    """``n`` rounded up to a multiple of an eighth of the power of two below it: sizes that graphs may share."""
+    step = 1 << max(0, n.bit_length() - 4)
+    return -(-n // step) * step
+
+
+def _q4_prompt_sizes(ctx, segs, window: int):
+    """(pages of 64 positions that these segments' keys take, those of the longest), rounded up."""
+    n = []
+    for s in segs:
+        q, kv = ctx.seg_q_len[s], ctx.seg_kv_len[s]
+        lo = max(kv - q - window + 1, 0) // 64 * 64 if window else 0
+        n.append(-(-(kv - lo) // 64))
+    return _q4_bucket(sum(n)), _q4_bucket(max(n))
+
+
+def _q4_work(ctx, group: int, hd: int, window: int, takes_short: bool):
+    """The step's work for the 4-bit attention, cached per step: tiles of query rows (token * group + head) of short
+    segments ``(row tiles, items, list or None)`` or None, and groups of long ones (of all, without ``takes_short``)."""
+    key = ("q4_work", group, hd, window, takes_short)
     got = ctx.scratch.get(key)
-    if got is None:
-        nt = _q4_row_tiles(max(ctx.seg_q_len) * group, hd)
-        if max(ctx.seg_q_len) * group <= 8 * nt:
-            got = (nt, len(ctx.seg_q_len), None)
+    if got is not None:
+        return got
+    n_seg = len(ctx.seg_q_len)
+    short = [s for s in range(n_seg) if not _q4_is_long(ctx.seg_q_len[s], group, hd)] if takes_short else []
+    items = None
+    if short:
+        most = max(ctx.seg_q_len[s] for s in short) * group
+        nt = _q4_row_tiles(most, hd)
+        if len(short) == n_seg and most <= 8 * nt:
+            items = (nt, n_seg, None)                    # item i is segment i
         else:
-            work = [(kv_len - n + min(n, -(-(r + 8 * nt) // group)), s, r)
-                    for s, (n, kv_len) in enumerate(zip(ctx.seg_q_len, ctx.seg_kv_len)) for r in range(0, n * group, 8 * nt)]
+            work = []
+            for s in short:
+                n, kv_len = ctx.seg_q_len[s], ctx.seg_kv_len[s]
+                work += [(kv_len - n + min(n, -(-(r + 8 * nt) // group)), s, r) for r in range(0, n * group, 8 * nt)]
             flat = [x for _, s, r in sorted(work, reverse=True) for x in (s, r)]     # the longest must not start last
-            got = (nt, len(work), ctx.rt.upload_i32(f"q4_items_{group}_{hd}", flat))
-        ctx.scratch[key] = got
+            items = (nt, len(work), ctx.rt.upload_i32(f"q4_items_{group}_{hd}", flat))
+    groups, at, room = [], [], 0
+    for s in range(n_seg):
+        if s in short:
+            continue
+        if at and room + ctx.seg_kv_len[s] > Q4_PROMPT_POSITIONS:
+            groups.append(at)
+            at, room = [], 0
+        at.append(s)
+        room += ctx.seg_kv_len[s]
+    if at:
+        groups.append(at)
+    plans = []
+    for k, segs in enumerate(groups):
+        pages, stride = _q4_prompt_sizes(ctx, segs, window)
+        rows = 256 if hd == 128 and ENABLED["attention_tc"] else 64
+        tpt = rows // group
+        work = [(ctx.seg_kv_len[s] - ctx.seg_q_len[s] + min(t0 + tpt, ctx.seg_q_len[s]), i, t0)
+                for i, s in enumerate(segs) for t0 in range(0, ctx.seg_q_len[s], tpt)]
+        flat = list(segs) + [x for _, i, t0 in sorted(work, reverse=True) for x in (i, t0)]
+        lists = ctx.rt.upload_i32(f"q4_prompt_{group}_{rows}", flat)
+        n = len(segs)
+        ints = ctx.rt.buffer(f"q4_plan_{window}_{k}", (8 * n + n * stride,), torch.int32)
+        check(lib.cuda().axon_q4_prompt_plan(ctx.segments.data_ptr(), n_seg, lists.data_ptr(), n, window, pages, stride, ints.data_ptr(),
+                                             ints[4 * n:].data_ptr(), ints[8 * n:].data_ptr(), _stream()))
+        plans.append((n, pages, rows, tpt, lists[n:], len(work), ints[:4 * n], ints[4 * n:8 * n], ints[8 * n:].view(n, stride)))
+    got = (items, plans)
+    ctx.scratch[key] = got
     return got
 
 
@@ -398,29 +464,57 @@ def _q4_takes(hd: int, page_size: int) -> bool:
 
 
 def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
-    """Tensor-core attention over a 4-bit cache; refuses head sizes other than 64, 128 and 256, dtypes
-    other than bfloat16, and pages whose 16-byte pieces of steps would straddle them (a multiple of 4 positions
-    is needed at head size 64, of 2 at 128)."""
-    if not ENABLED["attention_q4"] or ctx.segments is None or not _q4_takes(kv.head_dim, kv.page_size):
+    """Tensor-core attention over a 4-bit cache.  Segments of few query rows read the pages as they are; long ones have
+    the positions that they see read back once per layer, into pages that the bfloat16 attention takes.  Refuses dtypes
+    other than bfloat16, planes of two widths, groups of more than 64 heads, and head sizes and pages that
+    neither way takes (short: head sizes 64, 128 and 256, a multiple of 4 positions a page at 64, of 2 at 128; long:
+    head sizes 16, 32, 64 and 128).  Where only the long way takes a step that has long segments, all of it goes there."""
+    if not ENABLED["attention_q4"] or ctx.segments is None or kv.planes != 2 or kv.v_dim != kv.head_dim:
         return False
-    if kv.planes != 2 or kv.v_dim != kv.head_dim or heads % kv.kv_heads:
+    hd, group = kv.head_dim, heads // kv.kv_heads
+    if heads % kv.kv_heads or group > 64 or q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         return False
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16 or not q.is_contiguous() or not out.is_contiguous():
+    if not q.is_contiguous() or not out.is_contiguous():
         return False
-    nt, n_items, items = _q4_items(ctx, heads // kv.kv_heads, kv.head_dim)
+    takes_short = _q4_takes(hd, kv.page_size)
+    if not takes_short and not _q4_any_long(ctx, group, hd):
+        return False
+    items, plans = _q4_work(ctx, group, hd, kv.window, takes_short)
     cu = lib.cuda()
-    ctas = cu.axon_attention_q4_ctas(kv.head_dim, nt)
-    floats = 2 * ctas * 8 * nt * (kv.head_dim + 2) + ctas
-    scratch = ctx.rt.zeroed_buffer(f"q4_scratch_{kv.head_dim}_{nt}", (floats,), torch.float32)
-    check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
-                               None if items is None else items.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
-                               nt, scratch.data_ptr(), floats, _stream()))
+    if items is not None:
+        nt, n_items, which = items
+        ctas = cu.axon_attention_q4_ctas(hd, nt)
+        floats = 2 * ctas * 8 * nt * (hd + 2) + ctas
+        scratch = ctx.rt.zeroed_buffer(f"q4_scratch_{hd}_{nt}", (floats,), torch.float32)
+        check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
+                                   None if which is None else which.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
+                                   nt, scratch.data_ptr(), floats, _stream()))
+    for n, pages, rows, tpt, tiles, n_tiles, spans, segments, table in plans:
+        pool = ctx.rt.buffer("q4_prompt_pages", (pages, 1, 2, kv.kv_heads, 64, hd), torch.bfloat16)
+        layout = lib.KvLayout(block_table=table.data_ptr(), table_stride=table.shape[1], page_size=64, kv_heads=kv.kv_heads, head_dim=hd,
+                              page_stride=2 * kv.kv_heads * 64 * hd, entry_offset=0, v_offset=kv.kv_heads * 64 * hd, v_dim=hd, planes=2,
+                              n_pages=pages - 1, bits=0, fault=None)
+        check(cu.axon_kv_read_q4_pages(kv.pool.data_ptr(), kv._ref, spans.data_ptr(), n, kv.block_table.shape[0], pool.data_ptr(), 1,
+                                       pages, _stream()))
+        if rows == 256:
+            check(cu.axon_attention_tc(q.data_ptr(), pool.data_ptr(), out.data_ptr(), segments.data_ptr(), n, tiles.data_ptr(), n_tiles,
+                                       ctypes.byref(layout), heads, float(scale), int(kv.window), tpt, _stream()))
+        else:
+            check(cu.axon_attention_fa(q.data_ptr(), pool.data_ptr(), out.data_ptr(), segments.data_ptr(), n, tiles.data_ptr(), n_tiles,
+                                       ctypes.byref(layout), heads, float(scale), int(kv.window), 0, tpt, 1, None, None, _stream()))
     return True
 
 
 def q4_graph_key(ctx, heads: int, kv_heads: int, head_dim: int, window: int, precise: bool):
-    """What the 4-bit attention's launches take from the host beside the batch shape: nothing of the
-    tensor-core kernel's (it divides its work on the device), the share count of the plain one's."""
-    if not precise and ENABLED["attention_q4"] and _q4_takes(head_dim, ctx.rt.kv_page_size):
-        return ()
-    return (("q4_plain", q4_plain_splits(ctx, heads, kv_heads, window)),)
+    """What the 4-bit attention's launches take from the host beside the batch shape: nothing of the tensor-core kernel's
+    for few rows (it divides its work on the device), the room for what prompts read back, the share
+    count of the plain kernel."""
+    group = heads // kv_heads
+    key = []
+    takes = not precise and ENABLED["attention_q4"] and group <= 64
+    if takes and _q4_any_long(ctx, group, head_dim):
+        # (a portion of one request: steps of several are never captured)
+        key.append(("q4_prompt",) + _q4_prompt_sizes(ctx, range(len(ctx.seg_q_len)), window))
+    elif not (takes and _q4_takes(head_dim, ctx.rt.kv_page_size)):
+        key.append(("q4_plain", q4_plain_splits(ctx, heads, kv_heads, window)))
+    return tuple(key)

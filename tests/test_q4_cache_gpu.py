@@ -321,6 +321,25 @@ def test_long_contexts_in_shares(ops, heads, kv_heads, hd, ps, lens, window):
     check_attention(ops, cache, [1] * len(lens), heads, torch.float32, window)
 
 
+@pytest.mark.parametrize("heads,kv_heads,hd,ps", [(28, 4, 128, 16), (6, 2, 64, 32), (3, 1, 32, 16), (4, 2, 16, 5), (64, 1, 128, 16), (7, 1, 128, 7),
+                                                  (4, 1, 256, 16), (65, 1, 64, 16)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_prompts(ops, heads, kv_heads, hd, ps, window):
+    """Prompts whole and at the end of longer requests, beside short portions and single tokens."""
+    cache = Cache(ops, [300, 700, 41, 1, 650, 129], kv_heads, hd, ps, window=window, seed=21, loud=0.5)
+    check_attention(ops, cache, [300, 259, 3, 1, 100, 0], heads, torch.bfloat16, window, weight_half=2.0 ** -8)
+    check_attention(ops, cache, [0, 0, 0, 0, 0, 129], heads, torch.bfloat16, window, weight_half=2.0 ** -8)
+    check_attention(ops, cache, [0, 700, 0, 0, 650, 0], heads, torch.bfloat16, window, weight_half=2.0 ** -8)
+
+
+def test_prompts_read_back_in_groups(ops, monkeypatch):
+    """More positions than are read back at a time: groups of requests one after another."""
+    from axon_b200.kernels import fast
+    monkeypatch.setattr(fast, "Q4_PROMPT_POSITIONS", 700)
+    cache = Cache(ops, [300, 300, 900, 150, 333], 2, 128, 16, seed=22)
+    check_attention(ops, cache, [300, 200, 150, 150, 1], 6, torch.bfloat16, weight_half=2.0 ** -8)
+
+
 def test_what_is_not_finite_stays_with_who_sees_it(ops):
     """A NaN key or value is NaN for the tokens that see it and for no others, in every head's own channels."""
     for hd, heads, kv_heads in ((128, 6, 2), (64, 4, 4)):
