@@ -99,8 +99,7 @@ rope_kv_write_q4_kernel(const float* __restrict__ qkv, const float2* __restrict_
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int byte = q4_step_byte(top);
         const float inv = q4_inverse(byte);
-        uint32_t two = 0x8888u;
-        if (byte != Q4_NAN) two = q4_code(x[0], inv) | q4_code(x[1], inv) << 4 | q4_code(x[2], inv) << 8 | q4_code(x[3], inv) << 12;
+        const uint32_t two = q4_codes4(x[0], x[1], x[2], x[3], byte, inv);
         if (mine) {
             *reinterpret_cast<uint16_t*>(codes + c0 / 2) = (uint16_t)two;
             if ((lane & 3) == 0) steps[c0 / Q4_GROUP] = (uint8_t)byte;
@@ -164,7 +163,7 @@ rope_kv_write_q4_vec_kernel(const float* __restrict__ qkv, const float2* __restr
         const unsigned group = 0xFu << (threadIdx.x & 28);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-            const float* x = part ? b : a;
+            const float x[4] = {part ? b[0] : a[0], part ? b[1] : a[1], part ? b[2] : a[2], part ? b[3] : a[3]};
             uint32_t top = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
@@ -172,8 +171,7 @@ rope_kv_write_q4_vec_kernel(const float* __restrict__ qkv, const float2* __restr
             top = max(top, __shfl_xor_sync(group, top, 2));
             const int byte = q4_step_byte(top);
             const float inv = q4_inverse(byte);
-            uint32_t two = 0x8888u;
-            if (byte != Q4_NAN) two = q4_code(x[0], inv) | q4_code(x[1], inv) << 4 | q4_code(x[2], inv) << 8 | q4_code(x[3], inv) << 12;
+            const uint32_t two = q4_codes4(x[0], x[1], x[2], x[3], byte, inv);
             *reinterpret_cast<uint16_t*>(codes + part * (half / 2)) = (uint16_t)two;
             if ((threadIdx.x & 3) == 0) steps[part * (half / Q4_GROUP)] = (uint8_t)byte;
         }

@@ -73,11 +73,13 @@ __device__ __forceinline__ int q4_step_byte(uint32_t top) {
     return min(b, Q4_TOP);
 }
 __device__ __forceinline__ float q4_step(int byte) { return __half2float(__ushort_as_half((unsigned short)(byte << 7))); }
-// The nibble of x in a group with this step: `inv` is 1 / step (0 for a step of 0 or NaN).
-__device__ __forceinline__ uint32_t q4_code(float x, float inv) {
-    return (uint32_t)((int)fminf(fmaxf(rintf(__fmul_rn(x, inv)), -7.f), 7.f) + 8);
+__device__ __forceinline__ float q4_inverse(int byte) { return byte == 0 || byte == Q4_NAN ? 0.f : __frcp_rn(q4_step(byte)); }
+// The nibbles of four values of a group with this step byte; `inv` is 1 / step rounded to 32 bits (0 for a step of 0 or NaN).
+// Adding 1.5 * 2^23 + 8 rounds to whole numbers as rint does and leaves code + 8 in the last four bits.
+__device__ __forceinline__ uint32_t q4_codes4(float x0, float x1, float x2, float x3, int byte, float inv) {
+    auto code = [&](float x) { return __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x, inv), -7.f), 7.f), 12582920.0f)) & 15u; };
+    return byte == Q4_NAN ? 0x8888u : code(x0) | code(x1) << 4 | code(x2) << 8 | code(x3) << 12;
 }
-__device__ __forceinline__ float q4_inverse(int byte) { return byte == 0 || byte == Q4_NAN ? 0.f : __fdiv_rn(1.0f, q4_step(byte)); }
 // nibble i of a word of eight codes, as a float without its step
 __device__ __forceinline__ float q4_digit(uint32_t word, int i) {
     return __uint_as_float(0x4B000000u | ((word >> (4 * i)) & 15u)) - 8388616.0f;      // 2^23 + code, exactly

@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from . import lib
+from . import lib, ops
 from .lib import check
 
 EPI_STORE_F32, EPI_STORE_BF16, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2, 3
@@ -409,7 +409,7 @@ def _q4_prompt_sizes(ctx, segs, window: int):
 
 def _q4_work(ctx, group: int, hd: int, window: int, takes_short: bool):
     """The step's work for the 4-bit attention, cached per step: tiles of query rows (token * group + head) of short
-    segments ``(row tiles, items, list or None)`` or None, and groups of long ones (of all, without ``takes_short``)."""
+    segments ``(row tiles, items, list or None, scratch, its floats)`` or None, and groups of long ones (of all, without ``takes_short``)."""
     key = ("q4_work", group, hd, window, takes_short)
     got = ctx.scratch.get(key)
     if got is not None:
@@ -421,7 +421,7 @@ def _q4_work(ctx, group: int, hd: int, window: int, takes_short: bool):
         most = max(ctx.seg_q_len[s] for s in short) * group
         nt = _q4_row_tiles(most, hd)
         if len(short) == n_seg and most <= 8 * nt:
-            items = (nt, n_seg, None)                    # item i is segment i
+            items = (nt, n_seg, None)                    # (item i is segment i)
         else:
             work = []
             for s in short:
@@ -429,6 +429,9 @@ def _q4_work(ctx, group: int, hd: int, window: int, takes_short: bool):
                 work += [(kv_len - n + min(n, -(-(r + 8 * nt) // group)), s, r) for r in range(0, n * group, 8 * nt)]
             flat = [x for _, s, r in sorted(work, reverse=True) for x in (s, r)]     # the longest must not start last
             items = (nt, len(work), ctx.rt.upload_i32(f"q4_items_{group}_{hd}", flat))
+        ctas = lib.cuda().axon_attention_q4_ctas(hd, nt)
+        floats = 2 * ctas * 8 * nt * (hd + 2) + ctas
+        items += (ctx.rt.zeroed_buffer(f"q4_scratch_{hd}_{nt}", (floats,), torch.float32).data_ptr(), floats)
     groups, at, room = [], [], 0
     for s in range(n_seg):
         if s in short:
@@ -472,9 +475,12 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
     if not ENABLED["attention_q4"] or ctx.segments is None or kv.planes != 2 or kv.v_dim != kv.head_dim:
         return False
     hd, group = kv.head_dim, heads // kv.kv_heads
+    ops.quantised("attention", kv, q, out)
     if heads % kv.kv_heads or group > 64 or q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         return False
-    if not q.is_contiguous() or not out.is_contiguous():
+    if q.numel() != ctx.n_tokens * heads * hd or out.numel() != q.numel():
+        raise ValueError(f"attention takes queries and an output of {ctx.n_tokens} x {heads * hd}, not {list(q.shape)} and {list(out.shape)}")
+    if (q.data_ptr() | out.data_ptr()) & 15:
         return False
     takes_short = _q4_takes(hd, kv.page_size)
     if not takes_short and not _q4_any_long(ctx, group, hd):
@@ -482,13 +488,10 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
     items, plans = _q4_work(ctx, group, hd, kv.window, takes_short)
     cu = lib.cuda()
     if items is not None:
-        nt, n_items, which = items
-        ctas = cu.axon_attention_q4_ctas(hd, nt)
-        floats = 2 * ctas * 8 * nt * (hd + 2) + ctas
-        scratch = ctx.rt.zeroed_buffer(f"q4_scratch_{hd}_{nt}", (floats,), torch.float32)
+        nt, n_items, which, scratch, floats = items
         check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
                                    None if which is None else which.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
-                                   nt, scratch.data_ptr(), floats, _stream()))
+                                   nt, scratch, floats, _stream()))
     for n, pages, rows, tpt, tiles, n_tiles, spans, segments, table in plans:
         pool = ctx.rt.buffer("q4_prompt_pages", (pages, 1, 2, kv.kv_heads, 64, hd), torch.bfloat16)
         layout = lib.KvLayout(block_table=table.data_ptr(), table_stride=table.shape[1], page_size=64, kv_heads=kv.kv_heads, head_dim=hd,

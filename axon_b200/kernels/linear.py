@@ -12,7 +12,7 @@ from typing import Optional
 
 import torch
 
-from . import ops
+from . import fast, ops
 
 
 def linear(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -24,7 +24,6 @@ def linear(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, bias: Optional[t
     over K and its partial sums wait in scratch; ``ops.rmsnorm`` and ``ops.rope_kv_write``
     fold them on their way, ``ops.fold_partials`` does it for any other reader)."""
     if not precise:
-        from . import fast
         ran = fast.gemm(a, w, out, bias, accumulate, defer)
         if ran:
             return ran if isinstance(ran, fast.PendingFold) else None
@@ -36,7 +35,6 @@ def linear_swiglu(h: torch.Tensor, w_gate_up: torch.Tensor, act: torch.Tensor, r
     """``act = silu(gate) * up`` of ``h @ w_gate_up.T`` with interleaved gate/up rows."""
     n = h.shape[0]
     if not rt.precise:
-        from . import fast
         if fast.gemm_swiglu(h, w_gate_up, act):
             return
     gu = rt.buffer("gate_up", (n, w_gate_up.shape[0]), torch.float32)
@@ -47,7 +45,6 @@ def linear_swiglu(h: torch.Tensor, w_gate_up: torch.Tensor, act: torch.Tensor, r
 def attention(q: torch.Tensor, kv: ops.KvView, ctx, out: torch.Tensor, heads: int, scale: float,
               precise: bool = False) -> None:
     """Attention of the step's tokens over the paged cache (in the model's dtype or in 4 bits)."""
-    from . import fast
     if not precise and fast.attention(q, kv, ctx, out, heads, scale):
         return
     splits = fast.q4_plain_splits(ctx, heads, kv.kv_heads, kv.window) if kv.bits else 1
@@ -60,5 +57,4 @@ def attention_decode_fused(qkv: torch.Tensor, pending, table, rot: int, adjacent
     the sizes (or the 32-bit model) need the separate kernels, in which case nothing ran."""
     if precise:
         return False
-    from . import fast
     return fast.attention_decode_fused(qkv, pending, table, rot, adjacent, kv, ctx, out, heads, scale, write_kv)

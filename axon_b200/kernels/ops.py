@@ -204,16 +204,18 @@ def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: t
     """Rotates queries and keys and writes queries to ``q_out``, keys and values to the cache (quantised
     when ``kv`` has 4 bits).  ``pending`` (a ``fast.PendingFold`` whose output is ``qkv``): the product is
     still in partial sums; they are folded here (with the bias) and ``qkv`` itself is not read."""
-    _dev(qkv, table, positions, token_slot, q_out, kv.pool)
+    if kv.bits:
+        quantised("rope_kv_write", kv, qkv, table, positions, token_slot, q_out)
+    else:
+        _dev(qkv, table, positions, token_slot, q_out, kv.pool)
     n = q_out.shape[0]
     width = (heads + kv.kv_heads) * kv.head_dim + (kv.kv_heads * kv.v_dim if kv.planes == 2 else 0)
     if qkv.dtype != torch.float32 or qkv.shape[1] != width:
         raise ValueError("rope_kv_write reads float32 [n][(heads + kv_heads) * head_dim + kv_heads * v_dim]")
     if kv.bits:
-        _quantised("rope_kv_write", kv, qkv, q_out, positions, token_slot, table)
         if q_out.shape[1] != heads * kv.head_dim or qkv.shape[0] < n or positions.numel() < n or token_slot.numel() < n:
             raise ValueError("rope_kv_write takes a row of qkv, a position and a slot for each row of q_out")
-        if (positions.dtype, token_slot.dtype) != (torch.int32, torch.int32):
+        if positions.dtype != torch.int32 or token_slot.dtype != torch.int32:
             raise TypeError("positions and slots are int32")
         if table is not None and (table.dtype != torch.float32 or table.numel() < n * rot):
             raise ValueError("rope_kv_write takes a float32 rotation table [n][rot / 2][2]")
@@ -232,14 +234,18 @@ def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: t
                                         None if pending is None else _ptr(pending.bias), _stream()))
 
 
-def _quantised(what: str, kv: KvView, *tensors: Optional[torch.Tensor]) -> None:
-    """Refuse a view without quantised rows, or operands on another device than the one launches go to."""
+def quantised(what: str, kv: KvView, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuse a view without quantised rows, operands on another device than the one launches go to, and
+    operands that are not contiguous."""
     if not kv.bits:
         raise ValueError(f"{what} takes a cache with quantised rows")
     here = torch.cuda.current_device()
-    for t in (kv.pool, kv.block_table, *tensors):
-        if t is not None and t.device.index != here:
-            raise ValueError(f"{what}: an operand is on {t.device}, the current device is cuda:{here}")
+    if kv.pool.get_device() != here or kv.block_table.get_device() != here:
+        raise ValueError(f"{what}: the cache is on {kv.pool.device}, the current device is cuda:{here}")
+    for t in tensors:
+        if t is not None and (t.get_device() != here or not t.is_contiguous()):
+            raise ValueError(f"{what} takes contiguous CUDA tensors on the current device, cuda:{here}; there is no CPU path"
+                             f" (got one on {t.device})")
 
 
 def kv_read(kv: KvView, spans: torch.Tensor, keys: Optional[torch.Tensor], values: Optional[torch.Tensor] = None) -> None:
@@ -250,16 +256,16 @@ def kv_read(kv: KvView, spans: torch.Tensor, keys: Optional[torch.Tensor], value
     bfloat16, receives the position whose span covers ``r`` (the first such span); the numbers are exact in
     both types.  Rows of no span stay as they are, and so do those of positions outside the block table.
     Either output may be None; with one plane values are the keys."""
-    _quantised("kv_read", kv, spans, keys, values)
-    _dev(spans, keys, values, kv.pool)
+    quantised("kv_read", kv, spans, keys, values)
     if spans.dtype != torch.int32 or spans.dim() != 2 or spans.shape[0] != 4:
         raise ValueError("kv_read takes int32 spans [4][n]: slot, first position, count, first output row")
     if keys is None and values is None:
         raise ValueError("kv_read takes keys, values or both to write to")
     rows = (keys if keys is not None else values).shape[0]
-    for t, width, name in ((keys, kv.head_dim, "keys"), (values, kv.v_dim, "values")):
-        if t is not None and tuple(t.shape) != (rows, kv.kv_heads, width):
-            raise ValueError(f"kv_read writes {name} as [{rows}][{kv.kv_heads}][{width}], not {list(t.shape)}")
+    if keys is not None and keys.shape != (rows, kv.kv_heads, kv.head_dim):
+        raise ValueError(f"kv_read writes keys as [{rows}][{kv.kv_heads}][{kv.head_dim}], not {list(keys.shape)}")
+    if values is not None and values.shape != (rows, kv.kv_heads, kv.v_dim):
+        raise ValueError(f"kv_read writes values as [{rows}][{kv.kv_heads}][{kv.v_dim}], not {list(values.shape)}")
     if keys is not None and values is not None and keys.dtype != values.dtype:
         raise TypeError("keys and values are read back in one dtype")
     check(lib.cuda().axon_kv_read_q4(_ptr(kv.pool), kv._ref, _ptr(spans), spans.shape[1], kv.block_table.shape[0], _ptr(keys),
@@ -270,10 +276,9 @@ def attention_plain(q: torch.Tensor, kv: KvView, positions: torch.Tensor, token_
                     out: torch.Tensor, heads: int, scale: float, rt=None, splits: int = 1) -> None:
     """Attention of each token over its request's positions up to its own, by the plain kernels.  ``splits``
     (4-bit caches only; scratch comes from ``rt``): into how many shares each token's keys are cut."""
-    _dev(q, positions, token_slot, out, kv.pool)
     n = q.shape[0]
     if kv.bits:
-        _quantised("attention_plain", kv, q, positions, token_slot, out)
+        quantised("attention_plain", kv, q, positions, token_slot, out)
         if out.dtype != q.dtype or out.numel() != n * heads * kv.v_dim or q.numel() != n * heads * kv.head_dim:
             raise ValueError("attention_plain takes queries [n][heads * head_dim] and writes [n][heads * v_dim] in their dtype")
         scratch, floats = None, 0
@@ -284,6 +289,7 @@ def attention_plain(q: torch.Tensor, kv: KvView, positions: torch.Tensor, token_
                                                  kv._ref, n, heads, float(scale), int(kv.window), splits, _ptr(scratch), floats,
                                                  _stream()))
         return
+    _dev(q, positions, token_slot, out, kv.pool)
     if q.dtype != kv.pool.dtype or out.dtype != q.dtype:
         raise TypeError("queries, cache and output have one dtype")
     check(lib.cuda().axon_attention_plain(_ptr(q), _ptr(kv.pool), dtype_code(q), _ptr(positions), _ptr(token_slot),
