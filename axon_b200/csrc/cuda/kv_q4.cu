@@ -224,24 +224,31 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* _
                   long long n_rows, int rows_per_cta, int pad, Q4Out out) {
     __shared__ long long rec[Q4_READ_ROWS];                    // the row's record of kv head 0; -1: not written, -2: zeros
     __shared__ int at[Q4_READ_ROWS];                           // its place in the page
+    __shared__ int owner[Q4_READ_ROWS];                        // the first span that covers it
+    if (threadIdx.x < Q4_READ_ROWS) owner[threadIdx.x] = n_spans;
     pdl_launch_dependents();
     pdl_wait();
-    const long long r0 = (long long)blockIdx.x * rows_per_cta;
+    const long long r0 = (long long)blockIdx.x * rows_per_cta, r1 = min(r0 + rows_per_cta, n_rows);
+    __syncthreads();
+    for (int s = threadIdx.x; s < n_spans; s += Q4_READ_THREADS) {
+        const long long out0 = spans[3 * n_spans + s], count = max(spans[2 * n_spans + s], 0);
+        const long long a = max(out0, r0), b = min(out0 + (count + pad - 1) / pad * pad, r1);
+        for (long long r = a; r < b; ++r) atomicMin(&owner[r - r0], s);
+    }
+    __syncthreads();
     if (threadIdx.x < rows_per_cta) {
-        const long long r = r0 + threadIdx.x;
+        const int s = owner[threadIdx.x];
         long long where = -1;
         int in_page = 0;
-        for (int s = 0; s < n_spans && r < n_rows; ++s) {
-            const long long i = r - spans[3 * n_spans + s], count = spans[2 * n_spans + s];
-            if (i < 0 || i >= (count + pad - 1) / pad * pad) continue;
+        if (s < n_spans) {
+            const long long i = r0 + threadIdx.x - spans[3 * n_spans + s];
             const int slot = spans[s];
             const long long pos = spans[n_spans + s] + i, lp = pos / kv.page_size;
-            if (i >= count) where = -2;
+            if (i >= spans[2 * n_spans + s]) where = -2;
             else if (slot >= 0 && slot < n_slots && pos >= 0 && lp < kv.table_stride) {
                 where = kv.record_at(slot, (int)lp, 0);
                 in_page = (int)(pos - lp * kv.page_size);
             }
-            break;
         }
         rec[threadIdx.x] = where;
         at[threadIdx.x] = in_page;
