@@ -19,7 +19,7 @@
 // A warp works alone: its own ring of shared memory, filled by asynchronous copies of 16 bytes (with pages of 16
 // positions a kv head's codes and steps of keys and values are one run of 18 HD bytes), its own running
 // maximum and sum.  The maximum lags: O is rescaled only when a score exceeds it by 2^8.  The warps of a CTA take
-// chunks of 32 keys in turn and are merged at the end.  (Bulk copies counted by mbarriers were measured first: a
+// tiles of 16 keys in turn and are merged at the end.  (Bulk copies counted by mbarriers were measured first: a
 // copy's uniform operands cost the issuing warp some 30 instructions, these 5 a tile.)
 //
 // The grid is as many CTAs as fit at once, and the 16-key tiles of all (item, kv head) pairs, laid
@@ -35,10 +35,13 @@
 namespace axon {
 
 constexpr int QA_WARPS = 8, QA_THREADS = QA_WARPS * 32;
-constexpr int QA_KT = 2, QA_STAGES = 2;          // 16-key tiles per chunk, chunks in a warp's ring
+// 16-key tiles per chunk, chunks in a warp's ring (8 requests of 32,768 positions: 40.7 us; two chunks of two tiles 41.6,
+// four of one 42.9: what is in flight suffices, and smaller pieces share out better)
+constexpr int QA_KT = 1, QA_STAGES = 3;
 // A pair counts as its tiles and so many more when ranges are cut: what starting on it and merging the warps'
-// results cost the CTA, in tiles (with none, CTAs that met a dozen short requests finished last: see the launch bench of ragged contexts).
-constexpr int QA_PAIR_COST = 8;
+// results cost the CTA, in tiles.  64 requests of 300 to 8,192 positions: 53.8 us with none (CTAs that met a dozen short
+// requests finished last), 51.9 with 8, 47.3 with 16, 45.9 with 24.
+constexpr int QA_PAIR_COST = 24;
 constexpr int QA_LEAST = QA_WARPS * QA_KT;       // the shortest range: one chunk for each warp
 constexpr float QA_LAZY = 8.f;                   // log2 units a score may exceed the running maximum
 
@@ -672,7 +675,6 @@ attention_q4_kernel(const QaParams p) {
             __threadfence();
             last = atomicAdd(p.arrived + c0, 1u) == (unsigned)(c1 - c0);
             if (last) p.arrived[c0] = 0;                           // ready for the next launch
-            __threadfence();
         }
         __syncthreads();
         if (last) {

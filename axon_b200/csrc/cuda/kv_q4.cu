@@ -298,13 +298,13 @@ template <typename T>
 __global__ void __launch_bounds__(Q4P_THREADS)
 attention_q4_plain_kernel(const T* __restrict__ q, const uint8_t* __restrict__ pool, const int32_t* __restrict__ positions,
                           const int32_t* __restrict__ token_slot, T* __restrict__ out, PagedQ4 kv, int heads, float scale_log2,
-                          int window, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+                          int window, float* __restrict__ part_o, float2* __restrict__ part_ml, unsigned int* __restrict__ arrived) {
     extern __shared__ float q4p_smem[];
     const int hd = kv.hd, vd = kv.vd, group = heads / kv.kv_heads, blocks = (group + Q4P_HEADS - 1) / Q4P_HEADS;
     const int t = blockIdx.x, kh = blockIdx.y / blocks, h0 = kh * group + blockIdx.y % blocks * Q4P_HEADS;
     const int n_heads = min(Q4P_HEADS, (kh + 1) * group - h0);
     const int pitch = max(hd, vd) + 1;                         // odd: a column of the tile falls into 32 banks
-    float* qs = q4p_smem;                                      // [8][hd]
+    float* qs = q4p_smem;                                      // [hd][8]
     float* tile = qs + Q4P_HEADS * hd;                         // [64][pitch]
     float* sc = tile + Q4P_KEYS * pitch;                       // [64][8] scores, then weights
     __shared__ float m_run[Q4P_HEADS], l_run[Q4P_HEADS], corr[Q4P_HEADS];
@@ -317,7 +317,7 @@ attention_q4_plain_kernel(const T* __restrict__ q, const uint8_t* __restrict__ p
     const int tiles = (pos + 1 - lo_all + Q4P_KEYS - 1) / Q4P_KEYS, per = (tiles + gridDim.z - 1) / gridDim.z;
     const int lo = lo_all + (int)blockIdx.z * per * Q4P_KEYS, hi = min(pos + 1, lo + per * Q4P_KEYS);
     for (int i = tid; i < Q4P_HEADS * hd; i += Q4P_THREADS)
-        qs[i] = i / hd < n_heads ? ldf(q + ((long long)t * heads + h0) * hd + i) * scale_log2 : 0.f;
+        qs[i % hd * Q4P_HEADS + i / hd] = i / hd < n_heads ? ldf(q + ((long long)t * heads + h0) * hd + i) * scale_log2 : 0.f;
     if (tid < Q4P_HEADS) { m_run[tid] = -INFINITY; l_run[tid] = 0.f; }
     float acc[2][Q4P_HEADS];
 #pragma unroll
@@ -336,14 +336,27 @@ attention_q4_plain_kernel(const T* __restrict__ q, const uint8_t* __restrict__ p
         }
         __syncthreads();
         auto widen = [&](int codes, int steps, int width) {
+            constexpr int BATCH = 4;                           // words of a thread in flight together
             const int words = width / 8;
-            for (int i = tid; i < cnt * words; i += Q4P_THREADS) {
-                const int r = i / words, w = i % words;
-                const uint8_t* from = pool + rec[r];
-                const uint32_t word = *reinterpret_cast<const uint32_t*>(from + codes + ((long long)at[r] * words + w) * 4);
-                const float s = q4_step(from[steps + (long long)at[r] * (words / 2) + w / 2]);
+            for (int i0 = tid; i0 < cnt * words; i0 += BATCH * Q4P_THREADS) {
+                uint32_t word[BATCH];
+                int byte[BATCH];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) tile[r * pitch + w * 8 + j] = q4_digit(word, j) * s;
+                for (int k = 0; k < BATCH; ++k) {
+                    const int i = i0 + k * Q4P_THREADS, r = i / words, w = i - r * words;
+                    if (i >= cnt * words) continue;
+                    const uint8_t* from = pool + rec[r];
+                    word[k] = *reinterpret_cast<const uint32_t*>(from + codes + ((long long)at[r] * words + w) * 4);
+                    byte[k] = from[steps + (long long)at[r] * (words / 2) + w / 2];
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const int i = i0 + k * Q4P_THREADS, r = i / words, w = i - r * words;
+                    if (i >= cnt * words) continue;
+                    const float s = q4_step(byte[k]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) tile[r * pitch + w * 8 + j] = q4_digit(word[k], j) * s;
+                }
             }
         };
         widen(0, kv.k_steps, hd);
@@ -354,8 +367,8 @@ attention_q4_plain_kernel(const T* __restrict__ q, const uint8_t* __restrict__ p
                 const float* kr = tile + key * pitch;
                 for (int d = 0; d < hd; ++d) {
                     const float k = kr[d];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[i] = fmaf(qs[(half * 4 + i) * hd + d], k, s[i]);
+                    const float4 x = *reinterpret_cast<const float4*>(qs + d * Q4P_HEADS + half * 4);
+                    s[0] = fmaf(x.x, k, s[0]); s[1] = fmaf(x.y, k, s[1]); s[2] = fmaf(x.z, k, s[2]); s[3] = fmaf(x.w, k, s[3]);
                 }
             }
 #pragma unroll
@@ -418,31 +431,49 @@ attention_q4_plain_kernel(const T* __restrict__ q, const uint8_t* __restrict__ p
             else part_o[(part + i) * vd + d] = acc[c][i];
         }
     }
-    if (part_o != nullptr && tid < Q4P_HEADS) part_ml[part + tid] = make_float2(m_run[tid], l_run[tid]);
-}
-
-// The shares of a (token, head block) folded in ascending order: a CTA each.
-template <typename T>
-__global__ void __launch_bounds__(Q4P_THREADS)
-attention_q4_plain_fold_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, T* __restrict__ out, int heads,
-                               int kv_heads, int vd, int splits) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int group = heads / kv_heads, blocks = (group + Q4P_HEADS - 1) / Q4P_HEADS;
-    const int t = blockIdx.x, kh = blockIdx.y / blocks, h0 = kh * group + blockIdx.y % blocks * Q4P_HEADS;
-    const int n_heads = min(Q4P_HEADS, (kh + 1) * group - h0);
-    const long long part = ((long long)t * gridDim.y + blockIdx.y) * splits * Q4P_HEADS;
-    for (int i = threadIdx.x; i < n_heads * vd; i += Q4P_THREADS) {
+    if (part_o == nullptr) return;
+    if (tid < Q4P_HEADS) part_ml[part + tid] = make_float2(m_run[tid], l_run[tid]);
+    // the share that arrives last folds all of them, in ascending order
+    __shared__ bool last;
+    __syncthreads();
+    if (tid == 0) {
+        unsigned int* const counter = arrived + (long long)t * gridDim.y + blockIdx.y;
+        __threadfence();
+        last = atomicAdd(counter, 1u) == gridDim.z - 1;
+        __threadfence();
+        if (last) *counter = 0;                                // ready for the next launch
+    }
+    __syncthreads();
+    if (!last) return;
+    const long long first = part - (long long)blockIdx.z * Q4P_HEADS;
+    const int splits = gridDim.z;
+    for (int i = tid; i < n_heads * vd; i += Q4P_THREADS) {
         const int h = i / vd, d = i % vd;
-        float m = -INFINITY;
-        for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[part + s * Q4P_HEADS + h].x);
-        const float use = m == -INFINITY ? 0.f : m;
-        float l = 0.f, o = 0.f;
-        for (int s = 0; s < splits; ++s) {
-            const float2 ml = part_ml[part + s * Q4P_HEADS + h];
-            const float f = exp2f(ml.x - use);
-            l = fmaf(ml.y, f, l);
-            o = fmaf(part_o[(part + s * Q4P_HEADS + h) * vd + d], f, o);
+        constexpr int S = 8;                                   // shares asked for together
+        float top = -INFINITY, l = 0.f, o = 0.f;
+        for (int s0 = 0; s0 < splits; s0 += S) {
+            float2 ml[S];
+            float v[S];
+#pragma unroll
+            for (int k = 0; k < S; ++k) {
+                const bool there = s0 + k < splits;
+                const long long at_s = first + (long long)(s0 + k) * Q4P_HEADS + h;
+                ml[k] = there ? __ldcg(part_ml + at_s) : make_float2(-INFINITY, 0.f);
+                v[k] = there ? __ldcg(part_o + at_s * vd + d) : 0.f;
+            }
+            float up = top;
+#pragma unroll
+            for (int k = 0; k < S; ++k) up = fmaxf(up, ml[k].x);
+            const float use = up == -INFINITY ? 0.f : up, kept = exp2f(top - use);
+            top = up;
+            l *= kept;
+            o *= kept;
+#pragma unroll
+            for (int k = 0; k < S; ++k) {
+                const float f = exp2f(ml[k].x - use);
+                l = fmaf(ml[k].y, f, l);
+                o = fmaf(v[k], f, o);
+            }
         }
         stf(out + ((long long)t * heads + h0 + h) * vd + d, o / l);
     }
@@ -451,22 +482,17 @@ attention_q4_plain_fold_kernel(const float* __restrict__ part_o, const float2* _
 template <typename T>
 static int attention_q4_plain_launch(const T* q, const uint8_t* pool, const int32_t* positions, const int32_t* token_slot, T* out,
                                      const PagedQ4& kv, int n, int heads, float scale_log2, int window, int splits, float* scratch,
-                                     cudaStream_t stream) {
+                                     int32_t* counters, cudaStream_t stream) {
     const int group = heads / kv.kv_heads, gy = kv.kv_heads * ((group + Q4P_HEADS - 1) / Q4P_HEADS);
     const size_t smem = (Q4P_HEADS * kv.hd + Q4P_KEYS * ((kv.hd > kv.vd ? kv.hd : kv.vd) + 1) + Q4P_KEYS * Q4P_HEADS) * sizeof(float);
     constexpr size_t most = (Q4P_HEADS * 256 + Q4P_KEYS * 257 + Q4P_KEYS * Q4P_HEADS) * sizeof(float);
     if (int st = ensure_dynamic_smem<attention_q4_plain_kernel<T>>(most, "axon_attention_q4_plain")) return st;
     float* po = splits > 1 ? scratch : nullptr;
     float2* ml = splits > 1 ? reinterpret_cast<float2*>(scratch + (long long)n * gy * splits * Q4P_HEADS * kv.vd) : nullptr;
+    unsigned int* arrived = splits > 1 ? reinterpret_cast<unsigned int*>(counters) : nullptr;
     launch_pdl(attention_q4_plain_kernel<T>, dim3(n, gy, splits), dim3(Q4P_THREADS), smem, stream, q, pool, positions, token_slot, out, kv,
-               heads, scale_log2, window, po, ml);
-    if (int st = launch_status("axon_attention_q4_plain")) return st;
-    if (splits > 1) {
-        launch_pdl(attention_q4_plain_fold_kernel<T>, dim3(n, gy), dim3(Q4P_THREADS), 0, stream, (const float*)po, (const float2*)ml, out,
-                   heads, kv.kv_heads, kv.vd, splits);
-        return launch_status("axon_attention_q4_plain fold");
-    }
-    return AXON_OK;
+               heads, scale_log2, window, po, ml, arrived);
+    return launch_status("axon_attention_q4_plain");
 }
 
 }  // namespace axon
@@ -597,7 +623,8 @@ AXON_API long long axon_attention_q4_plain_scratch(int n, int heads, int kv_head
 
 AXON_API int axon_attention_q4_plain(const void* q, const void* pool, int dtype, const int32_t* positions, const int32_t* token_slot,
                                      void* out, const AxonKvLayout* layout, int n, int heads, float scale, int window, int splits,
-                                     float* scratch, long long scratch_floats, cudaStream_t stream) {
+                                     float* scratch, long long scratch_floats, int32_t* counters, long long n_counters, cudaStream_t stream) {
+    // counters: one for each (token, eight heads of a kv head), zeroed once; launches leave them zero
     if (n <= 0) return AXON_OK;
     PagedQ4 kv;
     if (int st = to_q4(layout, pool, "axon_attention_q4_plain", &kv)) return st;
@@ -607,11 +634,12 @@ AXON_API int axon_attention_q4_plain(const void* q, const void* pool, int dtype,
     if ((long long)kv.kv_heads * ((heads / kv.kv_heads + Q4P_HEADS - 1) / Q4P_HEADS) > 65535) { set_error("axon_attention_q4_plain: %d heads are too many", heads); return AXON_BAD_ARGUMENT; }
     const long long need = axon_attention_q4_plain_scratch(n, heads, kv.kv_heads, kv.vd, splits);
     if (need > 0 && (scratch == nullptr || scratch_floats < need || ((uintptr_t)scratch & 15))) { set_error("axon_attention_q4_plain: %d key shares need %lld floats of 16-byte aligned scratch", splits, need); return AXON_BAD_ARGUMENT; }
+    if (need > 0 && (counters == nullptr || n_counters < (long long)n * kv.kv_heads * ((heads / kv.kv_heads + Q4P_HEADS - 1) / Q4P_HEADS))) { set_error("axon_attention_q4_plain: %lld counters are too few", n_counters); return AXON_BAD_ARGUMENT; }
     const float scale_log2 = scale * 1.4426950408889634f;
     if (dtype == AXON_Q4_F32)
-        return attention_q4_plain_launch<float>((const float*)q, (const uint8_t*)pool, positions, token_slot, (float*)out, kv, n, heads, scale_log2, window, splits, scratch, stream);
+        return attention_q4_plain_launch<float>((const float*)q, (const uint8_t*)pool, positions, token_slot, (float*)out, kv, n, heads, scale_log2, window, splits, scratch, counters, stream);
     if (dtype == AXON_Q4_BF16)
-        return attention_q4_plain_launch<__nv_bfloat16>((const __nv_bfloat16*)q, (const uint8_t*)pool, positions, token_slot, (__nv_bfloat16*)out, kv, n, heads, scale_log2, window, splits, scratch, stream);
+        return attention_q4_plain_launch<__nv_bfloat16>((const __nv_bfloat16*)q, (const uint8_t*)pool, positions, token_slot, (__nv_bfloat16*)out, kv, n, heads, scale_log2, window, splits, scratch, counters, stream);
     set_error("axon_attention_q4_plain: unknown dtype %d", dtype);
     return AXON_BAD_ARGUMENT;
 }

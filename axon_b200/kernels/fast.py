@@ -367,6 +367,23 @@ def q4_plain_splits(ctx, heads: int, kv_heads: int, window: int) -> int:
     return max(1, min(-(-keys // Q4_PLAIN_KEYS), Q4_PLAIN_CTAS // max(ctas, 1)))
 
 
+
+
+def q4_plain_shares(ctx, kv, heads: int):
+    """The same with its scratch (None for one share), cached per step."""
+    key = ("q4_plain", heads, kv.kv_heads, kv.v_dim, kv.window)
+    got = ctx.scratch.get(key)
+    if got is None:
+        n = q4_plain_splits(ctx, heads, kv.kv_heads, kv.window)
+        got = ops.KeyShares()
+        if n > 1:
+            floats = lib.cuda().axon_attention_q4_plain_scratch(ctx.n_tokens, heads, kv.kv_heads, kv.v_dim, n)
+            got = ops.KeyShares(n, ctx.rt.buffer("q4_plain_scratch", (floats,), torch.float32),
+                                ctx.rt.zeroed_buffer("q4_plain_counters", (ctx.n_tokens * heads,), torch.int32))
+        ctx.scratch[key] = got
+    return got
+
+
 #: row tiles of 8 that the kernel holds at once, by head size
 Q4_ROW_TILES = {64: 4, 128: 4, 256: 1}
 

@@ -62,7 +62,7 @@ _SIGNATURES = {
                           c_longlong, P],
     "axon_attention_q4_ctas": [c_int, c_int],
     "axon_attention_q4_plain": [P, P, c_int, P, P, P, ctypes.POINTER(KvLayout), c_int, c_int, c_float, c_int, c_int, P,
-                                c_longlong, P],
+                                c_longlong, P, c_longlong, P],
     "axon_attention_plain": [P, P, c_int, P, P, P, ctypes.POINTER(KvLayout), c_int, c_int, c_float, c_int, P],
     "axon_residual_add": [P, P, c_int, c_longlong, P],
     "axon_convert": [P, c_int, P, c_int, c_longlong, P],

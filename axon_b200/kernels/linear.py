@@ -47,8 +47,8 @@ def attention(q: torch.Tensor, kv: ops.KvView, ctx, out: torch.Tensor, heads: in
     """Attention of the step's tokens over the paged cache (in the model's dtype or in 4 bits)."""
     if not precise and fast.attention(q, kv, ctx, out, heads, scale):
         return
-    splits = fast.q4_plain_splits(ctx, heads, kv.kv_heads, kv.window) if kv.bits else 1
-    ops.attention_plain(q, kv, ctx.positions, ctx.token_slot, out, heads, scale, rt=ctx.rt, splits=splits)
+    shares = fast.q4_plain_shares(ctx, kv, heads) if kv.bits else None
+    ops.attention_plain(q, kv, ctx.positions, ctx.token_slot, out, heads, scale, shares=shares)
 
 
 def attention_decode_fused(qkv: torch.Tensor, pending, table, rot: int, adjacent: bool, kv: ops.KvView, ctx,

@@ -272,22 +272,30 @@ def kv_read(kv: KvView, spans: torch.Tensor, keys: Optional[torch.Tensor], value
                                      _ptr(values), dtype_code(keys if keys is not None else values), rows, _stream()))
 
 
+@dataclass
+class KeyShares:
+    """How the plain attention over a 4-bit cache cuts each token's keys: the number of shares, float32 scratch for their
+    results (``axon_attention_q4_plain_scratch``), and int32 counters (zero, and left so), one per token and head at least."""
+
+    count: int = 1
+    scratch: Optional[torch.Tensor] = None
+    arrived: Optional[torch.Tensor] = None
+
+
 def attention_plain(q: torch.Tensor, kv: KvView, positions: torch.Tensor, token_slot: torch.Tensor,
-                    out: torch.Tensor, heads: int, scale: float, rt=None, splits: int = 1) -> None:
-    """Attention of each token over its request's positions up to its own, by the plain kernels.  ``splits``
-    (4-bit caches only; scratch comes from ``rt``): into how many shares each token's keys are cut."""
+                    out: torch.Tensor, heads: int, scale: float, shares: Optional[KeyShares] = None) -> None:
+    """Attention of each token over its request's positions up to its own, by the plain kernels.  ``shares``
+    (4-bit caches only): into how many shares each token's keys are cut, with their scratch."""
     n = q.shape[0]
     if kv.bits:
         quantised("attention_plain", kv, q, positions, token_slot, out)
         if out.dtype != q.dtype or out.numel() != n * heads * kv.v_dim or q.numel() != n * heads * kv.head_dim:
             raise ValueError("attention_plain takes queries [n][heads * head_dim] and writes [n][heads * v_dim] in their dtype")
-        scratch, floats = None, 0
-        if splits > 1:
-            floats = lib.cuda().axon_attention_q4_plain_scratch(n, heads, kv.kv_heads, kv.v_dim, splits)
-            scratch = rt.buffer("q4_plain_scratch", (floats,), torch.float32)
+        x = shares or KeyShares()
         check(lib.cuda().axon_attention_q4_plain(_ptr(q), _ptr(kv.pool), dtype_code(q), _ptr(positions), _ptr(token_slot), _ptr(out),
-                                                 kv._ref, n, heads, float(scale), int(kv.window), splits, _ptr(scratch), floats,
-                                                 _stream()))
+                                                 kv._ref, n, heads, float(scale), int(kv.window), x.count, _ptr(x.scratch),
+                                                 0 if x.scratch is None else x.scratch.numel(), _ptr(x.arrived),
+                                                 0 if x.arrived is None else x.arrived.numel(), _stream()))
         return
     _dev(q, positions, token_slot, out, kv.pool)
     if q.dtype != kv.pool.dtype or out.dtype != q.dtype:
