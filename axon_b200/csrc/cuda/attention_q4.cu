@@ -295,12 +295,16 @@ attention_q4_kernel(const QaParams p) {
     uint8_t* const ring = qa_smem + warp * (QA_STAGES * QA_KT * T::BYTES);
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
     pdl_launch_dependents();
-    pdl_wait();
 
+    // The division of the work and the first table entries do not wait for the kernel before: segments, lists and
+    // tables are copied to the device ahead of a step's kernels, none of which writes them.
     int item;
     uint32_t start;
     const QaPlan plan(p, R, &item, &start);
-    if (item >= p.n_items) return;                                 // (nothing left for this CTA)
+    if (item >= p.n_items) {                                       // nothing left for this CTA
+        pdl_wait();
+        return;
+    }
     uint32_t f = blockIdx.x * plan.per;
     const uint32_t f1 = f + min(plan.per, plan.total - f), per = plan.per;
     const QaMagic magic;
@@ -392,7 +396,7 @@ attention_q4_kernel(const QaParams p) {
     // first keys; while they come queries become B fragments, with the factors that bring rows' scores to log2 units
     uint32_t qf[NT == 1 ? HD / 16 : 1][2];
     float factor[NT][2];
-    auto begin_pair = [&]() {
+    auto begin_pair = [&](auto first_of_all) {
         head_src = p.pool + p.kv.entry_offset + (long long)kvh * p.kv.record;
         table = p.kv.block_table + (long long)it.slot * p.kv.table_stride;
         last_page = (it.kv_hi - 1) / ps;
@@ -400,6 +404,7 @@ attention_q4_kernel(const QaParams p) {
 #pragma unroll
         for (int j = 0; j < QA_STAGES; ++j) x[j] = pages(tile0 + warp * QA_KT + j * TURN);
         next = pages(tile0 + warp * QA_KT + QA_STAGES * TURN);
+        if (decltype(first_of_all)::value) pdl_wait();             // keys and queries may be the work of the kernel before
         const int r = NT == 1 ? g : 8 * warp + g, row = it.row0 + r;
         const bool mine = NT == 1 || warp < NT, live = mine && r < it.rows;
         uint4 raw[HD / 32];
@@ -428,8 +433,11 @@ attention_q4_kernel(const QaParams p) {
         }
     };
 
-    if (!advance()) return;
-    begin_pair();
+    if (!advance()) {
+        pdl_wait();
+        return;
+    }
+    begin_pair(std::true_type());
     for (;;) {
     const int rows = it.rows, pos_first = it.pos_first, pos_last = it.pos_last, row0 = it.row0, q_start = it.q_start;
     const int kv_lo = it.kv_lo, kv_hi = it.kv_hi;
@@ -637,7 +645,7 @@ attention_q4_kernel(const QaParams p) {
     const uint32_t first_place = pair_begin + plan.cost, last_place = first_place + it.tiles - 1;      // of the pair's tiles
     const int head0 = kvh * p.group;
     const bool more = advance();
-    if (more) begin_pair();
+    if (more) begin_pair(std::false_type());
     auto write_out = [&](int r, int d, const float4& acc, float sum) {
         const float inv = 128.f / sum;                             // (values carry a 1 / 128, as keys do)
         const int row = row0 + r, ahead = row < p.group ? 0 : row / p.group, tok = q_start + ahead, head = head0 + row - ahead * p.group;

@@ -129,12 +129,14 @@ rope_kv_write_q4_vec_kernel(const float* __restrict__ qkv, const float2* __restr
                             const int32_t* __restrict__ token_slot, T* __restrict__ q_out, uint8_t* __restrict__ pool, PagedQ4 kv,
                             int heads, int write_kv, SplitFold fold) {
     pdl_launch_dependents();
-    pdl_wait();
     const int t = blockIdx.x, half = kv.hd / 2, lanes = half / 4;                  // threads of a row
     const int items = (heads + (write_kv ? 2 * kv.kv_heads : 0)) * lanes;
     const float* row = qkv + (long long)t * ((heads + 2 * kv.kv_heads) * kv.hd);
+    // (positions, slots and tables are copied to the device ahead of a step's kernels: no need to wait for the one before)
     const int pos = positions[t], lp = pos / kv.page_size, in_page = pos - lp * kv.page_size;
-    const long long page = write_kv ? kv.record_at(token_slot[t], lp, 0) : 0;
+    const int entry = write_kv ? kv.block_table[(long long)token_slot[t] * kv.table_stride + lp] : 0;
+    pdl_wait();
+    const long long page = (long long)kv.page(entry) * kv.page_stride + kv.entry_offset;
     // (the items of a row are a multiple of four, so the lanes of a group are all here or all beyond the last item)
     for (int it = blockIdx.y * Q4_WRITE_THREADS + threadIdx.x; it < items; it += gridDim.y * Q4_WRITE_THREADS) {
         const int h = it / lanes, i0 = (it - h * lanes) * 4, col = h * kv.hd;

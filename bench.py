@@ -141,7 +141,8 @@ def prefill_flops(cfg, T):
 class Workbench:
     """An engine of one shape with random weights, and the timed workloads on it."""
 
-    def __init__(self, shape: str, layers: int, max_slots: int, pool_tokens, max_positions: int, max_step_tokens: int):
+    def __init__(self, shape: str, layers: int, max_slots: int, pool_tokens, max_positions: int, max_step_tokens: int,
+                 kv: str = "auto"):
         import torch
 
         import axon_b200 as axon
@@ -155,10 +156,13 @@ class Workbench:
         t0 = time.time()
         self.engine = build_engine(config=self.cfg, seed=1, dtype="bfloat16", page_size=16, max_tokens=pool_tokens,
                                    max_slots=max_slots, max_positions=max_positions, max_step_tokens=max_step_tokens,
-                                   gain_std=0.0)
+                                   gain_std=0.0, kv=kv)
         self.net = axon.Backend(None, axon.BackendOptions(), engine=self.engine)
         for g in self.engine.cache.groups:      # synthetic keys and values
-            g.pool.normal_(0.0, 0.5)
+            if g.need.bits:                     # bytes that are fine as codes and as steps (0.125 to 0.47)
+                g.pool.random_(0x60, 0x70)
+            else:
+                g.pool.normal_(0.0, 0.5)
         torch.cuda.synchronize()
         self.setup_s = time.time() - t0
         self.gen = torch.Generator().manual_seed(0)
@@ -177,7 +181,7 @@ class Workbench:
         from axon_b200.kernels import lib
         torch, engine, net = self.torch, self.engine, self.net
         V = self.cfg.vocab_size
-        _, weight_bytes, kv_bytes_per_pos = sizes_of(self.cfg)
+        weight_bytes, kv_bytes_per_pos = sizes_of(self.cfg)[1], engine.cache.bytes_per_token()
         caches = [net.new_cache() for _ in range(b)]
         for c in caches:          # a synthetic context: pages taken, keys and values random
             assert engine.cache.reserve(c.slot, context), "the bench's pool is too small for its contexts"
@@ -256,7 +260,7 @@ def bench_7b(args, pk, pk_src):
     room = args.context + 2 * args.steps + args.warmup + 3 + 64      # warm-up, the timed steps, the end-to-end steps
     pool_tokens = max(max_b * (-(-room // 16) * 16), args.prefill_tokens + 64)
     wb = Workbench("7b", args.layers, max_b, pool_tokens, max(room, args.prefill_tokens + 64),
-                   max(args.prefill_tokens, 64))
+                   max(args.prefill_tokens, 64), kv=args.kv)
     cfg = wb.cfg
     if args.prefill_only:
         ms = wb.time_prefill(args.prefill_tokens, max(3, args.steps))
@@ -297,6 +301,8 @@ def bench_7b(args, pk, pk_src):
         "clocks": next((r["clocks"] for r in main if r["clocks"]), None),
         "setup_s": round(wb.setup_s, 1),
     }
+    if args.kv != "auto":
+        out["config"]["kv"] = args.kv
     if prefill_ms:
         T, pm = args.prefill_tokens, med(prefill_ms)
         out["prefill"] = {"value": round(T / (pm / 1e3), 1), "tokens": T, "ms": round(pm, 3),
@@ -422,6 +428,7 @@ def main() -> int:
     ap.add_argument("--gpus", type=int, default=1)
     ap.add_argument("--steps", type=int, default=64)
     ap.add_argument("--warmup", type=int, default=8)
+    ap.add_argument("--kv", default="auto", choices=["auto", "q4"], help="cache type of the 7B workloads (q4: 4 bits a value)")
     ap.add_argument("--rounds", type=int, default=3, help="interleaved repeats of every measurement (medians are reported)")
     ap.add_argument("--impl", default="axon_b200", choices=["axon_b200", "reference"])
     ap.add_argument("--shape", default="7b", choices=["7b", "1.5b", "32b"],

@@ -417,6 +417,16 @@ def test_on_another_stream_and_in_a_graph(ops):
         on_side = out.clone()
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(on_side, eager)
+    # lists that a kernel on the stream has only just written
+    fresh = (ctx.segments, ctx.positions, ctx.token_slot, cache.view.block_table)
+    kept = [x.clone() for x in fresh]
+    for k in range(20):
+        for x, y in zip(fresh, kept):
+            x.zero_()
+            x.add_(y)
+        out.zero_()
+        run()
+        assert torch.equal(out, eager)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         run()
