@@ -3,6 +3,8 @@
 // kv_layout.h, the arithmetic in kv_q4.cuh.
 #include "kv_q4.cuh"
 
+#include <type_traits>
+
 namespace axon {
 
 __device__ __forceinline__ float4 q4_load4(const float* row, const SplitFold& fold, int t, int n) {
@@ -184,12 +186,12 @@ rope_kv_write_q4_vec_kernel(const float* __restrict__ qkv, const float2* __restr
 // threads find each row's span and page once, then every thread takes one word of eight codes of a row through all heads
 // and both planes, several loads at a time; neighbouring threads go along a row and then along positions,
 // which is how both sides lie in memory.  Output row r of plane p and kv head h starts at
-//   (r / block) * block_stride + (r % block) * row_stride + h * head_stride.
+//   (r / block) * block_stride + (r % block) * row_stride + h * head_stride,   block = 2^block_shift.
 // Bound by the bytes written, 3.6 times those read in bfloat16.
 struct Q4Out {
     void *k, *v;
     long long block_stride, row_stride, head_stride;
-    int block;
+    int block_shift;
 };
 template <typename T>
 __device__ __forceinline__ void q4_store8(T* dst, uint32_t word, int byte);
@@ -264,27 +266,47 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* _
     const int r_step = max(threads / words, 1);
     for (int i = tid; i < (threads / words > 0 ? r_step * words : words); i += threads) {      // (a row of more words than threads: several of them)
         const int w = i % words;
-        for (int r = i / words; r < rows_per_cta; r += r_step) {
-            if (rec[r] == -1) continue;
-            const bool held = rec[r] >= 0;
-            const uint8_t* from = pool + (held ? rec[r] : 0);
-            const uint8_t* const word_at = from + codes + ((long long)at[r] * words + w) * 4;
-            const uint8_t* const step_at = from + steps + (long long)at[r] * (words / 2) + w / 2;
-            const long long row = r0 + r;
-            T* dst = base + row / out.block * out.block_stride + row % out.block * out.row_stride + w * 8;
-            for (int h0 = 0; h0 < kv.kv_heads; h0 += Q4_READ_BATCH) {
-                uint32_t word[Q4_READ_BATCH];
-                int byte[Q4_READ_BATCH];
+        constexpr int ROWS = 2;                                // a thread's rows whose loads are in flight together
+        for (int ra = i / words; ra < rows_per_cta; ra += ROWS * r_step) {
+            long long where[ROWS];
+            const uint8_t *word_at[ROWS], *step_at[ROWS];
+            T* dst[ROWS];
 #pragma unroll
-                for (int k = 0; k < Q4_READ_BATCH; ++k) {
-                    const bool there = held && h0 + k < kv.kv_heads;
-                    word[k] = there ? *reinterpret_cast<const uint32_t*>(word_at + (long long)(h0 + k) * kv.record) : 0x88888888u;
-                    byte[k] = there ? step_at[(long long)(h0 + k) * kv.record] : 0;
-                }
-#pragma unroll
-                for (int k = 0; k < Q4_READ_BATCH; ++k)
-                    if (h0 + k < kv.kv_heads) q4_store8<T>(dst + (h0 + k) * out.head_stride, word[k], byte[k]);
+            for (int q = 0; q < ROWS; ++q) {
+                const int r = ra + q * r_step;
+                where[q] = r < rows_per_cta ? rec[r] : -1;
+                const long long row = r0 + r;
+                const int place = where[q] >= 0 ? at[r] : 0;
+                // (rows that hold nothing load from the pool's start and store zeros, or store nothing)
+                word_at[q] = pool + (where[q] >= 0 ? where[q] : 0) + codes + (place * words + w) * 4;
+                step_at[q] = pool + (where[q] >= 0 ? where[q] : 0) + steps + place * (words / 2) + w / 2;
+                dst[q] = base + (row >> out.block_shift) * out.block_stride + (row & ((1 << out.block_shift) - 1)) * out.row_stride + w * 8;
             }
+            auto batch = [&](auto n) {                         // `n` heads
+                uint32_t word[ROWS][decltype(n)::value];
+                int byte[ROWS][decltype(n)::value];
+#pragma unroll
+                for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+                    for (int k = 0; k < decltype(n)::value; ++k) {
+                        word[q][k] = *reinterpret_cast<const uint32_t*>(word_at[q] + k * kv.record);
+                        byte[q][k] = step_at[q][k * kv.record];
+                    }
+#pragma unroll
+                for (int q = 0; q < ROWS; ++q) {
+                    if (where[q] != -1) {
+#pragma unroll
+                        for (int k = 0; k < decltype(n)::value; ++k)
+                            q4_store8<T>(dst[q] + k * out.head_stride, where[q] >= 0 ? word[q][k] : 0x88888888u, where[q] >= 0 ? byte[q][k] : 0);
+                    }
+                    word_at[q] += decltype(n)::value * kv.record;
+                    step_at[q] += decltype(n)::value * kv.record;
+                    dst[q] += decltype(n)::value * out.head_stride;
+                }
+            };
+            int h = 0;
+            for (; h + Q4_READ_BATCH <= kv.kv_heads; h += Q4_READ_BATCH) batch(std::integral_constant<int, Q4_READ_BATCH>());
+            for (; h < kv.kv_heads; ++h) batch(std::integral_constant<int, 1>());
         }
     }
 }
@@ -565,7 +587,7 @@ AXON_API int axon_kv_read_q4(const void* pool, const AxonKvLayout* layout, const
         void* const k = apart && part ? nullptr : keys;
         void* const v = apart && !part ? nullptr : values;
         const long long width = k != nullptr ? kv.hd : kv.vd;
-        const Q4Out out{k, v, kv.kv_heads * width, 0, width, 1};
+        const Q4Out out{k, v, kv.kv_heads * width, 0, width, 0};
         if (int st = kv_read_launch(pool, kv, spans, n_spans, n_slots, dtype, n_rows, 1, out, stream)) return st;
     }
     return AXON_OK;
@@ -612,7 +634,7 @@ AXON_API int axon_kv_read_q4_pages(const void* pool, const AxonKvLayout* layout,
     if (kv.planes != 2 || kv.vd != kv.hd) { set_error("axon_kv_read_q4_pages: takes caches with key and value planes of one width"); return AXON_BAD_ARGUMENT; }
     if ((uintptr_t)pages_out & 15) { set_error("axon_kv_read_q4_pages: outputs must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
     const long long plane = (long long)kv.kv_heads * 64 * kv.hd;
-    const Q4Out out{pages_out, (uint8_t*)pages_out + plane * (dtype == AXON_Q4_F32 ? 4 : 2), 2 * plane, kv.hd, 64ll * kv.hd, 64};
+    const Q4Out out{pages_out, (uint8_t*)pages_out + plane * (dtype == AXON_Q4_F32 ? 4 : 2), 2 * plane, kv.hd, 64ll * kv.hd, 6};
     return kv_read_launch(pool, kv, spans, n_spans, n_slots, dtype, 64ll * pages, 64, out, stream);
 }
 

@@ -51,7 +51,7 @@ inline int to_q4(const AxonKvLayout* l, const void* pool, const char* what, Page
     const long long kc = up((long long)l->page_size * l->head_dim / 2), ks = up((long long)l->page_size * l->head_dim / 16);
     const long long vc = up((long long)l->page_size * vd / 2), vs = up((long long)l->page_size * vd / 16);
     const long long record = kc + ks + (l->planes == 1 ? 0 : vc + vs);
-    if (record > (1 << 30)) { set_error("%s: pages of %d positions are too large", what, l->page_size); return AXON_BAD_ARGUMENT; }
+    if (record > (1 << 28)) { set_error("%s: pages of %d positions are too large", what, l->page_size); return AXON_BAD_ARGUMENT; }
     PagedQ4 q;
     q.block_table = l->block_table; q.fault = l->fault;
     q.page_stride = l->page_stride; q.entry_offset = l->entry_offset;

@@ -62,10 +62,10 @@ def step_workspace_bytes(hidden_size: int, vocab_size: int, max_step_tokens: int
 
 def quantised_workspace_bytes(needs, max_slots: int, max_positions: int) -> int:
     """What prompts over a quantised cache take beside it: the bfloat16 pages that their keys and values are read back into."""
-    from ..kernels.fast import Q4_PROMPT_POSITIONS
+    from ..kernels.fast import q4_prompt_room
     widest = max((n.elements_per_token for entry in needs for n in entry.values() if getattr(n, "bits", 0)), default=0)
-    positions = min(max_slots * max_positions, max(max_positions, Q4_PROMPT_POSITIONS))
-    return 2 * widest * positions * 9 // 8
+    pages, ints = q4_prompt_room(max_slots, max_positions, max_slots * max_positions)
+    return 2 * widest * 64 * pages + 4 * ints if widest else 0
 
 
 def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] = None,

@@ -82,6 +82,10 @@ class Engine:
     def __init__(self, model: DecoderModel, cache: PagedCache, max_step_tokens: int = 8192):
         self.model, self.cache, self.rt = model, cache, model.rt
         self.rt.kv_page_size = cache.page_size
+        if self.rt.kv_bits:
+            from ..kernels import fast
+            self.rt.kv_prompt_pages, self.rt.kv_prompt_entries = fast.q4_prompt_room(
+                cache.max_slots, cache.max_positions, cache.n_pages * cache.page_size)
         self.max_step_tokens = max_step_tokens
         self._staging: List[torch.Tensor] = []
         self._events: List[Optional[torch.cuda.Event]] = []

@@ -414,6 +414,13 @@ def _q4_bucket(n: int) -> int:
     return -(-n // step) * step
 
 
+def q4_prompt_room(max_slots: int, max_positions: int, pool_positions: int):
+    """The most that a step's prompts take: (pages of 64 positions read back, integers of their plan)."""
+    at_once = min(max_slots * max_positions, max(max_positions, Q4_PROMPT_POSITIONS), pool_positions + 64 * max_slots)
+    longest = _q4_bucket(-(-max_positions // 64) + 1)
+    return _q4_bucket(-(-at_once // 64) + max_slots), max_slots * (8 + longest)
+
+
 def _q4_prompt_sizes(ctx, segs, window: int):
     """(pages of 64 positions that these segments' keys take, those of the longest), rounded up."""
     n = []
@@ -470,7 +477,8 @@ def _q4_work(ctx, group: int, hd: int, window: int, takes_short: bool):
         flat = list(segs) + [x for _, i, t0 in sorted(work, reverse=True) for x in (i, t0)]
         lists = ctx.rt.upload_i32(f"q4_prompt_{group}_{rows}", flat)
         n = len(segs)
-        ints = ctx.rt.buffer(f"q4_plan_{window}_{k}", (8 * n + n * stride,), torch.int32)
+        ints = ctx.rt.buffer(f"q4_plan_{window}_{k}", (max(8 * n + n * stride, ctx.rt.kv_prompt_entries),), torch.int32)
+        ints = ints[:8 * n + n * stride]
         check(lib.cuda().axon_q4_prompt_plan(ctx.segments.data_ptr(), n_seg, lists.data_ptr(), n, window, pages, stride, ints.data_ptr(),
                                              ints[4 * n:].data_ptr(), ints[8 * n:].data_ptr(), _stream()))
         plans.append((n, pages, rows, tpt, lists[n:], len(work), ints[:4 * n], ints[4 * n:8 * n], ints[8 * n:].view(n, stride)))
@@ -484,7 +492,8 @@ def _q4_takes(hd: int, page_size: int) -> bool:
 
 
 def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
-    """Tensor-core attention over a 4-bit cache.  Segments of few query rows read the pages as they are; long ones have
+    """Tensor-core attention over a 4-bit cache.  Its scratch belongs to ``ctx.rt``: calls that share a Runtime have to be
+    ordered (on one stream, or on streams that wait for one another).  Segments of few query rows read the pages as they are; long ones have
     the positions that they see read back once per layer, into pages that the bfloat16 attention takes.  Refuses dtypes
     other than bfloat16, planes of two widths, groups of more than 64 heads, and head sizes and pages that
     neither way takes (short: head sizes 64, 128 and 256, a multiple of 4 positions a page at 64, of 2 at 128; long:
@@ -510,7 +519,7 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
                                    None if which is None else which.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
                                    nt, scratch, floats, _stream()))
     for n, pages, rows, tpt, tiles, n_tiles, spans, segments, table in plans:
-        pool = ctx.rt.buffer("q4_prompt_pages", (pages, 1, 2, kv.kv_heads, 64, hd), torch.bfloat16)
+        pool = ctx.rt.buffer("q4_prompt_pages", (max(pages, ctx.rt.kv_prompt_pages), 1, 2, kv.kv_heads, 64, hd), torch.bfloat16)
         layout = lib.KvLayout(block_table=table.data_ptr(), table_stride=table.shape[1], page_size=64, kv_heads=kv.kv_heads, head_dim=hd,
                               page_stride=2 * kv.kv_heads * 64 * hd, entry_offset=0, v_offset=kv.kv_heads * 64 * hd, v_dim=hd, planes=2,
                               n_pages=pages - 1, bits=0, fault=None)

@@ -50,8 +50,10 @@ class Runtime:
             raise ValueError(f"cache rows have the model's dtype (0) or 4 bits a value, not {kv_bits}")
         #: bits of a cached value (0: the model's dtype) in the caches of parts that take them (``Part.kv_bits``)
         self.kv_bits = kv_bits
-        #: positions per cache page (the engine sets it)
+        #: positions per cache page, and what a step of prompts over a quantised cache takes at most: pages of 64
+        #: positions read back, block-table entries for them (the engine sets them, so that these buffers never grow)
         self.kv_page_size = 0
+        self.kv_prompt_pages, self.kv_prompt_entries = 0, 0
         #: the true 32-bit path: plain FFMA kernels everywhere
         self.precise = dtype == torch.float32
         self._buffers: Dict[str, torch.Tensor] = {}

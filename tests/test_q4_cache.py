@@ -70,6 +70,29 @@ def test_cache_types_by_name():
         BackendOptions().kv("f32")
 
 
+def test_room_for_prompts_is_never_outgrown():
+    """What a step's prompts need, however they lie, fits the buffers that the engine asks for once."""
+    from types import SimpleNamespace
+    from axon_b200.engine.build import quantised_workspace_bytes
+    from axon_b200.kernels import fast
+    from axon_b200.parts.spec import KvNeed
+    rng = np.random.default_rng(5)
+    for slots, most, pool in ((1, 100, 128), (16, 4096, 65536), (8, 32768, 100000), (128, 2000, 20000), (300, 70, 21000)):
+        pages, ints = fast.q4_prompt_room(slots, most, pool)
+        for _ in range(30):
+            n = int(rng.integers(1, slots + 1))
+            kv = np.minimum(rng.integers(1, most + 1, n), max(1, pool // n))
+            q = np.minimum(rng.integers(1, most + 1, n), kv)
+            if kv.sum() > max(most, fast.Q4_PROMPT_POSITIONS):
+                continue                                  # (such a step is taken in groups)
+            ctx = SimpleNamespace(seg_q_len=q.tolist(), seg_kv_len=kv.tolist())
+            for window in (0, 50):
+                p, stride = fast._q4_prompt_sizes(ctx, range(n), window)
+                assert p <= pages and 8 * n + n * stride <= ints
+    assert quantised_workspace_bytes([{"mixer": KvNeed(4, 128)}], 16, 4096) == 0
+    assert quantised_workspace_bytes([{"mixer": KvNeed(4, 128, bits=4)}, {}], 16, 4096) >= 65536 * 4 * 2 * 128 * 2
+
+
 def test_views_of_quantised_pools_are_checked():
     from axon_b200.kernels import ops
     table = torch.zeros(1, 4, dtype=torch.int32)

@@ -270,7 +270,11 @@ def check_attention(ops, cache, q_lens, heads, dtype, window=0, weight_half=2.0 
     """Against float64, within a bound worked out for each number: a score is a sum of hd products in
     32 bits (2^-23 a step: tensor cores cut sums), scaled (2^-22 of its size with the exponential's own error),
     a weight is rounded to half its step (``weight_half``; none in the 32-bit model), sums over keys and the
-    output round again."""
+    output round again.
+
+    Weights below 2^-14 of the running maximum's are subnormal halves in the kernel for few rows: off by 2^-25
+    at most, whatever their size.  The running maximum never exceeds the row's, so the largest weight and the sum
+    that all are divided by are at least 1, and the output is off by 2^-25 times the sum of |v| at most."""
     out, ctx, q, pos, slot, scale = attend(ops, cache, q_lens, heads, dtype, window, **kw)
     got = out.double().cpu().numpy().reshape(len(pos), heads, -1)
     qd = q.double().cpu().numpy().reshape(len(pos), heads, -1)
@@ -282,7 +286,8 @@ def check_attention(ops, cache, q_lens, heads, dtype, window=0, weight_half=2.0 
         for h in range(heads):
             want, mass, size = q4.attention(qd[rows, h], cache.k[s][:, h // group], cache.v[s][:, h // group], pos[rows], window, scale)
             e_s = size * ((cache.hd + 4) * 2.0 ** -23 + 2.0 ** -22)
-            tol = mass * (weight + 2 * e_s[:, None] + 2.0 ** -20 + (cache.lens[s] + 8) * 2.0 ** -23) + 1.01 * HALF[dtype] * np.abs(want) + 1e-30
+            tiny = 2.0 ** -25 * np.abs(cache.v[s][:, h // group]).sum(0) if weight else 0.0
+            tol = tiny + mass * (weight + 2 * e_s[:, None] + 2.0 ** -20 + (cache.lens[s] + 8) * 2.0 ** -23) + 1.01 * HALF[dtype] * np.abs(want) + 1e-30
             err = np.abs(got[rows, h] - want)
             assert (err <= tol).all(), f"request {s} head {h}: worst error {float((err / tol).max()):.2f} of its bound"
     return out, ctx
@@ -330,6 +335,81 @@ def test_prompts(ops, heads, kv_heads, hd, ps, window):
     check_attention(ops, cache, [300, 259, 3, 1, 100, 0], heads, torch.bfloat16, window, weight_half=2.0 ** -8)
     check_attention(ops, cache, [0, 0, 0, 0, 0, 129], heads, torch.bfloat16, window, weight_half=2.0 ** -8)
     check_attention(ops, cache, [0, 700, 0, 0, 650, 0], heads, torch.bfloat16, window, weight_half=2.0 ** -8)
+
+
+def test_many_requests(ops):
+    """More requests than a warp has lanes, with lengths far apart: ranges that hold parts of several pairs."""
+    rng = np.random.default_rng(6)
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(900), 75))]
+    for hd, heads, kv_heads in ((128, 6, 2), (64, 4, 4)):
+        cache = Cache(ops, lens, kv_heads, hd, 16, seed=23)
+        check_attention(ops, cache, [1] * 75, heads, torch.bfloat16)
+        check_attention(ops, cache, [min(l, 1 + i % 5) for i, l in enumerate(lens)], heads, torch.bfloat16, weight_half=2.0 ** -8)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_scales(ops, scale):
+    cache = Cache(ops, [70, 300], 2, 128, 16, seed=24)
+    for dtype in DTYPES:
+        check_attention(ops, cache, [1, 4], 6, dtype, scale=scale, weight_half=2.0 ** -8)
+
+
+def test_pages_gigabytes_apart(ops):
+    """A pool of more than 2**32 bytes: rows written to, read from and attended over in its first and last pages."""
+    kv_heads, hd, heads = 2, 128, 6
+    record = q4.parts(16, hd, hd, 2)[1]
+    n_pages = 2 ** 32 // (kv_heads * record) + 40
+    pool = torch.zeros(n_pages + 1, 1, kv_heads * record, dtype=torch.uint8, device=DEV)
+    table = i32([[n_pages - 1, 3, n_pages - 7, 0]])
+    for ps, view in ((16, ops.KvView(pool, table, 0, 16, kv_heads, hd, bits=4)),):
+        n = 60
+        qkv = torch.randn(n, (heads + 2 * kv_heads) * hd, generator=torch.Generator().manual_seed(3)).to(DEV)
+        q = torch.empty(n, heads * hd, dtype=torch.bfloat16, device=DEV)
+        ops.rope_kv_write(qkv, None, i32(range(n)), i32([0] * n), q, view, heads, 0)
+        k = torch.empty(n, kv_heads, hd, device=DEV)
+        v = torch.empty_like(k)
+        ops.kv_read(view, i32([[0], [0], [n], [0]]), k, v)
+        x = qkv.cpu().numpy()[:, heads * hd:].reshape(n, 2 * kv_heads, hd)
+        want = q4.values(*q4.quantise(x))
+        assert (k.double().cpu().numpy() == want[:, :kv_heads]).all() and (v.double().cpu().numpy() == want[:, kv_heads:]).all()
+        cache = Cache.__new__(Cache)
+        cache.lens, cache.kv_heads, cache.hd, cache.v_dim, cache.view = [n], kv_heads, hd, hd, view
+        cache.k, cache.v = [want[:, :kv_heads]], [want[:, kv_heads:]]
+        for q_len in (1, 5, 60):
+            check_attention(ops, cache, [q_len], heads, torch.bfloat16, weight_half=2.0 ** -8)
+        check_attention(ops, cache, [2], heads, torch.float32)
+
+
+def test_checked_tables(ops):
+    """With a fault record, an entry beyond the pool is recorded and the sink page used in its place, by every kernel."""
+    for hd, heads, kv_heads, dtype, q_lens in ((128, 6, 2, torch.bfloat16, [1]), (128, 28, 4, torch.bfloat16, [300]), (48, 3, 3, torch.float32, [1])):
+        cache = Cache(ops, [300], kv_heads, hd, 16, seed=25)
+        n_pages = cache.pool.shape[0] - 1
+        fault = torch.zeros(2, dtype=torch.int32, device=DEV)
+        view = ops.KvView(cache.pool, cache.dev_table, 1, 16, kv_heads, hd, bits=4, fault=fault)
+        cache.view = view
+        attend(ops, cache, q_lens, heads, dtype)
+        assert fault.tolist() == [0, 0]
+        plain = attend(ops, cache, q_lens, heads, dtype)[0].clone()
+        cache.view = ops.KvView(cache.pool, cache.dev_table, 1, 16, kv_heads, hd, bits=4)
+        assert torch.equal(attend(ops, cache, q_lens, heads, dtype)[0], plain)
+        cache.view = view
+        cache.pool[n_pages] = 0                           # the sink: finite
+        for bad in (n_pages + 5, -3):
+            cache.dev_table[0, 2] = bad
+            attend(ops, cache, q_lens, heads, dtype)
+            assert fault.tolist() == [1, bad]
+            fault.zero_()
+            ops.kv_read(view, i32([[0], [32], [4], [0]]), torch.empty(4, kv_heads, hd, device=DEV))
+            assert fault.tolist() == [1, bad]
+            fault.zero_()
+            before = cache.pool[:n_pages].clone()
+            for rot in (0, hd):
+                tab = torch.from_numpy(rope([33], hd)).to(DEV) if rot else None
+                ops.rope_kv_write(torch.ones(1, (heads + 2 * kv_heads) * hd, device=DEV), tab, i32([33]), i32([0]),
+                                  torch.empty(1, heads * hd, dtype=dtype, device=DEV), view, heads, rot)
+                assert fault.tolist() == [1, bad] and torch.equal(cache.pool[:n_pages], before)
+                fault.zero_()
 
 
 def test_prompts_read_back_in_groups(ops, monkeypatch):
@@ -538,6 +618,38 @@ def test_serving_with_a_quantised_cache(model_folders):
             assert axon.generate(alone, cache, p, logits, axon.GenOpts.greedy(24)).ids == o
     full = axon.Backend(axon.load(model_folders["C"]), axon.BackendOptions().max_ctx(256).dtype("float32"))
     assert net.engine.cache.bytes_per_token() * 64 == full.engine.cache.bytes_per_token() * 9
+
+
+def test_command_line(model_folders):
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT
+    run = lambda *a: subprocess.run([sys.executable, os.path.join(ROOT, "bin", "axon"), "gen", model_folders["C"], "1 2 3", "-n", "5", *a],  # noqa: E731
+                                    capture_output=True, text=True, timeout=300)
+    got = run("--kv", "q4")
+    assert got.returncode == 0 and len(got.stdout.split()) >= 5, got.stderr
+    bad = run("--kv", "q5")
+    assert bad.returncode != 0 and "q5" in bad.stderr
+
+
+def test_graphs_outlive_longer_contexts(model_folders):
+    """Portions of one size at the end of ever longer requests move no buffer that a captured step reads (the engine's own
+    buffers follow the tokens of a step, and what a portion reads back follows its context)."""
+    from axon_b200.engine.step import StepEntry
+    from test_engine_gpu import tokens_for
+    e = engine_for(model_folders["C"], "bfloat16", max_tokens=4096, max_positions=1000, max_step_tokens=1000)
+    a, b = e.open_request(), e.open_request()
+    e.step([StepEntry(b, tokens_for("C", 1, 100), [99])])
+    e.step([StepEntry(a, tokens_for("C", 0, 9), [8])])
+    for t in range(4):
+        e.step([StepEntry(a, [t], [0])])
+    graphs = dict(e._graphs)
+    assert graphs
+    for i in range(8):
+        e.step([StepEntry(b, tokens_for("C", 2 + i, 100), [99])])
+    e.step([StepEntry(a, [7], [0])])
+    assert all(e._graphs.get(k) is g for k, g in graphs.items()), "a captured step was thrown away"
 
 
 def test_reading_what_a_request_holds(model_folders):
