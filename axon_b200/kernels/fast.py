@@ -367,8 +367,6 @@ def q4_plain_splits(ctx, heads: int, kv_heads: int, window: int) -> int:
     return max(1, min(-(-keys // Q4_PLAIN_KEYS), Q4_PLAIN_CTAS // max(ctas, 1)))
 
 
-
-
 def q4_plain_shares(ctx, kv, heads: int):
     """The same with its scratch (None for one share), cached per step."""
     key = ("q4_plain", heads, kv.kv_heads, kv.v_dim, kv.window)
@@ -393,19 +391,47 @@ def _q4_row_tiles(rows: int, hd: int) -> int:
     return next((n for n in (1, 2, 4) if 8 * n >= rows or n == Q4_ROW_TILES[hd]))
 
 
-#: segments with more query rows (tokens x heads of a group) than this attend over keys and values read back into
-#: bfloat16 pages; the 4-bit kernel, which widens the keys anew for every 32 rows, takes the others
-Q4_SHORT_ROWS = 256
+#: query rows (tokens x heads of a group) up to which a segment always takes the 4-bit kernel, where there is one
+Q4_SHORT_ROWS = 64
 #: positions that are read back at a time (of several requests; one request is never cut)
 Q4_PROMPT_POSITIONS = 1 << 18
+#: Microseconds, measured on portions of 8 to 128 tokens of one and eight requests at 1,024 to 32,768 positions, heads
+#: 28 / 4 and 12 / 2 of 128 and 14 / 2 of 64: the 4-bit kernel takes a start and 1.2 ns for each 32 rows, kv head and 16 keys
+#: of 128 channels; reading back and the bfloat16 kernels a start and, for each CTA's tile of rows, 22 ns (head size 128, one
+#: CTA an SM) or 31 ns (smaller heads, three) a key.  128 tokens of one request at 8,192 positions, 28 / 4 heads: 81 us
+#: against 183; 64 tokens of eight requests at 2,048: 94 against 64.
+Q4_SHORT_START, Q4_SHORT_TILE, Q4_LONG_START = 8.0, 1.2e-3, 10.0
+Q4_LONG_KEY = {128: (0.022, SM_COUNT), 64: (0.031, 3 * SM_COUNT)}
 
 
-def _q4_is_long(n: int, group: int, hd: int) -> bool:
-    return hd in FA_HEAD_DIMS and n * group > Q4_SHORT_ROWS
-
-
-def _q4_any_long(ctx, group: int, hd: int) -> bool:
-    return _q4_is_long(ctx.max_q_len, group, hd)
+def _q4_long(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: bool):
+    """The segments that attend over keys and values read back into bfloat16 pages, because that is modelled to be
+    faster than the 4-bit kernel, which widens the keys anew for every 32 query rows.  Without ``takes_short`` (the 4-bit kernel
+    refuses the sizes): all of them if any has more than a few rows, else none."""
+    if hd not in FA_HEAD_DIMS or ctx.max_q_len * group <= Q4_SHORT_ROWS:
+        return ()
+    key = ("q4_long", group, kv_heads, hd, window, takes_short)
+    got = ctx.scratch.get(key)
+    if got is not None:
+        return got
+    got = tuple(range(len(ctx.seg_q_len)))
+    if takes_short:
+        got = tuple(s for s in got if ctx.seg_q_len[s] * group > Q4_SHORT_ROWS)
+        per_key, at_once = Q4_LONG_KEY[hd]
+        tpt = (256 if hd == 128 else 64) // group
+        short, tiles, longest = 0.0, 0.0, 0.0
+        for s in got:
+            n, kv = ctx.seg_q_len[s], ctx.seg_kv_len[s]
+            keys = min(kv - n / 2, window + tpt) if window else kv - n / 2        # that a tile of rows sees, about
+            short += -(-n * group // 32) * keys / 16
+            tiles += -(-n // tpt) * keys
+            longest = max(longest, min(kv, window + tpt) if window else kv)
+        t_short = Q4_SHORT_START + short * kv_heads * Q4_SHORT_TILE * hd / 128
+        t_long = Q4_LONG_START + per_key * max(longest, tiles * kv_heads / at_once)
+        if t_short <= t_long:
+            got = ()
+    ctx.scratch[key] = got
+    return got
 
 
 def _q4_bucket(n: int) -> int:
@@ -431,35 +457,38 @@ def _q4_prompt_sizes(ctx, segs, window: int):
     return _q4_bucket(sum(n)), _q4_bucket(max(n))
 
 
-def _q4_work(ctx, group: int, hd: int, window: int, takes_short: bool):
-    """The step's work for the 4-bit attention, cached per step: tiles of query rows (token * group + head) of short
-    segments ``(row tiles, items, list or None, scratch, its floats)`` or None, and groups of long ones (of all, without ``takes_short``)."""
-    key = ("q4_work", group, hd, window, takes_short)
+def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: bool):
+    """The step's work for the 4-bit attention, cached per step: launches of the 4-bit kernel (row tiles, items, list or None,
+    scratch, its floats), and groups of segments whose keys are read back."""
+    key = ("q4_work", group, kv_heads, hd, window, takes_short)
     got = ctx.scratch.get(key)
     if got is not None:
         return got
     n_seg = len(ctx.seg_q_len)
-    short = [s for s in range(n_seg) if not _q4_is_long(ctx.seg_q_len[s], group, hd)] if takes_short else []
-    items = None
-    if short:
-        most = max(ctx.seg_q_len[s] for s in short) * group
+    long = set(_q4_long(ctx, group, kv_heads, hd, window, takes_short))
+    short = [s for s in range(n_seg) if s not in long and ctx.seg_q_len[s] > 0]
+    launches = []
+    # single tokens beside portions get a launch of their own: with one row tile two CTAs fit an SM
+    few = [s for s in short if ctx.seg_q_len[s] * group <= 8]
+    for segs in ([short] if len(few) in (0, len(short)) else [few, [s for s in short if ctx.seg_q_len[s] * group > 8]]):
+        if not segs:
+            continue
+        most = max(ctx.seg_q_len[s] for s in segs) * group
         nt = _q4_row_tiles(most, hd)
-        if len(short) == n_seg and most <= 8 * nt:
-            items = (nt, n_seg, None)                    # (item i is segment i)
+        if len(segs) == n_seg and most <= 8 * nt:
+            n_items, which = n_seg, None                 # (item i is segment i)
         else:
             work = []
-            for s in short:
+            for s in segs:
                 n, kv_len = ctx.seg_q_len[s], ctx.seg_kv_len[s]
                 work += [(kv_len - n + min(n, -(-(r + 8 * nt) // group)), s, r) for r in range(0, n * group, 8 * nt)]
             flat = [x for _, s, r in sorted(work, reverse=True) for x in (s, r)]     # the longest must not start last
-            items = (nt, len(work), ctx.rt.upload_i32(f"q4_items_{group}_{hd}", flat))
+            n_items, which = len(work), ctx.rt.upload_i32(f"q4_items_{group}_{hd}_{nt}", flat).data_ptr()
         ctas = lib.cuda().axon_attention_q4_ctas(hd, nt)
         floats = 2 * ctas * 8 * nt * (hd + 2) + ctas
-        items += (ctx.rt.zeroed_buffer(f"q4_scratch_{hd}_{nt}", (floats,), torch.float32).data_ptr(), floats)
+        launches.append((nt, n_items, which, ctx.rt.zeroed_buffer(f"q4_scratch_{hd}_{nt}", (floats,), torch.float32).data_ptr(), floats))
     groups, at, room = [], [], 0
-    for s in range(n_seg):
-        if s in short:
-            continue
+    for s in sorted(long):
         if at and room + ctx.seg_kv_len[s] > Q4_PROMPT_POSITIONS:
             groups.append(at)
             at, room = [], 0
@@ -481,8 +510,14 @@ def _q4_work(ctx, group: int, hd: int, window: int, takes_short: bool):
         ints = ints[:8 * n + n * stride]
         check(lib.cuda().axon_q4_prompt_plan(ctx.segments.data_ptr(), n_seg, lists.data_ptr(), n, window, pages, stride, ints.data_ptr(),
                                              ints[4 * n:].data_ptr(), ints[8 * n:].data_ptr(), _stream()))
-        plans.append((n, pages, rows, tpt, lists[n:], len(work), ints[:4 * n], ints[4 * n:8 * n], ints[8 * n:].view(n, stride)))
-    got = (items, plans)
+        room = max(pages, ctx.rt.kv_prompt_pages)
+        pool = ctx.rt.buffer(f"q4_prompt_pages_{kv_heads}_{hd}", (room, 2, kv_heads, 64, hd), torch.bfloat16)
+        layout = lib.KvLayout(block_table=ints[8 * n:].data_ptr(), table_stride=stride, page_size=64, kv_heads=kv_heads, head_dim=hd,
+                              page_stride=2 * kv_heads * 64 * hd, entry_offset=0, v_offset=kv_heads * 64 * hd, v_dim=hd, planes=2,
+                              n_pages=room - 1, bits=0, fault=None)
+        plans.append((n, pages, rows, tpt, lists[n:].data_ptr(), len(work), ints.data_ptr(), ints[4 * n:].data_ptr(), pool.data_ptr(),
+                      ctypes.byref(layout)))
+    got = (launches, plans)
     ctx.scratch[key] = got
     return got
 
@@ -493,8 +528,8 @@ def _q4_takes(hd: int, page_size: int) -> bool:
 
 def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
     """Tensor-core attention over a 4-bit cache.  Its scratch belongs to ``ctx.rt``: calls that share a Runtime have to be
-    ordered (on one stream, or on streams that wait for one another).  Segments of few query rows read the pages as they are; long ones have
-    the positions that they see read back once per layer, into pages that the bfloat16 attention takes.  Refuses dtypes
+    ordered (on one stream, or on streams that wait for one another).  Segments of few query rows read the pages as they are; for long ones the
+    positions that they see are read back once per layer, into pages that the bfloat16 attention takes, where that is faster.  Refuses dtypes
     other than bfloat16, planes of two widths, groups of more than 64 heads, and head sizes and pages that
     neither way takes (short: head sizes 64, 128 and 256, a multiple of 4 positions a page at 64, of 2 at 128; long:
     head sizes 16, 32, 64 and 128).  Where only the long way takes a step that has long segments, all of it goes there."""
@@ -509,28 +544,22 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
     if (q.data_ptr() | out.data_ptr()) & 15:
         return False
     takes_short = _q4_takes(hd, kv.page_size)
-    if not takes_short and not _q4_any_long(ctx, group, hd):
+    if not takes_short and not _q4_long(ctx, group, kv.kv_heads, hd, kv.window, False):
         return False
-    items, plans = _q4_work(ctx, group, hd, kv.window, takes_short)
+    launches, plans = _q4_work(ctx, group, kv.kv_heads, hd, kv.window, takes_short)
     cu = lib.cuda()
-    if items is not None:
-        nt, n_items, which, scratch, floats = items
+    for nt, n_items, which, scratch, floats in launches:
         check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
-                                   None if which is None else which.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
+                                   which, n_items, kv._ref, heads, float(scale), int(kv.window),
                                    nt, scratch, floats, _stream()))
-    for n, pages, rows, tpt, tiles, n_tiles, spans, segments, table in plans:
-        pool = ctx.rt.buffer("q4_prompt_pages", (max(pages, ctx.rt.kv_prompt_pages), 1, 2, kv.kv_heads, 64, hd), torch.bfloat16)
-        layout = lib.KvLayout(block_table=table.data_ptr(), table_stride=table.shape[1], page_size=64, kv_heads=kv.kv_heads, head_dim=hd,
-                              page_stride=2 * kv.kv_heads * 64 * hd, entry_offset=0, v_offset=kv.kv_heads * 64 * hd, v_dim=hd, planes=2,
-                              n_pages=pages - 1, bits=0, fault=None)
-        check(cu.axon_kv_read_q4_pages(kv.pool.data_ptr(), kv._ref, spans.data_ptr(), n, kv.block_table.shape[0], pool.data_ptr(), 1,
-                                       pages, _stream()))
+    for n, pages, rows, tpt, tiles, n_tiles, spans, segments, pool, layout in plans:
+        check(cu.axon_kv_read_q4_pages(kv.pool.data_ptr(), kv._ref, spans, n, kv.block_table.shape[0], pool, 1, pages, _stream()))
         if rows == 256:
-            check(cu.axon_attention_tc(q.data_ptr(), pool.data_ptr(), out.data_ptr(), segments.data_ptr(), n, tiles.data_ptr(), n_tiles,
-                                       ctypes.byref(layout), heads, float(scale), int(kv.window), tpt, _stream()))
+            check(cu.axon_attention_tc(q.data_ptr(), pool, out.data_ptr(), segments, n, tiles, n_tiles, layout, heads, float(scale),
+                                       int(kv.window), tpt, _stream()))
         else:
-            check(cu.axon_attention_fa(q.data_ptr(), pool.data_ptr(), out.data_ptr(), segments.data_ptr(), n, tiles.data_ptr(), n_tiles,
-                                       ctypes.byref(layout), heads, float(scale), int(kv.window), 0, tpt, 1, None, None, _stream()))
+            check(cu.axon_attention_fa(q.data_ptr(), pool, out.data_ptr(), segments, n, tiles, n_tiles, layout, heads, float(scale),
+                                       int(kv.window), 0, tpt, 1, None, None, _stream()))
     return True
 
 
@@ -541,9 +570,11 @@ def q4_graph_key(ctx, heads: int, kv_heads: int, head_dim: int, window: int, pre
     group = heads // kv_heads
     key = []
     takes = not precise and ENABLED["attention_q4"] and group <= 64
-    if takes and _q4_any_long(ctx, group, head_dim):
+    takes_short = takes and _q4_takes(head_dim, ctx.rt.kv_page_size)
+    long = _q4_long(ctx, group, kv_heads, head_dim, window, takes_short) if takes else ()
+    if long:
         # (a portion of one request: steps of several are never captured)
-        key.append(("q4_prompt",) + _q4_prompt_sizes(ctx, range(len(ctx.seg_q_len)), window))
-    elif not (takes and _q4_takes(head_dim, ctx.rt.kv_page_size)):
+        key.append(("q4_prompt",) + _q4_prompt_sizes(ctx, long, window))
+    elif not takes_short:
         key.append(("q4_plain", q4_plain_splits(ctx, heads, kv_heads, window)))
     return tuple(key)

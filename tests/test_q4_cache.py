@@ -70,6 +70,28 @@ def test_cache_types_by_name():
         BackendOptions().kv("f32")
 
 
+def test_which_segments_are_read_back():
+    """The rule between the 4-bit kernel and reading back, against measured times (microseconds: 4-bit kernel, read back)."""
+    from types import SimpleNamespace
+    from axon_b200.kernels import fast
+    measured = {  # (heads, kv heads, head size, requests, tokens, positions)
+        (28, 4, 128, 1, 16, 8192): (25, 154), (28, 4, 128, 1, 128, 8192): (81, 183), (28, 4, 128, 1, 128, 1024): (24, 34),
+        (28, 4, 128, 8, 32, 2048): (54, 63), (28, 4, 128, 8, 64, 2048): (94, 64), (28, 4, 128, 1, 128, 32768): (273, 702),
+        (28, 4, 128, 1, 2048, 8192): (892, 331), (12, 2, 128, 8, 64, 2048): (49, 58), (12, 2, 128, 1, 128, 32768): (125, 695),
+        (14, 2, 64, 8, 64, 2048): (35, 71), (14, 2, 64, 1, 128, 8192): (28, 251),
+    }
+    for (heads, kv_heads, hd, n, tokens, kv), (short, long) in measured.items():
+        ctx = SimpleNamespace(seg_q_len=[tokens] * n, seg_kv_len=[kv] * n, max_q_len=tokens, scratch={})
+        took = fast._q4_long(ctx, heads // kv_heads, kv_heads, hd, 0, True)
+        assert len(took) in (0, n) and (bool(took) == (long < short)), (heads, kv_heads, hd, n, tokens, kv)
+    mixed = SimpleNamespace(seg_q_len=[1, 2000, 9, 1900], seg_kv_len=[5000, 2000, 40, 1900], max_q_len=2000, scratch={})
+    assert fast._q4_long(mixed, 7, 4, 128, 0, True) == (1, 3)
+    assert fast._q4_long(mixed, 2, 1, 16, 0, False) == (0, 1, 2, 3)       # no 4-bit kernel: everything, once something is long
+    assert fast._q4_long(mixed, 7, 4, 256, 0, True) == ()
+    few = SimpleNamespace(seg_q_len=[1, 3], seg_kv_len=[5000, 2000], max_q_len=3, scratch={})
+    assert fast._q4_long(few, 2, 1, 16, 0, False) == () and not few.scratch
+
+
 def test_room_for_prompts_is_never_outgrown():
     """What a step's prompts need, however they lie, fits the buffers that the engine asks for once."""
     from types import SimpleNamespace

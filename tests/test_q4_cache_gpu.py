@@ -420,6 +420,33 @@ def test_prompts_read_back_in_groups(ops, monkeypatch):
     check_attention(ops, cache, [300, 200, 150, 150, 1], 6, torch.bfloat16, weight_half=2.0 ** -8)
 
 
+def force(monkeypatch, way):
+    """Make every segment of more than 64 query rows go one way."""
+    from axon_b200.kernels import fast
+    monkeypatch.setattr(fast, "Q4_LONG_START" if way == "read back" else "Q4_SHORT_START", -1e9)
+
+
+@pytest.mark.parametrize("way", ["read back", "4-bit"])
+@pytest.mark.parametrize("heads,kv_heads,hd,ps", [(28, 4, 128, 16), (6, 2, 64, 32), (64, 1, 128, 16), (3, 1, 32, 16), (7, 1, 128, 48)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_prompts_by_either_way(ops, monkeypatch, way, heads, kv_heads, hd, ps, window):
+    force(monkeypatch, way)
+    cache = Cache(ops, [300, 700, 41, 1, 650, 129], kv_heads, hd, ps, window=window, seed=26, loud=0.5)
+    for q_lens in ([300, 259, 3, 1, 100, 0], [0, 0, 0, 0, 0, 129], [0, 700, 0, 0, 650, 0], [22, 1, 41, 1, 65, 2]):
+        check_attention(ops, cache, q_lens, heads, torch.bfloat16, window, weight_half=2.0 ** -8)
+
+
+def test_groups_of_prompts(ops, monkeypatch):
+    """Prompts read back in several groups, beside portions that are not."""
+    from axon_b200.kernels import fast
+    force(monkeypatch, "read back")
+    monkeypatch.setattr(fast, "Q4_PROMPT_POSITIONS", 700)
+    cache = Cache(ops, [300, 300, 900, 150, 333], 2, 128, 16, seed=27)
+    out, ctx = check_attention(ops, cache, [300, 200, 150, 150, 1], 6, torch.bfloat16, weight_half=2.0 ** -8)
+    plans = next(v[1] for k, v in ctx.scratch.items() if k[0] == "q4_work")
+    assert len(plans) == 3
+
+
 def test_what_is_not_finite_stays_with_who_sees_it(ops):
     """A NaN key or value is NaN for the tokens that see it and for no others, in every head's own channels."""
     for hd, heads, kv_heads in ((128, 6, 2), (64, 4, 4)):
