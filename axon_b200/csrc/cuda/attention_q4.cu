@@ -28,6 +28,10 @@
 // keys before it merges the warps' results of the last.  A pair that lies in one range whole is written out; the pieces
 // of the others go to scratch (at most two per CTA: the one its range begins in and the one it ends in), and the
 // CTA whose piece arrives last folds them in ascending order, so results do not depend on the order of arrival.
+//
+// Measured on a B200 (28 query and 4 kv heads of 128): 64 requests of 300 to 8,192 positions, 157 MB, 43 us = 3.65 TB/s,
+// 0.56 of the measured copy rate; 8 of 32,768 39 us (0.59); 8 of 2,048 7.8 us; one of 519 5.3 us.  The loop alone runs
+// at 0.8 of the copy rate, issuing 54 % of the time; the rest is the chain at both ends of a launch.
 #include "kv_q4.cuh"
 
 #include <type_traits>
@@ -239,8 +243,9 @@ struct QaPlan {
         }
         tiles = __reduce_add_sync(0xffffffffu, tiles) * p.kv.kv_heads;
         longest = __reduce_max_sync(0xffffffffu, longest);
-        // one CTA folds a pair's pieces: with few long pairs, as long a range (a turn of 16 tiles takes about 0.9 us) as the
-        // fold of as many pieces (0.05 us each) would take, which is about the square root of a pair's tiles
+        // one CTA folds a pair's pieces (about 0.12 us each): with few long pairs, ranges as long as the fold of their
+        // number, which is about the square root of a pair's tiles (one request of 32,768 positions: 16.2 us; with 1.5 times
+        // as long ranges 17.7, twice 19.9, 0.7 times 15.9)
         const uint32_t least = max((uint32_t)QA_LEAST, (uint32_t)sqrtf((float)longest));
         const uint32_t even = (tiles + p.ctas - 1) / p.ctas;
         padded = true;
