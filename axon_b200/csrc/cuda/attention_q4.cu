@@ -39,14 +39,13 @@
 namespace axon {
 
 constexpr int QA_WARPS = 8, QA_THREADS = QA_WARPS * 32;
-// 16-key tiles per chunk, chunks in a warp's ring (8 requests of 32,768 positions: 40.7 us; two chunks of two tiles 41.6,
-// four of one 42.9: what is in flight suffices, and smaller pieces share out better)
-constexpr int QA_KT = 1, QA_STAGES = 3;
+// Tiles in a warp's ring (8 requests of 32,768 positions: 40.7 us; four 42.9; two times two tiles 41.6)
+constexpr int QA_STAGES = 3;
 // A pair counts as its tiles and so many more when ranges are cut: what starting on it and merging the warps'
 // results cost the CTA, in tiles.  64 requests of 300 to 8,192 positions: 53.8 us with none (CTAs that met a dozen short
 // requests finished last), 51.9 with 8, 47.3 with 16, 45.9 with 24.
 constexpr int QA_PAIR_COST = 24;
-constexpr int QA_LEAST = QA_WARPS * QA_KT;       // the shortest range: one chunk for each warp
+constexpr int QA_LEAST = QA_WARPS;               // the shortest range: one tile for each warp
 constexpr float QA_LAZY = 8.f;                   // log2 units a score may exceed the running maximum
 
 struct QaParams {
@@ -65,8 +64,8 @@ struct QaParams {
 
 template <int HD> struct QaTile {
     static constexpr int KC = 8 * HD, KS = HD, BYTES = 2 * (KC + KS);      // codes and steps of 16 keys; a tile with its values
-    static constexpr int PIECES = BYTES / 16, LANE_PIECES = (QA_KT * PIECES + 31) / 32;   // 16-byte pieces of a tile; of a chunk per lane
-    static constexpr int RING = QA_WARPS * QA_STAGES * QA_KT * BYTES;
+    static constexpr int PIECES = BYTES / 16, LANE_PIECES = (PIECES + 31) / 32;      // 16-byte pieces of a tile, of a lane
+    static constexpr int RING = QA_WARPS * QA_STAGES * BYTES;
     static constexpr int PITCH = HD + 8;                                    // floats between rows of the merge buffer
     static constexpr int merge(int nt) { return QA_WARPS * 8 * nt * (PITCH + 2) * 4; }
     static constexpr int queries(int nt) { return nt > 1 ? HD / 16 * nt * 32 * 8 + 8 * nt * 4 : 0; }
@@ -297,7 +296,7 @@ attention_q4_kernel(const QaParams p) {
     uint2* const q_smem = reinterpret_cast<uint2*>(qa_smem + T::RING + T::merge(NT));         // [HD / 16][NT][lane], several row tiles
     float* const f_smem = reinterpret_cast<float*>(q_smem + HD / 16 * NT * 32);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t* const ring = qa_smem + warp * (QA_STAGES * QA_KT * T::BYTES);
+    uint8_t* const ring = qa_smem + warp * (QA_STAGES * T::BYTES);
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
     pdl_launch_dependents();
 
@@ -314,61 +313,39 @@ attention_q4_kernel(const QaParams p) {
     const uint32_t f1 = f + min(plan.per, plan.total - f), per = plan.per;
     const QaMagic magic;
 
-    // ---- copies: piece i of a chunk (of QA_KT * PIECES) is lane i % 32's
+    // ---- copies: piece i of a tile is lane i % 32's
     const int ps = p.kv.page_size;
     const uint8_t* head_src;                                       // the pair's record in page 0
     const int32_t* table;
     int tile0, tile1, last_page;
-    constexpr int TURN = QA_WARPS * QA_KT;                         // tiles between two chunks of a warp
-    struct Pages { int e[QA_KT]; };
-    auto pages = [&](int first) {                                 // table entries of the first positions of the tiles of the chunk at `first`
-        Pages x;
-#pragma unroll
-        for (int i = 0; i < QA_KT; ++i) x.e[i] = first + i < tile1 ? table[WHOLE ? first + i : (first + i) * 16 / ps] : 0;
-        return x;
-    };
-    auto request = [&](int first, const Pages& x, int stage) {
-        const int n = min(QA_KT, tile1 - first);
-        if (n > 0) {
-            const uint32_t dst = ring_addr + stage * (QA_KT * T::BYTES) + lane * 16;
-            const int pieces = n * T::PIECES;
+    auto entry_of = [&](int tile) { return tile < tile1 ? table[WHOLE ? tile : tile * 16 / ps] : 0; };     // of its first position
+    auto request = [&](int tile, int entry, int stage) {
+        if (tile < tile1) {
+            const uint32_t dst = ring_addr + stage * T::BYTES + lane * 16;
             if constexpr (WHOLE) {
-                const uint8_t* src[QA_KT];
+                const uint8_t* const src = head_src + (long long)entry * p.kv.page_stride + lane * 16;
 #pragma unroll
-                for (int i = 0; i < QA_KT; ++i) src[i] = head_src + (long long)x.e[i] * p.kv.page_stride + lane * 16 - i * T::BYTES;
-                auto copy = [&](int k) {
-                    const uint8_t* from = src[0];
-#pragma unroll
-                    for (int i = 1; i < QA_KT; ++i) if (32 * k + lane >= i * T::PIECES) from = src[i];
-                    qa_copy16(dst + k * 512, from + k * 512);
-                };
-                if (n == QA_KT && QA_KT * T::PIECES % 32 == 0) {
-#pragma unroll
-                    for (int k = 0; k < T::LANE_PIECES; ++k) copy(k);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < T::LANE_PIECES; ++k) if (32 * k + lane < pieces) copy(k);
-                }
+                for (int k = 0; k < T::LANE_PIECES; ++k) if (32 * k + lane < T::PIECES) qa_copy16(dst + k * 512, src + k * 512);
             } else {
                 // a tile's four parts lie apart, and with pages that are no multiple of 16 positions its keys do too
                 const bool together = ps % 16 == 0;
 #pragma unroll
                 for (int k = 0; k < T::LANE_PIECES; ++k) {
-                    const int i = 32 * k + lane, tile = i / T::PIECES, in_tile = i % T::PIECES * 16;      // (bytes)
-                    if (i >= pieces) continue;
+                    const int i = 32 * k + lane, in_tile = i * 16;                     // (bytes)
+                    if (i >= T::PIECES) continue;
                     const int half = in_tile / (T::KC + T::KS), in_half = in_tile % (T::KC + T::KS), steps = in_half >= T::KC;
                     const int in_part = in_half - (steps ? T::KC : 0), row = steps ? HD / 16 : HD / 2;
-                    const int key = in_part / row, pos = (first + tile) * 16 + key;
+                    const int key = in_part / row, pos = tile * 16 + key;
                     const int lp = min(pos / ps, last_page), in_page = pos % ps;      // (past the last page: some row of it, hidden later)
-                    const int entry = !together ? table[lp] : tile == 0 ? x.e[0] : x.e[1];
                     const int part = half ? (steps ? p.kv.v_steps : p.kv.v_codes) : (steps ? p.kv.k_steps : 0);
-                    qa_copy16(dst + k * 512, head_src + (long long)p.kv.page(entry) * p.kv.page_stride + part + in_page * row + in_part % row);
+                    qa_copy16(dst + k * 512, head_src + (long long)p.kv.page(together ? entry : table[lp]) * p.kv.page_stride + part +
+                                                 in_page * row + in_part % row);
                 }
             }
         }
         qa_copy_commit();
     };
-    Pages next;
+    int next;                                                      // the table entry of the tile to be asked for next
     QaItem it(p, item, R);
     int off = 0;
     uint32_t pair_weight = plan.weight(it.tiles);                  // (not zero: the plan gives an item that has tiles)
@@ -405,10 +382,10 @@ attention_q4_kernel(const QaParams p) {
         head_src = p.pool + p.kv.entry_offset + (long long)kvh * p.kv.record;
         table = p.kv.block_table + (long long)it.slot * p.kv.table_stride;
         last_page = (it.kv_hi - 1) / ps;
-        Pages x[QA_STAGES];
+        int entry[QA_STAGES];
 #pragma unroll
-        for (int j = 0; j < QA_STAGES; ++j) x[j] = pages(tile0 + warp * QA_KT + j * TURN);
-        next = pages(tile0 + warp * QA_KT + QA_STAGES * TURN);
+        for (int j = 0; j < QA_STAGES; ++j) entry[j] = entry_of(tile0 + warp + j * QA_WARPS);
+        next = entry_of(tile0 + warp + QA_STAGES * QA_WARPS);
         if (decltype(first_of_all)::value) pdl_wait();             // keys and queries may be the work of the kernel before
         const int r = NT == 1 ? g : 8 * warp + g, row = it.row0 + r;
         const bool mine = NT == 1 || warp < NT, live = mine && r < it.rows;
@@ -424,7 +401,7 @@ attention_q4_kernel(const QaParams p) {
             for (int w = 0; w < HD / 32; ++w) raw[w] = make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int j = 0; j < QA_STAGES; ++j) request(tile0 + warp * QA_KT + j * TURN, x[j], j);
+        for (int j = 0; j < QA_STAGES; ++j) request(tile0 + warp + j * QA_WARPS, entry[j], j);
         if constexpr (NT == 1) {
             const float scale = qa_query<HD>(qf, raw, p.scale_log2);
             factor[0][0] = __shfl_sync(0xffffffffu, scale, 8 * t);
@@ -609,24 +586,22 @@ attention_q4_kernel(const QaParams p) {
             }
         }
     };
-    // Chunks that every row sees whole go through a loop of their own: joined with the masked code behind one
+    // Tiles that every row sees whole go through a loop of their own: joined with the masked code behind one
     // branch, the compiler moved the accumulators from register to register every tile.
-    for (int at = tile0 + warp * QA_KT, stage = 0;;) {
-        auto take = [&](auto edge, int n_tiles) {
+    for (int tile = tile0 + warp, stage = 0;;) {
+        auto take = [&](auto edge) {
             qa_copy_wait<QA_STAGES - 1>();
             __syncwarp();                                          // every lane's pieces are there
-#pragma unroll 1
-            for (int i = 0; i < n_tiles; ++i) fold(edge, (at + i) * 16, ring + (stage * QA_KT + i) * T::BYTES);
+            fold(edge, tile * 16, ring + stage * T::BYTES);
             __syncwarp();                                          // every lane is done with the stage
-            request(at + QA_STAGES * TURN, next, stage);
-            next = pages(at + (QA_STAGES + 1) * TURN);
-            at += TURN;
+            request(tile + QA_STAGES * QA_WARPS, next, stage);
+            next = entry_of(tile + (QA_STAGES + 1) * QA_WARPS);
+            tile += QA_WARPS;
             if (++stage == QA_STAGES) stage = 0;
         };
-        while (at >= clear0 && at + QA_KT <= clear1) take(std::false_type(), QA_KT);
-        const int n_tiles = min(QA_KT, tile1 - at);
-        if (n_tiles <= 0) break;
-        take(std::true_type(), n_tiles);
+        while (tile >= clear0 && tile < clear1) take(std::false_type());
+        if (tile >= tile1) break;
+        take(std::true_type());
     }
     qa_copy_wait<0>();
 
