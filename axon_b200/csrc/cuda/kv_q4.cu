@@ -221,43 +221,11 @@ __device__ __forceinline__ void q4_store8<__nv_bfloat16>(__nv_bfloat16* dst, uin
 }
 
 constexpr int Q4_READ_ROWS = 32, Q4_READ_THREADS = 256, Q4_READ_BATCH = 4;      // (threads: for one plane, or half for each of two)
-// `pad`: the rows from a span's end up to the next multiple of `pad` of its rows hold zeros.
+// Writes a CTA's rows r0 .. once `rec` (a row's record of kv head 0; -1: not written, -2: zeros) and `at` (its place in
+// the page) are known.
 template <typename T>
-__global__ void __launch_bounds__(Q4_READ_THREADS)
-kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* __restrict__ spans, int n_spans, int n_slots,
-                  long long n_rows, int rows_per_cta, int pad, Q4Out out) {
-    __shared__ long long rec[Q4_READ_ROWS];                    // the row's record of kv head 0; -1: not written, -2: zeros
-    __shared__ int at[Q4_READ_ROWS];                           // its place in the page
-    __shared__ int owner[Q4_READ_ROWS];                        // the first span that covers it
-    if (threadIdx.x < Q4_READ_ROWS) owner[threadIdx.x] = n_spans;
-    pdl_launch_dependents();
-    pdl_wait();
-    const long long r0 = (long long)blockIdx.x * rows_per_cta, r1 = min(r0 + rows_per_cta, n_rows);
-    __syncthreads();
-    for (int s = threadIdx.x; s < n_spans; s += Q4_READ_THREADS) {
-        const long long out0 = spans[3 * n_spans + s], count = max(spans[2 * n_spans + s], 0);
-        const long long a = max(out0, r0), b = min(out0 + (count + pad - 1) / pad * pad, r1);
-        for (long long r = a; r < b; ++r) atomicMin(&owner[r - r0], s);
-    }
-    __syncthreads();
-    if (threadIdx.x < rows_per_cta) {
-        const int s = owner[threadIdx.x];
-        long long where = -1;
-        int in_page = 0;
-        if (s < n_spans) {
-            const long long i = r0 + threadIdx.x - spans[3 * n_spans + s];
-            const int slot = spans[s];
-            const long long pos = spans[n_spans + s] + i, lp = pos / kv.page_size;
-            if (i >= spans[2 * n_spans + s]) where = -2;
-            else if (slot >= 0 && slot < n_slots && pos >= 0 && lp < kv.table_stride) {
-                where = kv.record_at(slot, (int)lp, 0);
-                in_page = (int)(pos - lp * kv.page_size);
-            }
-        }
-        rec[threadIdx.x] = where;
-        at[threadIdx.x] = in_page;
-    }
-    __syncthreads();
+__device__ __forceinline__ void q4_read_rows(const uint8_t* __restrict__ pool, const PagedQ4& kv, const long long* rec, const int* at,
+                                             long long r0, int rows_per_cta, const Q4Out& out) {
     // with both planes to write the first half of the threads takes keys, the second values
     const bool both = out.k != nullptr && out.v != nullptr, is_v = both ? threadIdx.x >= Q4_READ_THREADS / 2 : out.v != nullptr;
     const int threads = both ? Q4_READ_THREADS / 2 : Q4_READ_THREADS, tid = both ? threadIdx.x % (Q4_READ_THREADS / 2) : threadIdx.x;
@@ -309,6 +277,107 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* _
             for (; h < kv.kv_heads; ++h) batch(std::integral_constant<int, 1>());
         }
     }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(Q4_READ_THREADS)
+kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* __restrict__ spans, int n_spans, int n_slots,
+                  long long n_rows, int rows_per_cta, Q4Out out) {
+    __shared__ long long rec[Q4_READ_ROWS];
+    __shared__ int at[Q4_READ_ROWS];
+    __shared__ int owner[Q4_READ_ROWS];                        // the first span that covers it
+    if (threadIdx.x < Q4_READ_ROWS) owner[threadIdx.x] = n_spans;
+    pdl_launch_dependents();
+    pdl_wait();
+    const long long r0 = (long long)blockIdx.x * rows_per_cta, r1 = min(r0 + rows_per_cta, n_rows);
+    __syncthreads();
+    for (int s = threadIdx.x; s < n_spans; s += Q4_READ_THREADS) {
+        const long long out0 = spans[3 * n_spans + s], count = max(spans[2 * n_spans + s], 0);
+        const long long a = max(out0, r0), b = min(out0 + count, r1);
+        for (long long r = a; r < b; ++r) atomicMin(&owner[r - r0], s);
+    }
+    __syncthreads();
+    if (threadIdx.x < rows_per_cta) {
+        const int s = owner[threadIdx.x];
+        long long where = -1;
+        int in_page = 0;
+        if (s < n_spans) {
+            const long long i = r0 + threadIdx.x - spans[3 * n_spans + s];
+            const int slot = spans[s];
+            const long long pos = spans[n_spans + s] + i, lp = pos / kv.page_size;
+            if (slot >= 0 && slot < n_slots && pos >= 0 && lp < kv.table_stride) {
+                where = kv.record_at(slot, (int)lp, 0);
+                in_page = (int)(pos - lp * kv.page_size);
+            }
+        }
+        rec[threadIdx.x] = where;
+        at[threadIdx.x] = in_page;
+    }
+    __syncthreads();
+    q4_read_rows<T>(pool, kv, rec, at, r0, rows_per_cta, out);
+}
+
+// Keys and values of whole prompts for the attention that takes bfloat16 pages: of each of the n_long segments named in `which`
+// the positions that its rows see, from a multiple of 64 on, one segment after another in pages of 64 positions
+// (two CTAs a page; rows behind a segment's last position are zeros).  The CTA at a segment's first page also writes what
+// that attention needs to find them: the segment counted from its first position here (`seg_out` [4][n_long]) and its row of
+// `table` [n_long][stride].  What `pages` and `stride` do not hold is left out (the host sizes both from the same lengths).
+template <typename T>
+__global__ void __launch_bounds__(Q4_READ_THREADS)
+kv_read_q4_pages_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* __restrict__ segments, int n_segments,
+                        const int32_t* __restrict__ which, int n_long, int window, int pages, int stride, int32_t* __restrict__ seg_out,
+                        int32_t* __restrict__ table, Q4Out out) {
+    __shared__ long long rec[Q4_READ_ROWS];
+    __shared__ int at[Q4_READ_ROWS];
+    __shared__ int who, first_page, lo, count;
+    pdl_launch_dependents();
+    const int page = blockIdx.x / 2;
+    if (threadIdx.x == 0) who = -1;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int base = 0;
+        for (int i0 = 0; i0 < n_long; i0 += 32) {
+            const int i = i0 + threadIdx.x;
+            int from = 0, keys = 0, n = 0;
+            if (i < n_long) {
+                const int q_len = segments[2 * n_segments + which[i]], kv_len = segments[3 * n_segments + which[i]];
+                from = window > 0 ? max(kv_len - q_len - window + 1, 0) / 64 * 64 : 0;
+                keys = kv_len - from;
+                n = min((keys + 63) / 64, stride);
+            }
+            int upto = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, d);
+                if ((int)threadIdx.x >= d) upto += x;
+            }
+            if (page >= base + upto - n && page < base + upto) { who = i; first_page = base + upto - n; lo = from; count = min(keys, n * 64); }
+            base += __shfl_sync(0xffffffffu, upto, 31);
+            if (base > page) break;
+        }
+    }
+    pdl_wait();
+    __syncthreads();
+    if (who < 0) return;
+    const int seg = which[who], slot = segments[seg];
+    if (page == first_page && blockIdx.x % 2 == 0) {
+        if (threadIdx.x == 0) {
+            seg_out[who] = who;
+            seg_out[n_long + who] = segments[n_segments + seg];
+            seg_out[2 * n_long + who] = segments[2 * n_segments + seg];
+            seg_out[3 * n_long + who] = count;
+        }
+        for (int j = threadIdx.x; j < stride; j += Q4_READ_THREADS) table[(long long)who * stride + j] = min(first_page + j, pages - 1);
+    }
+    const long long r0 = (long long)page * 64 + blockIdx.x % 2 * Q4_READ_ROWS;
+    if (threadIdx.x < Q4_READ_ROWS) {
+        const int i = (int)(r0 - (long long)first_page * 64) + threadIdx.x, pos = lo + i, lp = pos / kv.page_size;
+        const bool held = i < count && lp < kv.table_stride;
+        rec[threadIdx.x] = held ? kv.record_at(slot, lp, 0) : -2;
+        at[threadIdx.x] = held ? pos - lp * kv.page_size : 0;
+    }
+    __syncthreads();
+    q4_read_rows<T>(pool, kv, rec, at, r0, Q4_READ_ROWS, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -559,15 +628,15 @@ AXON_API int axon_rope_kv_write_q4(const float* qkv, const float* table, const i
 }
 
 static int kv_read_launch(const void* pool, const PagedQ4& kv, const int32_t* spans, int n_spans, int n_slots, int dtype, long long n_rows,
-                          int pad, const Q4Out& out, cudaStream_t stream) {
+                          const Q4Out& out, cudaStream_t stream) {
     int rows = Q4_READ_ROWS;
     while (rows > 1 && (n_rows + rows - 1) / rows < 2 * 148) rows /= 2;      // few rows: more CTAs rather than longer ones
     const long long ctas = (n_rows + rows - 1) / rows;
     if (ctas > 0x7fffffffLL) { set_error("axon_kv_read_q4: %lld rows are too many", n_rows); return AXON_BAD_ARGUMENT; }
     if (dtype == AXON_Q4_F32)
-        launch_pdl(kv_read_q4_kernel<float>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, pad, out);
+        launch_pdl(kv_read_q4_kernel<float>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, out);
     else if (dtype == AXON_Q4_BF16)
-        launch_pdl(kv_read_q4_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, pad, out);
+        launch_pdl(kv_read_q4_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, spans, n_spans, n_slots, n_rows, rows, out);
     else { set_error("axon_kv_read_q4: unknown dtype %d", dtype); return AXON_BAD_ARGUMENT; }
     return launch_status("axon_kv_read_q4");
 }
@@ -588,54 +657,26 @@ AXON_API int axon_kv_read_q4(const void* pool, const AxonKvLayout* layout, const
         void* const v = apart && !part ? nullptr : values;
         const long long width = k != nullptr ? kv.hd : kv.vd;
         const Q4Out out{k, v, kv.kv_heads * width, 0, width, 0};
-        if (int st = kv_read_launch(pool, kv, spans, n_spans, n_slots, dtype, n_rows, 1, out, stream)) return st;
+        if (int st = kv_read_launch(pool, kv, spans, n_spans, n_slots, dtype, n_rows, out, stream)) return st;
     }
     return AXON_OK;
 }
 
-// Tables for a prompt's attention over read-back keys.  For each of the n_long segments named in `which`: a span (see
-// axon_kv_read_q4) of the positions that its rows see, from a multiple of 64 on; its place in a pool of pages of 64
-// positions, one after another; and its segment as the attention kernels take it, counted from the span's first
-// position, with row i of `table` [n_long][stride] as its block table.  What `pages` or `stride` do not hold is left out (the
-// host sizes both from the same lengths).
-__global__ void q4_prompt_plan_kernel(const int32_t* __restrict__ segments, int n_segments, const int32_t* __restrict__ which, int n_long,
-                                      int window, int pages, int stride, int32_t* __restrict__ spans, int32_t* __restrict__ seg_out,
-                                      int32_t* __restrict__ table) {
-    pdl_launch_dependents();
-    pdl_wait();
-    int base = 0;
-    for (int i = 0; i < n_long; ++i) {
-        const int s = which[i], q_len = segments[2 * n_segments + s], kv_len = segments[3 * n_segments + s];
-        const int lo = window > 0 ? max(kv_len - q_len - window + 1, 0) / 64 * 64 : 0;
-        const int n = min(min((kv_len - lo + 63) / 64, stride), pages - base);
-        if (threadIdx.x == 0) {
-            spans[i] = segments[s]; spans[n_long + i] = lo; spans[2 * n_long + i] = min(kv_len - lo, n * 64); spans[3 * n_long + i] = base * 64;
-            seg_out[i] = i; seg_out[n_long + i] = segments[n_segments + s]; seg_out[2 * n_long + i] = q_len; seg_out[3 * n_long + i] = min(kv_len - lo, n * 64);
-        }
-        for (int j = threadIdx.x; j < stride; j += blockDim.x) table[(long long)i * stride + j] = min(base + j, pages - 1);
-        base += n;
-    }
-}
-AXON_API int axon_q4_prompt_plan(const int32_t* segments, int n_segments, const int32_t* which, int n_long, int window, int pages, int stride,
-                                 int32_t* spans, int32_t* seg_out, int32_t* table, cudaStream_t stream) {
+// See kv_read_q4_pages_kernel.  pages_out: bfloat16 [pages][2][kv_heads][64][head_dim].
+AXON_API int axon_kv_read_q4_pages(const void* pool, const AxonKvLayout* layout, const int32_t* segments, int n_segments, const int32_t* which,
+                                   int n_long, int window, int pages, int stride, int32_t* seg_out, int32_t* table, void* pages_out,
+                                   cudaStream_t stream) {
     if (n_long <= 0) return AXON_OK;
-    if (pages < 1 || stride < 1) { set_error("axon_q4_prompt_plan: no room (%d pages, %d per request)", pages, stride); return AXON_BAD_ARGUMENT; }
-    launch_pdl(q4_prompt_plan_kernel, dim3(1), dim3(256), 0, stream, segments, n_segments, which, n_long, window, pages, stride, spans, seg_out, table);
-    return launch_status("axon_q4_prompt_plan");
-}
-
-// The positions of the plan's spans into its pool of pages [pages][2][kv_heads][64][head_dim]; rows behind a span's end in
-// its last page are zeros.
-AXON_API int axon_kv_read_q4_pages(const void* pool, const AxonKvLayout* layout, const int32_t* spans, int n_spans, int n_slots,
-                                   void* pages_out, int dtype, int pages, cudaStream_t stream) {
-    if (pages <= 0 || n_spans <= 0) return AXON_OK;
     PagedQ4 kv;
     if (int st = to_q4(layout, pool, "axon_kv_read_q4_pages", &kv)) return st;
     if (kv.planes != 2 || kv.vd != kv.hd) { set_error("axon_kv_read_q4_pages: takes caches with key and value planes of one width"); return AXON_BAD_ARGUMENT; }
+    if (pages < 1 || stride < 1 || pages > (1 << 29)) { set_error("axon_kv_read_q4_pages: no room (%d pages, %d per request)", pages, stride); return AXON_BAD_ARGUMENT; }
     if ((uintptr_t)pages_out & 15) { set_error("axon_kv_read_q4_pages: outputs must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
     const long long plane = (long long)kv.kv_heads * 64 * kv.hd;
-    const Q4Out out{pages_out, (uint8_t*)pages_out + plane * (dtype == AXON_Q4_F32 ? 4 : 2), 2 * plane, kv.hd, 64ll * kv.hd, 6};
-    return kv_read_launch(pool, kv, spans, n_spans, n_slots, dtype, 64ll * pages, 64, out, stream);
+    const Q4Out out{pages_out, (uint8_t*)pages_out + plane * 2, 2 * plane, kv.hd, 64ll * kv.hd, 6};
+    launch_pdl(kv_read_q4_pages_kernel<__nv_bfloat16>, dim3(2 * pages), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, segments,
+               n_segments, which, n_long, window, pages, stride, seg_out, table, out);
+    return launch_status("axon_kv_read_q4_pages");
 }
 
 // Floats of scratch that axon_attention_q4_plain needs for its key shares (0 for one share).

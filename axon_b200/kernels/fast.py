@@ -483,10 +483,11 @@ def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: 
                 n, kv_len = ctx.seg_q_len[s], ctx.seg_kv_len[s]
                 work += [(kv_len - n + min(n, -(-(r + 8 * nt) // group)), s, r) for r in range(0, n * group, 8 * nt)]
             flat = [x for _, s, r in sorted(work, reverse=True) for x in (s, r)]     # the longest must not start last
-            n_items, which = len(work), ctx.rt.upload_i32(f"q4_items_{group}_{hd}_{nt}", flat).data_ptr()
+            n_items, which = len(work), ctx.rt.upload_i32(f"q4_items_{group}_{hd}_{nt}", flat)
         ctas = lib.cuda().axon_attention_q4_ctas(hd, nt)
         floats = 2 * ctas * 8 * nt * (hd + 2) + ctas
-        launches.append((nt, n_items, which, ctx.rt.zeroed_buffer(f"q4_scratch_{hd}_{nt}", (floats,), torch.float32).data_ptr(), floats))
+        scratch = ctx.rt.zeroed_buffer(f"q4_scratch_{hd}_{nt}", (floats,), torch.float32)
+        launches.append((nt, n_items, which, scratch.data_ptr(), floats, scratch))
     groups, at, room = [], [], 0
     for s in sorted(long):
         if at and room + ctx.seg_kv_len[s] > Q4_PROMPT_POSITIONS:
@@ -506,17 +507,14 @@ def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: 
         flat = list(segs) + [x for _, i, t0 in sorted(work, reverse=True) for x in (i, t0)]
         lists = ctx.rt.upload_i32(f"q4_prompt_{group}_{rows}", flat)
         n = len(segs)
-        ints = ctx.rt.buffer(f"q4_plan_{window}_{k}", (max(8 * n + n * stride, ctx.rt.kv_prompt_entries),), torch.int32)
-        ints = ints[:8 * n + n * stride]
-        check(lib.cuda().axon_q4_prompt_plan(ctx.segments.data_ptr(), n_seg, lists.data_ptr(), n, window, pages, stride, ints.data_ptr(),
-                                             ints[4 * n:].data_ptr(), ints[8 * n:].data_ptr(), _stream()))
+        ints = ctx.rt.buffer(f"q4_plan_{window}_{k}", (max(4 * n + n * stride, ctx.rt.kv_prompt_entries),), torch.int32)
         room = max(pages, ctx.rt.kv_prompt_pages)
         pool = ctx.rt.buffer(f"q4_prompt_pages_{kv_heads}_{hd}", (room, 2, kv_heads, 64, hd), torch.bfloat16)
-        layout = lib.KvLayout(block_table=ints[8 * n:].data_ptr(), table_stride=stride, page_size=64, kv_heads=kv_heads, head_dim=hd,
+        layout = lib.KvLayout(block_table=ints[4 * n:].data_ptr(), table_stride=stride, page_size=64, kv_heads=kv_heads, head_dim=hd,
                               page_stride=2 * kv_heads * 64 * hd, entry_offset=0, v_offset=kv_heads * 64 * hd, v_dim=hd, planes=2,
                               n_pages=room - 1, bits=0, fault=None)
-        plans.append((n, pages, rows, tpt, lists[n:].data_ptr(), len(work), ints.data_ptr(), ints[4 * n:].data_ptr(), pool.data_ptr(),
-                      ctypes.byref(layout)))
+        plans.append((n, pages, stride, rows, tpt, lists.data_ptr(), lists[n:].data_ptr(), len(work), ints.data_ptr(), ints[4 * n:].data_ptr(),
+                      pool.data_ptr(), ctypes.byref(layout), (lists, ints, pool)))
     got = (launches, plans)
     ctx.scratch[key] = got
     return got
@@ -548,12 +546,13 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
         return False
     launches, plans = _q4_work(ctx, group, kv.kv_heads, hd, kv.window, takes_short)
     cu = lib.cuda()
-    for nt, n_items, which, scratch, floats in launches:
+    for nt, n_items, which, scratch, floats, _held in launches:
         check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
-                                   which, n_items, kv._ref, heads, float(scale), int(kv.window),
+                                   None if which is None else which.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
                                    nt, scratch, floats, _stream()))
-    for n, pages, rows, tpt, tiles, n_tiles, spans, segments, pool, layout in plans:
-        check(cu.axon_kv_read_q4_pages(kv.pool.data_ptr(), kv._ref, spans, n, kv.block_table.shape[0], pool, 1, pages, _stream()))
+    for n, pages, stride, rows, tpt, which, tiles, n_tiles, segments, table, pool, layout, _held in plans:
+        check(cu.axon_kv_read_q4_pages(kv.pool.data_ptr(), kv._ref, ctx.segments.data_ptr(), len(ctx.seg_q_len), which, n, int(kv.window),
+                                       pages, stride, segments, table, pool, _stream()))
         if rows == 256:
             check(cu.axon_attention_tc(q.data_ptr(), pool, out.data_ptr(), segments, n, tiles, n_tiles, layout, heads, float(scale),
                                        int(kv.window), tpt, _stream()))
