@@ -731,6 +731,7 @@ static int attention_fa_launch(const void* q, const void* pool, void* out, const
                                float scale, int window, int decode, int tokens_per_tile, int n_splits,
                                float* scratch, unsigned int* counters, const FusedQkv& fused, cudaStream_t stream) {
     if (n_items <= 0) return AXON_OK;
+    if (layout->bits) { set_error("axon_attention_fa: takes a cache of whole elements, not of %d bits", layout->bits); return AXON_BAD_ARGUMENT; }
     const int hd = layout->head_dim, kvh = layout->kv_heads;
     if (heads % kvh) { set_error("axon_attention_fa: %d heads over %d kv heads", heads, kvh); return AXON_BAD_ARGUMENT; }
     const int group = heads / kvh, bm = decode ? 16 : 64;

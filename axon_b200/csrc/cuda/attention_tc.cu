@@ -443,6 +443,7 @@ AXON_API int axon_attention_tc(const void* q, const void* pool, void* out, const
                                const int32_t* items, int n_items, const AxonKvLayout* layout, int heads, float scale,
                                int window, int tokens_per_tile, cudaStream_t stream) {
     if (n_items <= 0) return AXON_OK;
+    if (layout->bits) { set_error("axon_attention_tc: takes a cache of whole elements, not of %d bits", layout->bits); return AXON_BAD_ARGUMENT; }
     const int kvh = layout->kv_heads;
     if (layout->head_dim != AT_HD) { set_error("axon_attention_tc: head size %d is not 128", layout->head_dim); return AXON_BAD_ARGUMENT; }
     if (heads % kvh) { set_error("axon_attention_tc: %d heads over %d kv heads", heads, kvh); return AXON_BAD_ARGUMENT; }

@@ -557,6 +557,7 @@ AXON_API int axon_rope_kv_write(const float* qkv, const float* table, const int3
     // (see axon_gemm_tc_small); they are folded here and `qkv` itself is not read
     if (n <= 0) return AXON_OK;
     if (partial != nullptr && (splits < 1 || ntok < n)) { set_error("axon_rope_kv_write: bad partial sums (splits %d, tokens %d of %d)", splits, n, ntok); return AXON_BAD_ARGUMENT; }
+    if (layout->bits) { set_error("axon_rope_kv_write: takes a cache of whole elements, not of %d bits", layout->bits); return AXON_BAD_ARGUMENT; }
     const SplitFold fold{partial, partial ? bias : nullptr, splits, ntok};
     const int hd = layout->head_dim;
     if (hd % 2 || rot % 2 || rot > hd || rot < 0) { set_error("axon_rope_kv_write: head size %d / rotated size %d must be even and rot <= head", hd, rot); return AXON_BAD_ARGUMENT; }
@@ -589,6 +590,7 @@ AXON_API int axon_attention_plain(const void* q, const void* pool, int dtype, co
                                   const int32_t* token_slot, void* out, const AxonKvLayout* layout,
                                   int n, int heads, float scale, int window, cudaStream_t stream) {
     if (n <= 0) return AXON_OK;
+    if (layout->bits) { set_error("axon_attention_plain: takes a cache of whole elements, not of %d bits", layout->bits); return AXON_BAD_ARGUMENT; }
     const int hd = layout->head_dim;
     if (hd > 256 || hd < 1) { set_error("axon_attention_plain: head size %d is not in 1..256", hd); return AXON_BAD_ARGUMENT; }
     if (layout->v_dim > 256) { set_error("axon_attention_plain: value rows of %d elements exceed 256", layout->v_dim); return AXON_BAD_ARGUMENT; }

@@ -240,6 +240,26 @@ def test_refusals(ops):
         ops.attention_plain(torch.zeros(4, 3 * 64, device=DEV), cache.view, pos, pos, torch.zeros(4, 3 * 64, device=DEV), 3, 0.1)
 
 
+def test_other_launchers_refuse_quantised_pools(ops):
+    """The kernels of caches in whole elements look at the layout, whoever calls them."""
+    from axon_b200.kernels import lib
+    cache = Cache(ops, [20], 2, 64, 16)
+    x, one = torch.zeros(1, 4 * 64, dtype=torch.bfloat16, device=DEV), i32([0, 0, 1, 1])
+    calls = {
+        "axon_rope_kv_write": (torch.zeros(1, 8 * 64, device=DEV).data_ptr(), None, one.data_ptr(), one.data_ptr(), x.data_ptr(),
+                               cache.pool.data_ptr(), 1, cache.view._ref, 1, 4, 0, 0, 1, None, 0, 0, None, lib.current_stream()),
+        "axon_attention_plain": (x.data_ptr(), cache.pool.data_ptr(), 1, one.data_ptr(), one.data_ptr(), x.data_ptr(), cache.view._ref, 1, 4,
+                                 0.1, 0, lib.current_stream()),
+        "axon_attention_fa": (x.data_ptr(), cache.pool.data_ptr(), x.data_ptr(), one.data_ptr(), 1, None, 1, cache.view._ref, 4, 0.1, 0, 1, 1, 1,
+                              None, None, lib.current_stream()),
+        "axon_attention_tc": (x.data_ptr(), cache.pool.data_ptr(), x.data_ptr(), one.data_ptr(), 1, one.data_ptr(), 1, cache.view._ref, 4, 0.1, 0,
+                              1, lib.current_stream()),
+    }
+    for name, args in calls.items():
+        with pytest.raises(lib.KernelError, match="4 bits"):
+            lib.check(getattr(lib.cuda(), name)(*args))
+
+
 # -- attention --------------------------------------------------------------
 
 def attend(ops, cache, q_lens, heads, dtype, window=0, seed=9, scale=None, rt=None, precise=None, q=None):
