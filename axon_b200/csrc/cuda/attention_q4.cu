@@ -215,48 +215,74 @@ struct QaItem {
 // How all pairs, laid end to end (items in order, the kv heads of each in order), fall to the CTAs: a range
 // of `per` places each.  Where the pairs cut into pieces of equal length that start at their beginnings make no more
 // pieces than there are CTAs, a pair's tiles are padded to whole ranges, so that no CTA has two pieces; else pairs follow one
-// another without gaps but for `cost` places before each.  Every warp works it out for itself, 32 items at a
-// time.  (The launcher has seen to it that full block tables count in 32 bits.)
-struct QaPlan {
+// another without gaps but for `cost` places before each.  Everything counts in 32 bits: the launcher has seen to it that
+// tiles + QA_PAIR_COST * pairs stay below 2^31, there are no more pieces than that, and a padded division, taken for
+// no more pieces than CTAs only, has ctas * per places at most, which is within ctas * (QA_LEAST + the shortest range) of the tiles.
+struct QaDivision {
     uint32_t total, per, cost;
     bool padded;
-    // what a pair of `tiles` takes: its cost, then its tiles
-    __device__ __forceinline__ uint32_t weight(uint32_t tiles) const {
-        return tiles == 0 ? 0 : padded ? (tiles + per - 1) / per * per : tiles + cost;
-    }
-    __device__ __forceinline__ uint32_t sum(const QaParams& p, int most_rows, uint32_t mine) const {
-        const int lane = threadIdx.x & 31;
-        uint32_t x = weight(mine);                                 // (the first 32 items' tiles are in registers)
-        for (int i = lane + 32; i < p.n_items; i += 32) x += weight(QaItem(p, i, most_rows).tiles);
-        return __reduce_add_sync(0xffffffffu, x) * p.kv.kv_heads;
-    }
-    // `item`: the one that this CTA's range begins in, `start`: where its first pair begins
-    __device__ __forceinline__ QaPlan(const QaParams& p, int most_rows, int* item, uint32_t* start) {
-        const int lane = threadIdx.x & 31;
-        const uint32_t mine = lane < p.n_items ? QaItem(p, lane, most_rows).tiles : 0;
-        uint32_t tiles = mine, longest = mine;
-        for (int i = lane + 32; i < p.n_items; i += 32) {
-            const uint32_t n = QaItem(p, i, most_rows).tiles;
-            tiles += n;
-            longest = max(longest, n);
-        }
-        tiles = __reduce_add_sync(0xffffffffu, tiles) * p.kv.kv_heads;
-        longest = __reduce_max_sync(0xffffffffu, longest);
+    // the length of ranges that pairs are padded to
+    __host__ __device__ __forceinline__ QaDivision(uint32_t tiles, uint32_t longest, uint32_t ctas) {
         // one CTA folds a pair's pieces (about 0.12 us each): with few long pairs, ranges as long as the fold of their
         // number, which is about the square root of a pair's tiles (one request of 32,768 positions: 16.2 us; with 1.5 times
         // as long ranges 17.7, twice 19.9, 0.7 times 15.9)
-        const uint32_t least = max((uint32_t)QA_LEAST, (uint32_t)sqrtf((float)longest));
-        const uint32_t even = (tiles + p.ctas - 1) / p.ctas;
+        least = (uint32_t)sqrtf((float)longest);
+        least = least > (uint32_t)QA_LEAST ? least : (uint32_t)QA_LEAST;
+        const uint32_t even = (tiles + ctas - 1) / ctas;
         padded = true;
         cost = 0;
-        per = (max(least, even) + QA_LEAST - 1) / QA_LEAST * QA_LEAST;
-        total = sum(p, most_rows, mine);
-        if (total > p.ctas * per) {
-            padded = false;
-            cost = QA_PAIR_COST;
-            total = sum(p, most_rows, mine);
-            per = max(least, (total + p.ctas - 1) / p.ctas);
+        total = 0;
+        per = ((least > even ? least : even) + QA_LEAST - 1) / QA_LEAST * QA_LEAST;
+    }
+    __host__ __device__ __forceinline__ uint32_t pieces(uint32_t tiles) const { return (tiles + per - 1) / per; }
+    // the choice, once the pieces of all pairs are counted
+    __host__ __device__ __forceinline__ void settle(uint32_t all_pieces, uint32_t tiles, uint32_t pairs, uint32_t ctas) {
+        if (all_pieces <= ctas) {
+            total = all_pieces * per;
+            return;
         }
+        padded = false;
+        cost = QA_PAIR_COST;
+        total = tiles + cost * pairs;
+        const uint32_t even = (total + ctas - 1) / ctas;
+        per = least > even ? least : even;
+    }
+    // what a pair of `tiles` takes: its cost, then its tiles
+    __host__ __device__ __forceinline__ uint32_t weight(uint32_t tiles) const {
+        return tiles == 0 ? 0 : padded ? pieces(tiles) * per : tiles + cost;
+    }
+private:
+    uint32_t least;
+};
+// Every warp works the division out for itself, 32 items at a time.
+struct QaPlan : QaDivision {
+    // `item`: the one that this CTA's range begins in, `start`: where its first pair begins
+    __device__ __forceinline__ QaPlan(const QaParams& p, int most_rows, int* item, uint32_t* start)
+        : QaPlan(p, most_rows, (int)(threadIdx.x & 31) < p.n_items ? QaItem(p, (int)(threadIdx.x & 31), most_rows).tiles : 0, item, start) {}
+private:
+    struct Sums { uint32_t tiles, longest, pairs; };
+    // (`mine`: the first 32 items' tiles stay in registers)
+    static __device__ __forceinline__ Sums sums(const QaParams& p, int most_rows, uint32_t mine) {
+        Sums s{mine, mine, mine != 0};
+        for (int i = (int)(threadIdx.x & 31) + 32; i < p.n_items; i += 32) {
+            const uint32_t n = QaItem(p, i, most_rows).tiles;
+            s.tiles += n;
+            s.longest = max(s.longest, n);
+            s.pairs += n != 0;
+        }
+        s.tiles = __reduce_add_sync(0xffffffffu, s.tiles) * p.kv.kv_heads;
+        s.longest = __reduce_max_sync(0xffffffffu, s.longest);
+        s.pairs = __reduce_add_sync(0xffffffffu, s.pairs) * p.kv.kv_heads;
+        return s;
+    }
+    __device__ __forceinline__ QaPlan(const QaParams& p, int most_rows, uint32_t mine, int* item, uint32_t* start)
+        : QaPlan(p, most_rows, mine, sums(p, most_rows, mine), item, start) {}
+    __device__ __forceinline__ QaPlan(const QaParams& p, int most_rows, uint32_t mine, const Sums& s, int* item, uint32_t* start)
+        : QaDivision(s.tiles, s.longest, p.ctas) {
+        const int lane = threadIdx.x & 31;
+        uint32_t n_pieces = pieces(mine);
+        for (int i = lane + 32; i < p.n_items; i += 32) n_pieces += pieces(QaItem(p, i, most_rows).tiles);
+        settle(__reduce_add_sync(0xffffffffu, n_pieces) * p.kv.kv_heads, s.tiles, s.pairs, p.ctas);
         // the item of this CTA's first place
         const uint32_t f = blockIdx.x * per;
         uint32_t base = 0;
@@ -725,6 +751,22 @@ using namespace axon;
 // How many CTAs an attention launch has (two fit an SM with one tile of 8 rows, up to head size 128).
 AXON_API int axon_attention_q4_ctas(int head_dim, int row_tiles) { return (row_tiles == 1 && head_dim <= 128 ? 2 : 1) * 148; }
 
+// How an attention launch of `ctas` CTAs divides items of these many 16-key tiles among them, worked out on the host by the
+// kernel's own arithmetic: out = {places in all, places of a CTA, places before each pair, 1 if pairs are padded to whole ranges}.
+AXON_API int axon_attention_q4_division(const int32_t* tiles, int n_items, int kv_heads, int ctas, uint32_t* out) {
+    uint32_t sum = 0, longest = 0, pairs = 0, n_pieces = 0;
+    for (int i = 0; i < n_items; ++i) {
+        sum += tiles[i];
+        longest = (uint32_t)tiles[i] > longest ? tiles[i] : longest;
+        pairs += tiles[i] != 0;
+    }
+    QaDivision d(sum * kv_heads, longest, ctas);
+    for (int i = 0; i < n_items; ++i) n_pieces += d.pieces(tiles[i]);
+    d.settle(n_pieces * kv_heads, sum * kv_heads, pairs * kv_heads, ctas);
+    out[0] = d.total; out[1] = d.per; out[2] = d.cost; out[3] = d.padded;
+    return AXON_OK;
+}
+
 // Attention of `n_items` tiles of up to 8 * row_tiles query rows (row_tiles 1, 2 or 4; at head size 256 1).  items null:
 // item i is segment i, whose rows all fit one tile.  scratch: 2 * ctas * 8 * row_tiles * (head_dim + 2) + ctas floats, zeroed once:
 // launches leave the last ctas of them zero.
@@ -738,7 +780,7 @@ AXON_API int axon_attention_q4(const void* q, const void* pool, void* out, const
     if (p.kv.planes != 2 || p.kv.vd != hd) { set_error("axon_attention_q4: takes caches with key and value planes of one width"); return AXON_BAD_ARGUMENT; }
     if (heads < 1 || heads % p.kv.kv_heads) { set_error("axon_attention_q4: %d heads over %d kv heads", heads, p.kv.kv_heads); return AXON_BAD_ARGUMENT; }
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)scratch) & 15) { set_error("axon_attention_q4: operands must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
-    if ((double)n_items * p.kv.kv_heads * ((double)p.kv.table_stride * p.kv.page_size / 16 + 1) > 2147483647.0) { set_error("axon_attention_q4: %d items of %d kv heads at up to %d pages are too many", n_items, p.kv.kv_heads, p.kv.table_stride); return AXON_BAD_ARGUMENT; }
+    if ((double)n_items * p.kv.kv_heads * ((double)p.kv.table_stride * p.kv.page_size / 16 + 1 + QA_PAIR_COST) > 2147483647.0) { set_error("axon_attention_q4: %d items of %d kv heads at up to %d pages are too many", n_items, p.kv.kv_heads, p.kv.table_stride); return AXON_BAD_ARGUMENT; }
     // a copy moves 16 bytes: at head size 64 the steps of four positions, which have to lie in one page
     if (p.kv.page_size % (hd >= 256 ? 1 : 256 / hd)) { set_error("axon_attention_q4: pages of %d positions of %d values do not fall into pieces it can copy", p.kv.page_size, hd); return AXON_BAD_ARGUMENT; }
     p.ctas = axon_attention_q4_ctas(hd, row_tiles);

@@ -60,6 +60,7 @@ _SIGNATURES = {
     "axon_attention_q4": [P, P, P, P, c_int, P, c_int, ctypes.POINTER(KvLayout), c_int, c_float, c_int, c_int, P,
                           c_longlong, P],
     "axon_attention_q4_ctas": [c_int, c_int],
+    "axon_attention_q4_division": [P, c_int, c_int, c_int, P],
     "axon_attention_q4_plain": [P, P, c_int, P, P, P, ctypes.POINTER(KvLayout), c_int, c_int, c_float, c_int, c_int, P,
                                 c_longlong, P, c_longlong, P],
     "axon_attention_plain": [P, P, c_int, P, P, P, ctypes.POINTER(KvLayout), c_int, c_int, c_float, c_int, P],

@@ -131,3 +131,57 @@ def test_views_of_quantised_pools_are_checked():
         ops.KvView(good, table.long(), 1, 16, 2, 64, bits=4)
     with pytest.raises(ValueError, match="multiple of 16"):
         ops.KvView(good, table, 1, 16, 2, 40, bits=4)
+
+
+def division(tiles, kv_heads, ctas):
+    """How an attention launch divides items of these many tiles: (places in all, of a CTA, before a pair, padded)."""
+    from axon_b200.kernels import lib
+    t, out = np.ascontiguousarray(tiles, np.int32), np.zeros(4, np.uint32)
+    lib.check(lib.cuda().axon_attention_q4_division(t.ctypes.data, len(t), kv_heads, ctas, out.ctypes.data))
+    return [int(x) for x in out]
+
+
+def check_division(tiles, kv_heads, ctas):
+    """Every pair's tiles lie in the ranges that the CTAs go through, worked out in unbounded integers."""
+    total, per, cost, padded = division(tiles, kv_heads, ctas)
+    tiles = np.asarray(tiles, np.int64)
+    weights = np.where(tiles == 0, 0, -(-tiles // per) * per if padded else tiles + cost)
+    assert total == int(weights.sum()) * kv_heads < 2 ** 32, "the places of all pairs were miscounted"
+    assert total <= ctas * per < 2 ** 32, "there are more places than the CTAs go through"
+    assert per >= 8 and (not padded or per % 8 == 0)
+    # a CTA has two pieces of others' pairs at most: where pairs follow one another, those that its range begins and ends in
+    if padded:
+        assert cost == 0 and int((-(-tiles // per)).sum()) * kv_heads <= ctas
+    return padded
+
+
+def test_work_is_divided_whole():
+    """The guard of the launcher lets through up to 2**31 tiles with what pairs cost; the division counts them all."""
+    rng = np.random.default_rng(8)
+    seen = set()
+    for k in range(400):
+        kv_heads, ctas = int(rng.choice([1, 2, 4, 8, 16])), int(rng.choice([148, 296]))
+        n = int(np.exp(rng.uniform(0, np.log(33000))))
+        most = 2 ** 31 // (n * kv_heads) - 25
+        longest = int(np.exp(rng.uniform(0, np.log(max(min(most, 2 ** 27), 2)))))
+        kind = k % 4
+        tiles = (np.full(n, longest) if kind == 0 else rng.integers(0, longest + 1, n) if kind == 1 else
+                 np.maximum(longest - np.arange(n) // 2, 1) if kind == 2 else np.where(rng.random(n) < 0.02, longest, rng.integers(0, 9, n)))
+        if tiles.sum() == 0:
+            continue
+        seen.add(check_division(tiles, kv_heads, ctas))
+    assert seen == {0, 1}
+    for n, kv_heads in ((1, 1), (148, 1), (149, 1), (33000, 8)):        # the largest that the launcher takes
+        check_division(np.full(n, 2 ** 31 // (n * kv_heads) - 25), kv_heads, 148)
+
+
+# heads, kv heads of 256, tokens, positions at the portion's end: pairs times the longest range pass 2**32 and wrap to a small number
+PORTIONS_THAT_WRAP = [(32, 8, 4096, 39936), (32, 8, 4096, 77824), (32, 8, 4096, 115712), (16, 8, 8192, 41984), (16, 16, 8192, 41984), (64, 8, 2048, 38912)]
+
+
+@pytest.mark.parametrize("heads,kv_heads,tokens,end", PORTIONS_THAT_WRAP)
+def test_portions_of_very_many_items_are_divided_whole(heads, kv_heads, tokens, end):
+    group = heads // kv_heads
+    rows = np.arange(0, tokens * group, 8)
+    tiles = (end - tokens + np.minimum(tokens, -(-(rows + 8) // group)) + 15) // 16
+    assert not check_division(tiles, kv_heads, 148)

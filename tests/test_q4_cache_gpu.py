@@ -720,3 +720,64 @@ def test_reading_what_a_request_holds(model_folders):
     assert held[0][0].shape == held[1][0].shape and held[1][0].dtype == torch.float32
     # of layer 0 the two engines quantise the same numbers; of layer 1 the keys have moved by what layer 0's rounding did
     assert float((held[0][0] - held[1][0]).abs().max()) < float(held[0][0].abs().max())
+
+
+# -- large portions ---------------------------------------------------------
+
+def random_pages(ops, positions, kv_heads, hd, seed, ps=16):
+    """One request of many positions whose pages hold random codes and steps of 0.125 to 0.47; the view, its keys and its values."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    n_pages, record = -(-positions // ps), q4.parts(ps, hd, hd, 2)[1]
+    pool = torch.randint(0, 256, (n_pages + 1, 1, kv_heads * record), dtype=torch.uint8, device=DEV, generator=g)
+    heads = pool.view(n_pages + 1, kv_heads, record)
+    for at, row in q4.parts(ps, hd, hd, 2)[0][1::2]:
+        heads[:, :, at:at + ps * row] = heads[:, :, at:at + ps * row] & 0x0F | 0x60
+    table = torch.randperm(n_pages, generator=g, device=DEV).int().view(1, -1)
+    view = ops.KvView(pool, table, 0, ps, kv_heads, hd, bits=4)
+    k = torch.empty(positions, kv_heads, hd, device=DEV)
+    v = torch.empty_like(k)
+    ops.kv_read(view, i32([[0], [0], [positions], [0]]), k, v)
+    return view, k, v
+
+
+def check_rows(out, q, k, v, rows, first, heads, scale, weight_half):
+    """Some rows of a portion whose first token is at position ``first``, against float64 on the device, within
+    ``check_attention``'s bound and what 4-bit attention's half-precision queries may lose: rows are scaled to the largest element
+    in [1, 2), where halves are off by 2^-25 at most below 2^-14 and hold a bfloat16 element's eight bits above 2^-17."""
+    hd, kv_heads = k.shape[2], k.shape[1]
+    group = heads // kv_heads
+    for h in range(kv_heads):
+        kd, vd = k[:, h].double(), v[:, h].double()
+        for r in rows:
+            n = first + r + 1
+            qr = q[r].view(heads, hd)[h * group:(h + 1) * group].double()
+            s = qr @ kd[:n].T * scale
+            w = torch.softmax(s, -1)
+            want, mass = w @ vd[:n], w @ vd[:n].abs()
+            e_s = ((qr.abs() @ kd[:n].abs().T).amax(-1) * ((hd + 4) * 2.0 ** -23 + 2.0 ** -22) +
+                   qr.abs().amax(-1) * 2.0 ** -25 * kd[:n].abs().sum(-1).amax()) * abs(scale)
+            tol = (2.0 ** -25 * vd[:n].abs().sum(0) + mass * (weight_half + 2 * e_s[:, None] + 2.0 ** -20 + (n + 8) * 2.0 ** -23) +
+                   1.01 * 2.0 ** -8 * want.abs() + 1e-30)
+            err = (out[r].view(heads, hd)[h * group:(h + 1) * group].double() - want).abs()
+            assert bool((err <= tol).all()), f"token {r}, kv head {h}: {float((err / tol).max()):.2f} of its bound"
+
+
+@pytest.mark.parametrize("heads,kv_heads,tokens,end", [(32, 8, 4096, 39936), (64, 8, 2048, 38912)])
+def test_portions_of_very_many_items(ops, heads, kv_heads, tokens, end):
+    """Heads of 256 take 8 query rows an item: 16,384 pairs of items and kv heads, whose ranges once wrapped in 32 bits."""
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import Runtime, StepContext
+    view, k, v = random_pages(ops, end, kv_heads, 256, 31)
+    q = (torch.randn(tokens, heads * 256, generator=torch.Generator().manual_seed(5)) * 0.5).bfloat16().to(DEV)
+    out = torch.full_like(q, float("nan"))
+    ctx = StepContext(rt=Runtime(torch.bfloat16, DEV, kv_bits=4), n_tokens=tokens, tokens=None, positions=i32(range(end - tokens, end)),
+                      token_slot=i32([0] * tokens), seg_slot=[0], seg_q_start=[0], seg_q_len=[tokens], seg_kv_len=[end],
+                      segments=i32([[0], [0], [tokens], [end]]))
+    linear.attention(q, view, ctx, out, heads, 1 / 16)
+    assert bool(torch.isfinite(out).all()), "rows were left as they were"
+    rows = [0, tokens - 1] + np.random.default_rng(2).integers(0, tokens, 14).tolist()
+    check_rows(out, q, k, v, rows, end - tokens, heads, 1 / 16, 2.0 ** -11)
+    # nothing of that division is left for the next launch
+    again = torch.full_like(q, float("nan"))
+    linear.attention(q, view, ctx, again, heads, 1 / 16)
+    assert torch.equal(again, out)
