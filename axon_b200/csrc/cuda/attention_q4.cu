@@ -58,7 +58,7 @@ struct QaParams {
     float2* part_ml;             // the same without the last index: maximum (log2 units) and sum
     unsigned int* arrived;       // [CTA]: pieces written of the pair that begins in the CTA's range and ends in another's; zero between launches
     PagedQ4 kv;
-    int n_segments, n_items, heads, group, ctas, window;
+    int n_segments, n_items, heads, group, ctas, window, staged;
     float scale_log2;
 };
 
@@ -326,8 +326,9 @@ attention_q4_kernel(const QaParams p) {
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
     pdl_launch_dependents();
 
-    // The division of the work and the first table entries do not wait for the kernel before: segments, lists and
-    // tables are copied to the device ahead of a step's kernels, none of which writes them.
+    // The division of the work and the first table entries do not wait for the kernel before where segments, lists
+    // and tables were copied to the device ahead of a step's kernels, none of which writes them.
+    if (!p.staged) pdl_wait();
     int item;
     uint32_t start;
     const QaPlan plan(p, R, &item, &start);
@@ -769,10 +770,11 @@ AXON_API int axon_attention_q4_division(const int32_t* tiles, int n_items, int k
 
 // Attention of `n_items` tiles of up to 8 * row_tiles query rows (row_tiles 1, 2 or 4; at head size 256 1).  items null:
 // item i is segment i, whose rows all fit one tile.  scratch: 2 * ctas * 8 * row_tiles * (head_dim + 2) + ctas floats, zeroed once:
-// launches leave the last ctas of them zero.
+// launches leave the last ctas of them zero.  staged: segments and the block table were copied to the device before the kernels in
+// flight were launched (pdl.cuh).
 AXON_API int axon_attention_q4(const void* q, const void* pool, void* out, const int32_t* segments, int n_segments,
                                const int32_t* items, int n_items, const AxonKvLayout* layout, int heads, float scale, int window,
-                               int row_tiles, float* scratch, long long scratch_floats, cudaStream_t stream) {
+                               int row_tiles, float* scratch, long long scratch_floats, int staged, cudaStream_t stream) {
     if (n_items <= 0) return AXON_OK;
     QaParams p;
     if (int st = to_q4(layout, pool, "axon_attention_q4", &p.kv)) return st;
@@ -790,7 +792,7 @@ AXON_API int axon_attention_q4(const void* q, const void* pool, void* out, const
     p.segments = segments; p.items = items;
     p.part_o = scratch; p.part_ml = reinterpret_cast<float2*>(scratch + rows * hd);
     p.arrived = reinterpret_cast<unsigned int*>(scratch + rows * (hd + 2));
-    p.n_segments = n_segments; p.n_items = n_items; p.heads = heads; p.group = heads / p.kv.kv_heads; p.window = window;
+    p.n_segments = n_segments; p.n_items = n_items; p.heads = heads; p.group = heads / p.kv.kv_heads; p.window = window; p.staged = staged;
     p.scale_log2 = scale * 1.4426950408889634f;
 #define AXON_Q4_CASE(HD, NT) if (hd == HD && row_tiles == NT) return launch_q4<HD, NT>(p, stream)
     AXON_Q4_CASE(64, 1); AXON_Q4_CASE(64, 2); AXON_Q4_CASE(64, 4);

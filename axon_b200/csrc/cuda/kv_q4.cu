@@ -129,12 +129,13 @@ template <typename T>
 __global__ void __launch_bounds__(Q4_WRITE_THREADS)
 rope_kv_write_q4_vec_kernel(const float* __restrict__ qkv, const float2* __restrict__ table, const int32_t* __restrict__ positions,
                             const int32_t* __restrict__ token_slot, T* __restrict__ q_out, uint8_t* __restrict__ pool, PagedQ4 kv,
-                            int heads, int write_kv, SplitFold fold) {
+                            int heads, int write_kv, int staged, SplitFold fold) {
     pdl_launch_dependents();
+    if (!staged) pdl_wait();
     const int t = blockIdx.x, half = kv.hd / 2, lanes = half / 4;                  // threads of a row
     const int items = (heads + (write_kv ? 2 * kv.kv_heads : 0)) * lanes;
     const float* row = qkv + (long long)t * ((heads + 2 * kv.kv_heads) * kv.hd);
-    // (positions, slots and tables are copied to the device ahead of a step's kernels: no need to wait for the one before)
+    // (staged positions, slots and tables are no work of the kernel before: no need to wait for it)
     const int pos = positions[t], lp = pos / kv.page_size, in_page = pos - lp * kv.page_size;
     const int entry = write_kv ? kv.block_table[(long long)token_slot[t] * kv.table_stride + lp] : 0;
     pdl_wait();
@@ -325,12 +326,13 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* _
 template <typename T>
 __global__ void __launch_bounds__(Q4_READ_THREADS)
 kv_read_q4_pages_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* __restrict__ segments, int n_segments,
-                        const int32_t* __restrict__ which, int n_long, int window, int pages, int stride, int32_t* __restrict__ seg_out,
-                        int32_t* __restrict__ table, Q4Out out) {
+                        const int32_t* __restrict__ which, int n_long, int window, int pages, int stride, int staged,
+                        int32_t* __restrict__ seg_out, int32_t* __restrict__ table, Q4Out out) {
     __shared__ long long rec[Q4_READ_ROWS];
     __shared__ int at[Q4_READ_ROWS];
     __shared__ int who, first_page, lo, count;
     pdl_launch_dependents();
+    if (!staged) pdl_wait();
     const int page = blockIdx.x / 2;
     if (threadIdx.x == 0) who = -1;
     __syncthreads();
@@ -594,11 +596,12 @@ using namespace axon;
 
 enum { AXON_Q4_F32 = 0, AXON_Q4_BF16 = 1 };          // the dtype codes of generic.cu
 
-// Rotates q and k (as axon_rope_kv_write), writes q in `dtype` and k and v quantised into the pool.
+// Rotates q and k (as axon_rope_kv_write), writes q in `dtype` and k and v quantised into the pool.  staged: positions, slots and
+// the block table were copied to the device before the kernels in flight were launched (pdl.cuh).
 AXON_API int axon_rope_kv_write_q4(const float* qkv, const float* table, const int32_t* positions, const int32_t* token_slot,
                                    void* q_out, void* pool, int dtype, const AxonKvLayout* layout, int n, int heads, int rot,
                                    int adjacent, int write_kv, const float* partial, int splits, int ntok, const float* bias,
-                                   cudaStream_t stream) {
+                                   int staged, cudaStream_t stream) {
     if (n <= 0) return AXON_OK;
     if (partial != nullptr && (splits < 1 || ntok < n)) { set_error("axon_rope_kv_write_q4: bad partial sums (splits %d, tokens %d of %d)", splits, n, ntok); return AXON_BAD_ARGUMENT; }
     PagedQ4 kv;
@@ -612,9 +615,9 @@ AXON_API int axon_rope_kv_write_q4(const float* qkv, const float* table, const i
         // few tokens: a CTA per 192 of a token's items; many: a CTA per token
         const dim3 vgrid(n, n >= 4 * 148 ? 1 : (items + Q4_WRITE_THREADS - 1) / Q4_WRITE_THREADS);
         if (dtype == AXON_Q4_F32)
-            launch_pdl(rope_kv_write_q4_vec_kernel<float>, vgrid, dim3(Q4_WRITE_THREADS), 0, stream, qkv, (const float2*)table, positions, token_slot, (float*)q_out, (uint8_t*)pool, kv, heads, write_kv, fold);
+            launch_pdl(rope_kv_write_q4_vec_kernel<float>, vgrid, dim3(Q4_WRITE_THREADS), 0, stream, qkv, (const float2*)table, positions, token_slot, (float*)q_out, (uint8_t*)pool, kv, heads, write_kv, staged, fold);
         else
-            launch_pdl(rope_kv_write_q4_vec_kernel<__nv_bfloat16>, vgrid, dim3(Q4_WRITE_THREADS), 0, stream, qkv, (const float2*)table, positions, token_slot, (__nv_bfloat16*)q_out, (uint8_t*)pool, kv, heads, write_kv, fold);
+            launch_pdl(rope_kv_write_q4_vec_kernel<__nv_bfloat16>, vgrid, dim3(Q4_WRITE_THREADS), 0, stream, qkv, (const float2*)table, positions, token_slot, (__nv_bfloat16*)q_out, (uint8_t*)pool, kv, heads, write_kv, staged, fold);
         return launch_status("axon_rope_kv_write_q4");
     }
     const int rows = heads + kv.planes * kv.kv_heads;
@@ -662,10 +665,11 @@ AXON_API int axon_kv_read_q4(const void* pool, const AxonKvLayout* layout, const
     return AXON_OK;
 }
 
-// See kv_read_q4_pages_kernel.  pages_out: bfloat16 [pages][2][kv_heads][64][head_dim].
+// See kv_read_q4_pages_kernel.  staged: segments and the block table were copied to the device before the kernels in flight
+// were launched (the list `which` has to be in any case).  pages_out: bfloat16 [pages][2][kv_heads][64][head_dim].
 AXON_API int axon_kv_read_q4_pages(const void* pool, const AxonKvLayout* layout, const int32_t* segments, int n_segments, const int32_t* which,
                                    int n_long, int window, int pages, int stride, int32_t* seg_out, int32_t* table, void* pages_out,
-                                   cudaStream_t stream) {
+                                   int staged, cudaStream_t stream) {
     if (n_long <= 0) return AXON_OK;
     PagedQ4 kv;
     if (int st = to_q4(layout, pool, "axon_kv_read_q4_pages", &kv)) return st;
@@ -675,7 +679,7 @@ AXON_API int axon_kv_read_q4_pages(const void* pool, const AxonKvLayout* layout,
     const long long plane = (long long)kv.kv_heads * 64 * kv.hd;
     const Q4Out out{pages_out, (uint8_t*)pages_out + plane * 2, 2 * plane, kv.hd, 64ll * kv.hd, 6};
     launch_pdl(kv_read_q4_pages_kernel<__nv_bfloat16>, dim3(2 * pages), dim3(Q4_READ_THREADS), 0, stream, (const uint8_t*)pool, kv, segments,
-               n_segments, which, n_long, window, pages, stride, seg_out, table, out);
+               n_segments, which, n_long, window, pages, stride, staged, seg_out, table, out);
     return launch_status("axon_kv_read_q4_pages");
 }
 

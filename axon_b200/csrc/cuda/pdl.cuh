@@ -10,7 +10,10 @@
 //    before the first global write of any kind (an earlier kernel may still be reading
 //    the target).  After it, all memory operations of all earlier kernels are visible.
 //  * Before pdl_wait() a kernel only reads data that no kernel of the step writes
-//    (weights, tensor maps) and touches its own shared and tensor memory.
+//    (weights, tensor maps) and touches its own shared and tensor memory.  A step's own lists
+//    (positions, slots, segments, work lists) and block tables are such data only when the caller
+//    says so (`staged`: they were copied to the device before the step's first kernel); a kernel
+//    that is not told so waits before it reads them.
 #pragma once
 
 #include <cuda_runtime.h>

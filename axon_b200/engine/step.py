@@ -287,7 +287,7 @@ class Engine:
                 seg_slot=seg_slot, seg_q_start=seg_q_start, seg_q_len=seg_q_len, seg_kv_len=seg_kv_len,
                 segments=dev[3 * n:3 * n + 4 * s].view(4, s),
                 unit_items=dev[total - 2 * s: total] if decode_only else None,
-                host_positions=host_positions)
+                host_positions=host_positions, staged=True)
         want_rows = dev[3 * n + 4 * s: 3 * n + 4 * s + n_want] if n_want else None
 
         if graph_key is None:

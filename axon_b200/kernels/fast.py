@@ -549,10 +549,10 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
     for nt, n_items, which, scratch, floats, _held in launches:
         check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),
                                    None if which is None else which.data_ptr(), n_items, kv._ref, heads, float(scale), int(kv.window),
-                                   nt, scratch, floats, _stream()))
+                                   nt, scratch, floats, int(ctx.staged), _stream()))
     for n, pages, stride, rows, tpt, which, tiles, n_tiles, segments, table, pool, layout, _held in plans:
         check(cu.axon_kv_read_q4_pages(kv.pool.data_ptr(), kv._ref, ctx.segments.data_ptr(), len(ctx.seg_q_len), which, n, int(kv.window),
-                                       pages, stride, segments, table, pool, _stream()))
+                                       pages, stride, segments, table, pool, int(ctx.staged), _stream()))
         if rows == 256:
             check(cu.axon_attention_tc(q.data_ptr(), pool, out.data_ptr(), segments, n, tiles, n_tiles, layout, heads, float(scale),
                                        int(kv.window), tpt, _stream()))

@@ -54,11 +54,11 @@ _SIGNATURES = {
     "axon_rope_kv_write": [P, P, P, P, P, P, c_int, ctypes.POINTER(KvLayout), c_int, c_int, c_int, c_int, c_int,
                            P, c_int, c_int, P, P],
     "axon_rope_kv_write_q4": [P, P, P, P, P, P, c_int, ctypes.POINTER(KvLayout), c_int, c_int, c_int, c_int, c_int,
-                              P, c_int, c_int, P, P],
+                              P, c_int, c_int, P, c_int, P],
     "axon_kv_read_q4": [P, ctypes.POINTER(KvLayout), P, c_int, c_int, P, P, c_int, c_longlong, P],
-    "axon_kv_read_q4_pages": [P, ctypes.POINTER(KvLayout), P, c_int, P, c_int, c_int, c_int, c_int, P, P, P, P],
+    "axon_kv_read_q4_pages": [P, ctypes.POINTER(KvLayout), P, c_int, P, c_int, c_int, c_int, c_int, P, P, P, c_int, P],
     "axon_attention_q4": [P, P, P, P, c_int, P, c_int, ctypes.POINTER(KvLayout), c_int, c_float, c_int, c_int, P,
-                          c_longlong, P],
+                          c_longlong, c_int, P],
     "axon_attention_q4_ctas": [c_int, c_int],
     "axon_attention_q4_division": [P, c_int, c_int, c_int, P],
     "axon_attention_q4_plain": [P, P, c_int, P, P, P, ctypes.POINTER(KvLayout), c_int, c_int, c_float, c_int, c_int, P,

@@ -44,7 +44,8 @@ def linear_swiglu(h: torch.Tensor, w_gate_up: torch.Tensor, act: torch.Tensor, r
 
 def attention(q: torch.Tensor, kv: ops.KvView, ctx, out: torch.Tensor, heads: int, scale: float,
               precise: bool = False) -> None:
-    """Attention of the step's tokens over the paged cache (in the model's dtype or in 4 bits)."""
+    """Attention of the step's tokens over the paged cache (in the model's dtype or in 4 bits).  ``ctx.staged`` says
+    whether the step's lists and the block table may be read before the kernel before has finished."""
     if not precise and fast.attention(q, kv, ctx, out, heads, scale):
         return
     shares = fast.q4_plain_shares(ctx, kv, heads) if kv.bits else None

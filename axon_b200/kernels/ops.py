@@ -200,10 +200,12 @@ def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, table: torch.Ten
 
 def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: torch.Tensor,
                   token_slot: torch.Tensor, q_out: torch.Tensor, kv: KvView, heads: int, rot: int,
-                  adjacent: bool = False, write_kv: bool = True, pending=None) -> None:
+                  adjacent: bool = False, write_kv: bool = True, pending=None, staged: bool = False) -> None:
     """Rotates queries and keys and writes queries to ``q_out``, keys and values to the cache (quantised
     when ``kv`` has 4 bits).  ``pending`` (a ``fast.PendingFold`` whose output is ``qkv``): the product is
-    still in partial sums; they are folded here (with the bias) and ``qkv`` itself is not read."""
+    still in partial sums; they are folded here (with the bias) and ``qkv`` itself is not read.  ``staged``:
+    positions, slots and the block table were there before the kernels in flight were launched
+    (``StepContext.staged``), so that they may be read while the kernel before is still running."""
     if kv.bits:
         quantised("rope_kv_write", kv, qkv, table, positions, token_slot, q_out)
     else:
@@ -219,11 +221,11 @@ def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: t
             raise TypeError("positions and slots are int32")
         if table is not None and (table.dtype != torch.float32 or table.numel() < n * rot):
             raise ValueError("rope_kv_write takes a float32 rotation table [n][rot / 2][2]")
-        write = lib.cuda().axon_rope_kv_write_q4
+        write, more = lib.cuda().axon_rope_kv_write_q4, (int(staged),)
     else:
         if q_out.dtype != kv.pool.dtype:
             raise TypeError("queries and the cache have one dtype")
-        write = lib.cuda().axon_rope_kv_write
+        write, more = lib.cuda().axon_rope_kv_write, ()          # (waits in any case)
     if pending is not None:
         pending.claim(qkv, accumulate=False)
     check(write(_ptr(qkv), _ptr(table), _ptr(positions), _ptr(token_slot), _ptr(q_out),
@@ -231,7 +233,7 @@ def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: t
                                         int(write_kv), None if pending is None else _ptr(pending.partial),
                                         0 if pending is None else pending.splits,
                                         0 if pending is None else pending.ntok,
-                                        None if pending is None else _ptr(pending.bias), _stream()))
+                                        None if pending is None else _ptr(pending.bias), *more, _stream()))
 
 
 def quantised(what: str, kv: KvView, *tensors: Optional[torch.Tensor]) -> None:

@@ -155,6 +155,10 @@ class StepContext:
     #: host copies for parts that run on the host side of a step (toy parts, tests)
     host_positions: Optional[List[int]] = None
     scratch: Dict[Any, Any] = field(default_factory=dict)
+    #: the tensors above and the caches' block tables were copied to the device before the step's first
+    #: kernel, and no kernel of the step writes them: kernels may read them before the kernel before
+    #: them has finished.  Left False where they may be the work of a kernel just launched
+    staged: bool = False
 
     @property
     def max_q_len(self) -> int:

@@ -176,7 +176,7 @@ class Attention(Mixer):
                                               write_cache, precise=rt.precise):
             q = rt.buffer("q", (n, self.q_dim))
             ops.rope_kv_write(qkv, table, ctx.positions, ctx.token_slot, q, cache, self.heads, rot, adjacent,
-                              write_kv=write_cache, pending=owed)
+                              write_kv=write_cache, pending=owed, staged=ctx.staged)
             _linear.attention(q, cache, ctx, att, self.heads, self.scale, precise=rt.precise)
         return _linear.linear(att, self.w_o, x, bias=self.b_o, accumulate=True, precise=rt.precise, defer=defer)
 

@@ -781,3 +781,91 @@ def test_portions_of_very_many_items(ops, heads, kv_heads, tokens, end):
     again = torch.full_like(q, float("nan"))
     linear.attention(q, view, ctx, again, heads, 1 / 16)
     assert torch.equal(again, out)
+
+
+# -- lists that are a kernel's work -----------------------------------------
+
+def picks(values):
+    """Logits whose argmax is ``values`` [n], in rows long enough that the kernel that finds them runs for a while after it has let
+    its successor start."""
+    v = torch.tensor(np.asarray(values).reshape(-1))
+    logits = torch.zeros(len(v), 400_000, device=DEV)
+    logits[torch.arange(len(v)), v.to(DEV)] = 1.0
+    return logits
+
+
+def test_positions_slots_and_tables_just_written_by_a_kernel(ops):
+    """What a launch just before has still to write is waited for: by the write, the attention's both ways and the plain kernels."""
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import Runtime, StepContext
+    heads, kv_heads, hd = 14, 2, 128
+    cache = Cache(ops, [700, 650], kv_heads, hd, 16, seed=33)
+    rt = Runtime(torch.bfloat16, DEV, kv_bits=4)
+    table_logits = picks(cache.table)
+    table = torch.zeros_like(cache.dev_table)
+    view = ops.KvView(cache.pool, table, 1, 16, kv_heads, hd, bits=4)
+
+    # the write: positions, slots, table
+    tab = torch.from_numpy(rope([690, 33], hd)).to(DEV)
+    qkv = torch.randn(2, (heads + 2 * kv_heads) * hd, generator=torch.Generator().manual_seed(2)).to(DEV)
+    q = torch.empty(2, heads * hd, dtype=torch.bfloat16, device=DEV)
+    for late in ("positions", "slots", "table"):
+        pool = cache.pool.clone()
+        ops.rope_kv_write(qkv, tab, i32([690, 33]), i32([0, 1]), q, ops.KvView(pool, cache.dev_table, 1, 16, kv_heads, hd, bits=4), heads, hd)
+        got = cache.pool.clone()
+        x = {"positions": i32([0, 0]), "slots": i32([1, 0]), "table": table.zero_()}
+        fine = {"positions": i32([690, 33]), "slots": i32([0, 1]), "table": cache.dev_table}
+        logits = {"positions": picks([690, 33]), "slots": picks([0, 1]), "table": table_logits}[late]
+        torch.cuda.synchronize()
+        ops.argmax(logits, x[late].view(-1))
+        use = {**fine, late: x[late]}
+        ops.rope_kv_write(qkv, tab, use["positions"], use["slots"], q, ops.KvView(got, use["table"], 1, 16, kv_heads, hd, bits=4), heads, hd)
+        assert torch.equal(got, pool), f"{late} were read too early"
+
+    # attention: segments and table, single tokens, portions and prompts read back
+    for q_lens in ([1, 1], [4, 3], [300, 650]):
+        n = sum(q_lens)
+        want, _, qs, pos, slot, scale = attend(ops, cache, q_lens, heads, torch.bfloat16)
+        seg = np.array([[0, 1], [0, q_lens[0]], q_lens, cache.lens])
+        for late in ("segments", "table"):
+            segments = i32([[0, 0], [0, 0], [1, 1], [1, 1]]) if late == "segments" else i32(seg)
+            table.zero_() if late == "table" else table.copy_(cache.dev_table)
+            logits = picks(seg) if late == "segments" else table_logits
+            ctx = StepContext(rt=rt, n_tokens=n, tokens=None, positions=i32(pos), token_slot=i32(slot), seg_slot=[0, 1], seg_q_start=[0, q_lens[0]],
+                              seg_q_len=list(q_lens), seg_kv_len=list(cache.lens), segments=segments)
+            out = torch.zeros_like(want)
+            linear.attention(qs, cache.view, ctx, out, heads, scale)             # (lists and scratch of this shape are there from now on)
+            torch.cuda.synchronize()
+            out.zero_()
+            ops.argmax(logits, (segments if late == "segments" else table).view(-1))
+            linear.attention(qs, view, ctx, out, heads, scale)
+            assert torch.equal(out, want), f"{late} were read too early by portions of {q_lens}"
+    # the plain kernels, and reading back
+    cache32 = attend(ops, cache, [1, 1], heads, torch.float32)
+    table.zero_()
+    torch.cuda.synchronize()
+    ops.argmax(table_logits, table.view(-1))
+    out = torch.empty_like(cache32[0])
+    ops.attention_plain(cache32[2], view, i32(cache32[3]), i32(cache32[4]), out, heads, cache32[5])
+    again = torch.empty_like(out)
+    ops.attention_plain(cache32[2], cache.view, i32(cache32[3]), i32(cache32[4]), again, heads, cache32[5])
+    assert torch.equal(out, again)
+    table.zero_()
+    torch.cuda.synchronize()
+    ops.argmax(table_logits, table.view(-1))
+    keys = torch.empty(650, kv_heads, hd, device=DEV)
+    ops.kv_read(view, i32([[1], [0], [650], [0]]), keys)
+    assert (keys.double().cpu().numpy() == cache.k[1]).all()
+
+
+def test_a_step_of_the_engine_is_staged(model_folders):
+    """The engine copies what a step's kernels read before the first of them, and says so; a context made by hand does not."""
+    from axon_b200.engine.step import StepEntry
+    from axon_b200.parts.base import StepContext
+    assert StepContext.__dataclass_fields__["staged"].default is False
+    e = engine_for(model_folders["C"], "bfloat16")
+    e.cuda_graphs = False
+    seen, forward = [], e.model.forward
+    e.model.forward = lambda ctx, *a, **kw: (seen.append(ctx.staged), forward(ctx, *a, **kw))[1]
+    e.step([StepEntry(e.open_request(), [1, 2, 3], [2])])
+    assert seen == [True]
