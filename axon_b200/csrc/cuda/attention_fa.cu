@@ -236,9 +236,10 @@ attention_fa_kernel(const FaParams p) {
     extern __shared__ __align__(128) unsigned char smem_raw[];
     pdl_launch_dependents();
     // The prompt shape waits here: queries and this step's keys come from the kernels before.
-    // The decode shape first requests the key tiles that hold only older positions (nothing in
-    // this step writes them; lengths and block tables are in place before the step starts), so
-    // that the cache streams in while the kernels before are still finishing.
+    // The decode shape of a staged step first requests the key tiles that hold only older positions
+    // (nothing in such a step writes them; lengths and block tables are in place before it starts),
+    // so that the cache streams in while the kernels before are still finishing.  Other steps' launches
+    // start when the kernels before have finished (launch_fa).
     if (!DECODE) pdl_wait();
     const uint32_t smem = (uint32_t)__cvta_generic_to_shared(smem_raw);
     // decode: [Q | K tiles | V tiles].  prefill: [K tiles | V tiles] with the queries parked in
@@ -685,14 +686,15 @@ __global__ void __launch_bounds__(FA_COMBINE_THREADS) attention_combine_kernel(c
 }
 
 template <int HD, bool DECODE, bool CHECKED>
-static int launch_fa(const FaParams& p, int n_items, int kv_heads, cudaStream_t stream) {
+static int launch_fa(const FaParams& p, int n_items, int kv_heads, bool staged, cudaStream_t stream) {
     constexpr int BM = DECODE ? 16 : 64;
     constexpr size_t tiles = (DECODE ? (size_t)BM * HD * 2 : 0) + 2 * (DECODE ? 3 : 2) * (size_t)FA_BN * HD * 2;
     constexpr size_t merge = DECODE ? (size_t)BM * HD * 2 + (4 * 16 * (HD + 8) + 4 * 16 * 2) * sizeof(float) : 0;
     constexpr size_t smem = tiles > merge ? tiles : merge;
     if (int st = ensure_dynamic_smem<attention_fa_kernel<HD, DECODE, CHECKED>>(smem, "axon_attention_fa")) return st;
     dim3 grid(n_items, kv_heads, DECODE ? p.n_splits : 1);
-    launch_pdl(attention_fa_kernel<HD, DECODE, CHECKED>, grid, dim3(FA_THREADS), smem, stream, p);
+    // (a wait at the kernel's top under a run-time flag cost the fused decode step up to 1 %, staged or not)
+    launch_chained(!DECODE || staged, attention_fa_kernel<HD, DECODE, CHECKED>, grid, dim3(FA_THREADS), smem, stream, p);
     int st = launch_status("axon_attention_fa");
     if (st != AXON_OK) return st;
     if (DECODE && p.n_splits > 1 && p.counters == nullptr) {
@@ -755,8 +757,8 @@ static int attention_fa_launch(const void* q, const void* pool, void* out, const
 #define AXON_FA_CASE(HD)                                                                         \
     case HD:                                                                                     \
         if (p.kv.fault != nullptr)                                                               \
-            return decode ? launch_fa<HD, true, true>(p, n_items, kvh, stream) : launch_fa<HD, false, true>(p, n_items, kvh, stream); \
-        return decode ? launch_fa<HD, true, false>(p, n_items, kvh, stream) : launch_fa<HD, false, false>(p, n_items, kvh, stream);
+            return decode ? launch_fa<HD, true, true>(p, n_items, kvh, decode == 2, stream) : launch_fa<HD, false, true>(p, n_items, kvh, false, stream); \
+        return decode ? launch_fa<HD, true, false>(p, n_items, kvh, decode == 2, stream) : launch_fa<HD, false, false>(p, n_items, kvh, false, stream);
     switch (hd) {
         AXON_FA_CASE(16)
         AXON_FA_CASE(32)
@@ -767,6 +769,8 @@ static int attention_fa_launch(const void* q, const void* pool, void* out, const
 #undef AXON_FA_CASE
 }
 
+// decode: 0 tiles of up to 64 query rows, 1 tiles of up to 16 with the keys split, 2 the same for a staged step: segments,
+// items and the block table were copied to the device ahead of the kernels in flight, which write no cache rows of positions before the segments' own.
 AXON_API int axon_attention_fa(const void* q, const void* pool, void* out, const int32_t* segments, int n_segments,
                                const int32_t* items, int n_items, const AxonKvLayout* layout, int heads,
                                float scale, int window, int decode, int tokens_per_tile, int n_splits,
@@ -782,12 +786,12 @@ AXON_API int axon_attention_fa(const void* q, const void* pool, void* out, const
 // biases added, or (partial != null) still owed the partial sums of a deferred split-K product
 // with its bias.  table: (cos, sin) [tokens][hd / 2] for pairs (i, i + hd / 2) over the whole
 // head, or null for no rotation.  write_kv == 0: the cache holds the new positions already
-// (a layer reading another layer's cache).  Otherwise as axon_attention_fa with decode != 0.
+// (a layer reading another layer's cache).  Otherwise as axon_attention_fa with decode 2 where `staged` is set, else 1.
 AXON_API int axon_attention_fa_decode_fused(const float* qkv, const float* partial, int fold_splits, int fold_ntok,
                                             const float* bias, const float* table, int write_kv, void* pool, void* out,
                                             const int32_t* segments, int n_segments, const AxonKvLayout* layout,
                                             int heads, float scale, int window, int tokens_per_tile, int max_q_len,
-                                            int n_splits, float* scratch, unsigned int* counters, cudaStream_t stream) {
+                                            int n_splits, float* scratch, unsigned int* counters, int staged, cudaStream_t stream) {
     const int hd = layout->head_dim;
     if (max_q_len < 1 || max_q_len > tokens_per_tile) { set_error("axon_attention_fa_decode_fused: segments of up to %d tokens do not fit tiles of %d", max_q_len, tokens_per_tile); return AXON_BAD_ARGUMENT; }
     if (qkv == nullptr) { set_error("axon_attention_fa_decode_fused: no q/k/v product given"); return AXON_BAD_ARGUMENT; }
@@ -801,8 +805,8 @@ AXON_API int axon_attention_fa_decode_fused(const float* qkv, const float* parti
     f.table = (const float2*)table;
     f.qkv_width = (heads + 2 * layout->kv_heads) * hd;
     f.write_kv = write_kv;
-    return attention_fa_launch(qkv, pool, out, segments, n_segments, nullptr, n_segments, layout, heads, scale, window, 1,
-                               tokens_per_tile, n_splits, scratch, counters, f, stream);
+    return attention_fa_launch(qkv, pool, out, segments, n_segments, nullptr, n_segments, layout, heads, scale, window,
+                               staged ? 2 : 1, tokens_per_tile, n_splits, scratch, counters, f, stream);
 }
 
 // ---------------------------------------------------------------------------

@@ -309,7 +309,7 @@ def attention_decode_fused(qkv, pending, table, rot: int, adjacent: bool, kv, ct
         ctx.segments.data_ptr(), n, kv._ref, heads, float(scale), int(kv.window), 16 // (heads // kv.kv_heads),
         ctx.max_q_len, splits,
         None if scratch is None else scratch.data_ptr(),
-        counters.data_ptr() if FA_FOLD_IN_KERNEL and n * kv.kv_heads <= counters.numel() else None, _stream()))
+        counters.data_ptr() if FA_FOLD_IN_KERNEL and n * kv.kv_heads <= counters.numel() else None, int(ctx.staged), _stream()))
     return True
 
 
@@ -339,7 +339,7 @@ def attention(q, kv, ctx, out, heads: int, scale: float) -> bool:
         check(cu.axon_attention_fa(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), n_seg,
                                    None if it["dec"] is None else it["dec"].data_ptr(), it["n_dec"], kv._ref, heads,
                                    float(scale), int(kv.window),
-                                   1, it["tpt_dec"], splits, None if scratch is None else scratch.data_ptr(),
+                                   2 if ctx.staged else 1, it["tpt_dec"], splits, None if scratch is None else scratch.data_ptr(),
                                    counters.data_ptr() if FA_FOLD_IN_KERNEL and it["n_dec"] * kv.kv_heads <= counters.numel() else None,
                                    _stream()))
     if it["n_pre"] and use_tc:

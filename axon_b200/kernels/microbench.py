@@ -71,7 +71,7 @@ def _ctx(segs, items=True):
     unit = i32([[s, 0] for s in range(len(segs))]).flatten() if all(n == 1 for _, n, _ in segs) else None
     return StepContext(rt=rt, n_tokens=at, tokens=i32([0] * at), positions=i32(pos), token_slot=i32(slot_of),
                        seg_slot=rows[0], seg_q_start=rows[1], seg_q_len=rows[2], seg_kv_len=rows[3],
-                       segments=i32(rows), unit_items=unit, host_positions=pos)
+                       segments=i32(rows), unit_items=unit, host_positions=pos, staged=True)
 
 
 def main() -> int:

@@ -156,8 +156,8 @@ class StepContext:
     host_positions: Optional[List[int]] = None
     scratch: Dict[Any, Any] = field(default_factory=dict)
     #: the tensors above and the caches' block tables were copied to the device before the step's first
-    #: kernel, and no kernel of the step writes them: kernels may read them before the kernel before
-    #: them has finished.  Left False where they may be the work of a kernel just launched
+    #: kernel, and the kernels of the step write neither them nor cached rows of positions before its own: kernels may
+    #: read all these before the kernel before them has finished.  Left False where they may be the work of a kernel just launched
     staged: bool = False
 
     @property

@@ -993,3 +993,44 @@ def test_tensor_pipe_probe_times_the_attention_products(ops):
     fast.check(lib.cuda().axon_mma_probe(5, steps, scratch.data_ptr(), cycles, fast._stream()))
     assert cycles[0] / steps >= 1024 and cycles[1] / steps >= 1024
     assert lib.cuda().axon_mma_probe(1, 0, scratch.data_ptr(), cycles, fast._stream()) != 0      # refused: no steps
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(28, 4, 128), (6, 2, 64)])
+def test_decode_attention_waits_for_lists_just_written(ops, heads, kv_heads, hd, fused):
+    """Segments and a block table that the launch just before has still to write: a step that is not said to be staged
+    waits for them.  Staged or not, the same bits."""
+    from axon_b200.kernels import fast
+    from axon_b200.parts import StepContext
+    lens = [700, 333]
+    view, table = make_cache(ops, torch.bfloat16, kv_heads, hd, 16, 100, 2, 704, seed=19)
+    view.pool.copy_(rand(*view.pool.shape, dtype=torch.bfloat16, seed=140))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    segments = [[0, 1], [0, 1], [1, 1], lens]
+    q = rand(2, heads * hd, dtype=torch.bfloat16, seed=141)
+    qkv = rand(2, (heads + 2 * kv_heads) * hd, seed=142)
+
+    def step(seg, view, staged, late=None):
+        ctx = StepContext(rt=_ctx_for([(0, 1, 5)]).rt, n_tokens=2, tokens=None, positions=i32([l - 1 for l in lens]), token_slot=i32([0, 1]),
+                          seg_slot=[0, 1], seg_q_start=[0, 1], seg_q_len=[1, 1], seg_kv_len=lens, segments=seg,
+                          unit_items=i32([[0, 0], [1, 0]]).flatten(), staged=staged)
+        out = torch.zeros(2, heads * hd, dtype=torch.bfloat16, device=DEV)
+        run = (lambda: fast.attention_decode_fused(qkv, None, None, 0, False, view, ctx, out, heads, 0.1, False)) if fused else (
+            lambda: fast.attention(q, view, ctx, out, heads, 0.1))
+        if late is not None:
+            values, target = late
+            target.copy_(torch.zeros_like(target) if target.numel() != 8 else i32([[0, 0], [0, 0], [1, 1], [1, 1]]))
+            logits = torch.zeros(values.numel(), 400_000, device=DEV)
+            logits[torch.arange(values.numel(), device=DEV), values.flatten().long()] = 1.0
+            torch.cuda.synchronize()
+            ops.argmax(logits, target.view(-1))          # lets its successor start long before it writes
+        assert run()
+        return out
+
+    want = step(i32(segments), view, True)
+    assert torch.equal(step(i32(segments), view, False), want) and want.float().abs().sum() > 0
+    seg = torch.zeros(4, 2, dtype=torch.int32, device=DEV)
+    assert torch.equal(step(seg, view, False, (i32(segments), seg)), want), "segments were read too early"
+    other = torch.zeros_like(table)
+    late_view = ops.KvView(view.pool, other, 1, 16, kv_heads, hd)
+    assert torch.equal(step(i32(segments), late_view, False, (table, other)), want), "the block table was read too early"
