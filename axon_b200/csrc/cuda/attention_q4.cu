@@ -689,7 +689,10 @@ attention_q4_kernel(const QaParams p) {
         if (threadIdx.x == 0) {
             __threadfence();
             last = atomicAdd(p.arrived + c0, 1u) == (unsigned)(c1 - c0);
-            if (last) p.arrived[c0] = 0;                           // ready for the next launch
+            if (last) {
+                __threadfence();                                   // the others' pieces, counted by their atomics, are seen from here on
+                p.arrived[c0] = 0;                                 // ready for the next launch
+            }
         }
         __syncthreads();
         if (last) {

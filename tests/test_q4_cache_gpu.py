@@ -869,3 +869,24 @@ def test_a_step_of_the_engine_is_staged(model_folders):
     e.model.forward = lambda ctx, *a, **kw: (seen.append(ctx.staged), forward(ctx, *a, **kw))[1]
     e.step([StepEntry(e.open_request(), [1, 2, 3], [2])])
     assert seen == [True]
+
+
+def test_pieces_are_folded_when_all_have_arrived(ops):
+    """Requests cut into many pieces, two sets of queries in turn: scratch holds the other call's pieces whenever a CTA folds, and a
+    piece read before it arrived would show in the bits."""
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import Runtime, StepContext
+    for positions, heads, kv_heads in ((32768, 12, 2), (9001, 28, 4), (700, 14, 2)):
+        view, _, _ = random_pages(ops, positions, kv_heads, 128, 41)
+        ctx = StepContext(rt=Runtime(torch.bfloat16, DEV, kv_bits=4), n_tokens=1, tokens=None, positions=i32([positions - 1]), token_slot=i32([0]),
+                          seg_slot=[0], seg_q_start=[0], seg_q_len=[1], seg_kv_len=[positions], segments=i32([[0], [0], [1], [positions]]))
+        qs = [(torch.randn(1, heads * 128, generator=torch.Generator().manual_seed(s)) * 0.3).bfloat16().to(DEV) for s in (1, 2)]
+        outs = [torch.zeros_like(q) for q in qs]
+        for q, o in zip(qs, outs):
+            linear.attention(q, view, ctx, o, heads, 0.09)
+        assert torch.isfinite(outs[0]).all() and not torch.equal(*outs)
+        got = torch.zeros(300, 2, heads * 128, dtype=torch.bfloat16, device=DEV)
+        for k in range(300):
+            for j in range(2):
+                linear.attention(qs[j], view, ctx, got[k, j:j + 1], heads, 0.09)
+        assert all(bool((got[:, j] == outs[j]).all()) for j in range(2))
