@@ -361,23 +361,24 @@ Q4_PLAIN_KEYS, Q4_PLAIN_HEADS, Q4_PLAIN_CTAS = 64, 8, 5 * SM_COUNT
 
 
 def q4_plain_splits(ctx, heads: int, kv_heads: int, window: int) -> int:
-    """Into how many shares the plain 4-bit attention cuts each token's keys: as many as fill the GPU."""
+    """Into how many shares the plain 4-bit attention cuts each token's keys: as many as fill the GPU, and where that is one
+    for each 64 keys, a number rounded up (shares without keys add nothing), so that decoding meets few different ones."""
     keys = min(ctx.max_kv_len, window) if window else ctx.max_kv_len
     ctas = ctx.n_tokens * kv_heads * -(-(heads // kv_heads) // Q4_PLAIN_HEADS)
-    return max(1, min(-(-keys // Q4_PLAIN_KEYS), Q4_PLAIN_CTAS // max(ctas, 1)))
+    return max(1, min(_q4_bucket(-(-keys // Q4_PLAIN_KEYS), 4), Q4_PLAIN_CTAS // max(ctas, 1)))
 
 
 def q4_plain_shares(ctx, kv, heads: int):
-    """The same with its scratch (None for one share), cached per step."""
+    """The same with its scratch (None for one share), cached per step.  Launches of more than one share have at most Q4_PLAIN_CTAS
+    CTAs, which is what scratch and counters are sized for, once: they never move under a captured graph."""
     key = ("q4_plain", heads, kv.kv_heads, kv.v_dim, kv.window)
     got = ctx.scratch.get(key)
     if got is None:
         n = q4_plain_splits(ctx, heads, kv.kv_heads, kv.window)
         got = ops.KeyShares()
         if n > 1:
-            floats = lib.cuda().axon_attention_q4_plain_scratch(ctx.n_tokens, heads, kv.kv_heads, kv.v_dim, n)
-            got = ops.KeyShares(n, ctx.rt.buffer("q4_plain_scratch", (floats,), torch.float32),
-                                ctx.rt.zeroed_buffer("q4_plain_counters", (ctx.n_tokens * heads,), torch.int32))
+            got = ops.KeyShares(n, ctx.rt.buffer(f"q4_plain_scratch_{kv.v_dim}", (Q4_PLAIN_CTAS * Q4_PLAIN_HEADS * (kv.v_dim + 2),), torch.float32),
+                                ctx.rt.zeroed_buffer("q4_plain_counters", (Q4_PLAIN_CTAS,), torch.int32))
         ctx.scratch[key] = got
     return got
 
@@ -434,9 +435,10 @@ def _q4_long(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: 
     return got
 
 
-def _q4_bucket(n: int) -> int:
-    """``n`` rounded up to a multiple of an eighth of the power of two below it: sizes that graphs may share."""
-    step = 1 << max(0, n.bit_length() - 4)
+def _q4_bucket(n: int, parts: int = 8) -> int:
+    """``n`` rounded up to a multiple of an eighth (``parts``: a power of two) of the power of two below it: sizes that
+    graphs may share."""
+    step = 1 << max(0, n.bit_length() - parts.bit_length())
     return -(-n // step) * step
 
 

@@ -277,7 +277,8 @@ def kv_read(kv: KvView, spans: torch.Tensor, keys: Optional[torch.Tensor], value
 @dataclass
 class KeyShares:
     """How the plain attention over a 4-bit cache cuts each token's keys: the number of shares, float32 scratch for their
-    results (``axon_attention_q4_plain_scratch``), and int32 counters (zero, and left so), one per token and head at least."""
+    results (``axon_attention_q4_plain_scratch``), and int32 counters (zero, and left so), one for each token and eight heads
+    of a kv head."""
 
     count: int = 1
     scratch: Optional[torch.Tensor] = None

@@ -185,3 +185,23 @@ def test_portions_of_very_many_items_are_divided_whole(heads, kv_heads, tokens, 
     rows = np.arange(0, tokens * group, 8)
     tiles = (end - tokens + np.minimum(tokens, -(-(rows + 8) // group)) + 15) // 16
     assert not check_division(tiles, kv_heads, 148)
+
+
+def test_key_shares_of_the_plain_attention():
+    """Few different counts while a context grows (each is a captured step), no share of more than 64 keys unless the GPU is full,
+    and scratch whose size follows none of it."""
+    from types import SimpleNamespace
+    from axon_b200.kernels import fast, lib
+    for heads, kv_heads, tokens, window in ((8, 2, 1, 0), (6, 1, 1, 0), (28, 4, 3, 0), (8, 2, 4, 1024), (8, 8, 64, 0), (40, 2, 1, 0)):
+        counts = set()
+        for kv in range(1, 30000, 7):
+            ctx = SimpleNamespace(max_kv_len=kv, n_tokens=tokens)
+            n = fast.q4_plain_splits(ctx, heads, kv_heads, window)
+            tiles = -(-(min(kv, window) if window else kv) // 64)
+            full = max(1, fast.Q4_PLAIN_CTAS // (tokens * kv_heads * -(-(heads // kv_heads) // 8)))
+            assert n >= min(tiles, full) and n <= max(full, 1) and (n <= tiles * 1.25 or n == 1)
+            counts.add(n)
+            if n > 1:
+                assert lib.cuda().axon_attention_q4_plain_scratch(tokens, heads, kv_heads, 64, n) <= fast.Q4_PLAIN_CTAS * fast.Q4_PLAIN_HEADS * 66
+                assert tokens * kv_heads * -(-(heads // kv_heads) // 8) <= fast.Q4_PLAIN_CTAS
+        assert len(counts) <= 36, len(counts)

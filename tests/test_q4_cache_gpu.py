@@ -890,3 +890,22 @@ def test_pieces_are_folded_when_all_have_arrived(ops):
             for j in range(2):
                 linear.attention(qs[j], view, ctx, got[k, j:j + 1], heads, 0.09)
         assert all(bool((got[:, j] == outs[j]).all()) for j in range(2))
+
+
+@pytest.mark.parametrize("name,dtype", [("C", "float32"), ("D", "bfloat16")])
+def test_graphs_of_the_plain_kernels_outlive_longer_contexts(model_folders, name, dtype):
+    """Decoding beside ever longer contexts moves no buffer of a captured step, and captures few steps."""
+    from axon_b200.engine.step import StepEntry
+    from test_engine_gpu import tokens_for
+    e = engine_for(model_folders[name], dtype, max_tokens=4096, max_positions=2100, max_step_tokens=1000)
+    a, b = e.open_request(), e.open_request()
+    e.step([StepEntry(a, tokens_for(name, 0, 200), [199])])
+    e.step([StepEntry(b, tokens_for(name, 0, 200), [199])])
+    captured = []
+    for i in range(18):
+        e.step([StepEntry(b, tokens_for(name, 2 + i, 100), [99])])
+        e.step([StepEntry(a, [1], [0]), StepEntry(b, [2], [0])])
+        captured.append(dict(e._graphs))
+    for graphs in captured:
+        assert all(e._graphs.get(k) is g for k, g in graphs.items()), "a captured step was thrown away"
+    assert captured[0] and sum(k[0] == 2 for k in e._graphs) <= 12
