@@ -95,7 +95,10 @@ class BackendOptions:
     def kv(self, kv: str) -> "BackendOptions":
         """The cache type.  ``auto``, ``bf16`` and ``f32``: the model's dtype (the latter two are accepted
         when they agree with it).  ``q4``: keys and values are quantised to 4 bits as they are written
-        (4.5 bits a value with their steps, 3.6 times as many positions as bf16 in the same memory)."""
+        (4.5 bits a value with their steps, 3.6 times as many positions as bf16 in the same memory).  Beside the pool a
+        bfloat16 model then takes pages that prompts are read back into: one layer's keys and values in bfloat16, of as many
+        positions as all requests may hold but at most 262,144, or one request's if it may hold more (4 kv heads of 128: 2 KiB a
+        position, 576 MiB at most with 16 requests of 32,768)."""
         parse_kv(kv, self._dtype)
         return replace(self, _kv="q4" if kv == "q4" else "auto")
 

@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import math
 import os
 from typing import Optional, Union
 
@@ -60,12 +61,13 @@ def step_workspace_bytes(hidden_size: int, vocab_size: int, max_step_tokens: int
     return max_step_tokens * hidden_size * 64 + 4 * vocab_size * max(max_slots, 1)
 
 
-def quantised_workspace_bytes(needs, max_slots: int, max_positions: int) -> int:
-    """What prompts over a quantised cache take beside it: the bfloat16 pages that their keys and values are read back into."""
-    from ..kernels.fast import q4_prompt_room
-    widest = max((n.elements_per_token for entry in needs for n in entry.values() if getattr(n, "bits", 0)), default=0)
+def quantised_workspace_bytes(needs, max_slots: int, max_positions: int, dtype: torch.dtype = torch.bfloat16) -> int:
+    """What prompts over a quantised cache take beside it: the bfloat16 pages that their keys and values are read back into
+    (nothing in the 32-bit model, whose kernels read the cache as it is)."""
+    from ..kernels.fast import q4_prompt_buffers, q4_prompt_room
     pages, ints = q4_prompt_room(max_slots, max_positions, max_slots * max_positions)
-    return 2 * widest * 64 * pages + 4 * ints if widest else 0
+    shapes = q4_prompt_buffers(needs, pages).values() if dtype == torch.bfloat16 else ()
+    return sum(2 * math.prod(s) + 4 * ints for s in shapes)
 
 
 def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] = None,
@@ -85,7 +87,8 @@ def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] 
     ``AXON_CHECK_TABLES=1``) is a debugging mode in which the kernels compare every
     block-table entry they read with the pool's size and the step raises instead of
     following a bad one.  ``kv`` is the cache type: ``auto`` (the model's dtype) or ``q4`` (quantised to
-    4 bits as it is written, in every part that takes it).
+    4 bits as it is written, in every part that takes it; a bfloat16 model then takes bfloat16 pages of up to 262,144
+    positions of one layer beside the pool, which prompts are read back into).
     """
     dev = require_gpu(device)
     dt = parse_dtype(dtype)
@@ -111,7 +114,7 @@ def build_engine(folder: Optional[str] = None, *, config: Optional[ModelConfig] 
             max_tokens = plan_pool_tokens(free, bytes_per_token(model.needs, dt, page_size), page_size, max_slots, max_positions,
                                           step_workspace_bytes(spec.hidden_size, spec.vocab_size,
                                                                min(max_step_tokens, max_slots * max_positions), max_slots)
-                                          + quantised_workspace_bytes(model.needs, max_slots, max_positions))
+                                          + quantised_workspace_bytes(model.needs, max_slots, max_positions, dt))
             if max_tokens < page_size:
                 raise RuntimeError(f"{free >> 20} MiB are free on {dev} once the weights are placed: no room for a cache pool")
         if check_tables is None:

@@ -86,6 +86,10 @@ class Engine:
             from ..kernels import fast
             self.rt.kv_prompt_pages, self.rt.kv_prompt_entries = fast.q4_prompt_room(
                 cache.max_slots, cache.max_positions, cache.n_pages * cache.page_size)
+            if not self.rt.precise:
+                # here rather than at the first long prompt: an engine that was built has its memory
+                for name, shape in fast.q4_prompt_buffers(model.needs, self.rt.kv_prompt_pages).items():
+                    self.rt.buffer(name, shape, torch.bfloat16)
         self.max_step_tokens = max_step_tokens
         self._staging: List[torch.Tensor] = []
         self._events: List[Optional[torch.cuda.Event]] = []

@@ -449,6 +449,17 @@ def q4_prompt_room(max_slots: int, max_positions: int, pool_positions: int):
     return _q4_bucket(-(-at_once // 64) + max_slots), max_slots * (8 + longest)
 
 
+def q4_prompt_buffers(needs, pages: int):
+    """The bfloat16 pages that prompts over a model's 4-bit caches are read back into: ``{scratch name: shape}``, one for each
+    count and size of heads (layers take turns), for ``needs`` as the model lists them and ``pages`` of 64 positions."""
+    return {_q4_pages_name(n.kv_heads, n.head_dim): (pages, 2, n.kv_heads, 64, n.head_dim) for entry in needs for n in entry.values()
+            if getattr(n, "bits", 0) and n.planes == 2 and n.value_dim == n.head_dim and n.head_dim in FA_HEAD_DIMS}
+
+
+def _q4_pages_name(kv_heads: int, hd: int) -> str:
+    return f"q4_prompt_pages_{kv_heads}_{hd}"
+
+
 def _q4_prompt_sizes(ctx, segs, window: int):
     """(pages of 64 positions that these segments' keys take, those of the longest), rounded up."""
     n = []
@@ -511,7 +522,7 @@ def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: 
         n = len(segs)
         ints = ctx.rt.buffer(f"q4_plan_{window}_{k}", (max(4 * n + n * stride, ctx.rt.kv_prompt_entries),), torch.int32)
         room = max(pages, ctx.rt.kv_prompt_pages)
-        pool = ctx.rt.buffer(f"q4_prompt_pages_{kv_heads}_{hd}", (room, 2, kv_heads, 64, hd), torch.bfloat16)
+        pool = ctx.rt.buffer(_q4_pages_name(kv_heads, hd), (room, 2, kv_heads, 64, hd), torch.bfloat16)
         layout = lib.KvLayout(block_table=ints[4 * n:].data_ptr(), table_stride=stride, page_size=64, kv_heads=kv_heads, head_dim=hd,
                               page_stride=2 * kv_heads * 64 * hd, entry_offset=0, v_offset=kv_heads * 64 * hd, v_dim=hd, planes=2,
                               n_pages=room - 1, bits=0, fault=None)

@@ -205,3 +205,19 @@ def test_key_shares_of_the_plain_attention():
                 assert lib.cuda().axon_attention_q4_plain_scratch(tokens, heads, kv_heads, 64, n) <= fast.Q4_PLAIN_CTAS * fast.Q4_PLAIN_HEADS * 66
                 assert tokens * kv_heads * -(-(heads // kv_heads) // 8) <= fast.Q4_PLAIN_CTAS
         assert len(counts) <= 36, len(counts)
+
+
+def test_memory_that_prompts_are_read_back_into():
+    """Counted for each count and size of heads that can be read back, not at all for the 32-bit model."""
+    from axon_b200.engine.build import quantised_workspace_bytes
+    from axon_b200.kernels import fast
+    from axon_b200.parts.spec import KvNeed, StateNeed
+    a, b = KvNeed(4, 128, bits=4), KvNeed(2, 64, window=100, bits=4)
+    needs = [{"x": a}, {"x": b, "y": StateNeed((3,), "float32")}, {"x": KvNeed(4, 128, window=50, bits=4)}, {}, {"x": KvNeed(8, 128)},
+             {"x": KvNeed(1, 256, bits=4)}, {"x": KvNeed(1, 64, v_dim=32, bits=4)}, {"x": KvNeed(1, 64, planes=1, bits=4)}]
+    pages, ints = fast.q4_prompt_room(16, 4096, 65536)
+    assert fast.q4_prompt_buffers(needs, pages) == {fast._q4_pages_name(4, 128): (pages, 2, 4, 64, 128), fast._q4_pages_name(2, 64): (pages, 2, 2, 64, 64)}
+    each = [quantised_workspace_bytes([{"x": n}], 16, 4096) for n in (a, b)]
+    assert each[0] == pages * 64 * 2 * 4 * 128 * 2 + 4 * ints and quantised_workspace_bytes(needs, 16, 4096) == sum(each)
+    assert quantised_workspace_bytes(needs, 16, 4096, torch.float32) == 0
+    assert quantised_workspace_bytes([{"x": KvNeed(1, 256, bits=4)}], 16, 4096) == 0

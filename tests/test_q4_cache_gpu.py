@@ -909,3 +909,19 @@ def test_graphs_of_the_plain_kernels_outlive_longer_contexts(model_folders, name
     for graphs in captured:
         assert all(e._graphs.get(k) is g for k, g in graphs.items()), "a captured step was thrown away"
     assert captured[0] and sum(k[0] == 2 for k in e._graphs) <= 12
+
+
+def test_prompts_take_no_memory_that_was_not_there(model_folders, monkeypatch):
+    """An engine over a 4-bit cache has what its longest prompts are read back into from the start, and the 32-bit model nothing."""
+    from axon_b200.engine.step import StepEntry
+    from test_engine_gpu import tokens_for
+    force(monkeypatch, "read back")
+    for dtype in ("bfloat16", "float32"):
+        e = engine_for(model_folders["C"], dtype, max_tokens=4096, max_positions=1500, max_step_tokens=3000, max_slots=2)
+        held = {k: v.data_ptr() for k, v in e.rt._buffers.items() if k.startswith("q4_prompt_pages")}
+        assert len(held) == (dtype == "bfloat16")
+        slots = [e.open_request(), e.open_request()]
+        e.step([StepEntry(s, tokens_for("C", i, 1500), [1499]) for i, s in enumerate(slots)])
+        took = any(k.startswith("q4_plan") for k in e.rt._buffers)
+        assert took == (dtype == "bfloat16"), "the prompts should have been read back in the bfloat16 model"
+        assert {k: v.data_ptr() for k, v in e.rt._buffers.items() if k.startswith("q4_prompt_pages")} == held
