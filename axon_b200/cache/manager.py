@@ -224,20 +224,22 @@ class PagedCache:
         """Cache bytes one position takes over all groups."""
         return bytes_per_token([g.need for g in self.groups for _ in g.members], self.dtype, self.page_size)
 
-    def read(self, slot: int, entry: int, part: Optional[str] = None, first: int = 0,
+    def read(self, slot: int, entry: int, part: Optional[str] = None, first: Optional[int] = None,
              count: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """What a request holds for one part of schedule entry ``entry``: its keys ``[count][kv_heads][head_dim]``
-        and values ``[count][kv_heads][v_dim]`` at positions ``first ..`` (by default all it holds), in the
-        model's dtype, read back from the pages whatever form they keep rows in.  Positions that a
-        window has given back are refused."""
+        and values ``[count][kv_heads][v_dim]`` at positions ``first ..`` (by default all that its next token can see: of
+        a part with a window the last ``window - 1``), in the model's dtype, read back from the pages whatever form they
+        keep rows in.  Positions whose page a window has given back are refused."""
         v = self.view(entry, part)
         if not isinstance(v, KvView):
             raise ValueError(f"schedule entry {entry} has no one part that keeps keys and values; name it")
         if not self.manager.is_open(slot):
             raise ValueError(f"slot {slot} is not open")
         n = self.length(slot)
+        seen = max(0, n - v.window + 1) if v.window else 0
+        kept = seen // self.page_size * self.page_size
+        first = seen if first is None else first
         count = n - first if count is None else count
-        kept = max(0, n - v.window) if v.window else 0
         if first < kept or count < 0 or first + count > n:
             raise ValueError(f"slot {slot} holds positions {kept}..{n - 1}, not {first}..{first + count - 1}")
         self.sync_tables()

@@ -925,3 +925,36 @@ def test_prompts_take_no_memory_that_was_not_there(model_folders, monkeypatch):
         took = any(k.startswith("q4_plan") for k in e.rt._buffers)
         assert took == (dtype == "bfloat16"), "the prompts should have been read back in the bfloat16 model"
         assert {k: v.data_ptr() for k, v in e.rt._buffers.items() if k.startswith("q4_prompt_pages")} == held
+
+
+@pytest.mark.parametrize("bits", [0, 4])
+@pytest.mark.parametrize("window,n", [(17, 50), (17, 48), (17, 40), (1, 24), (1, 25), (64, 50), (9, 8), (9, 9)])
+def test_reading_a_part_with_a_window(ops, bits, window, n):
+    """By default what the next token can see; whatever lies in pages that are still held on demand, and nothing given back."""
+    from axon_b200.cache.manager import PagedCache
+    from axon_b200.parts.spec import KvNeed
+    ps, kv_heads, hd = 8, 2, 32
+    cache = PagedCache([{"mixer": KvNeed(kv_heads, hd, window=window, bits=bits)}], torch.float32, DEV, page_size=ps, max_tokens=128, max_slots=2,
+                       max_positions=64, shuffle_seed=3)
+    slot, other = cache.open(), cache.open()
+    qkv = torch.randn(n, 3 * kv_heads * hd, generator=torch.Generator().manual_seed(n)).to(DEV)
+    kv = qkv.view(n, 3, kv_heads, hd)[:, 1:].cpu().numpy()
+    want = q4.values(*q4.quantise(kv)) if bits else kv.astype(np.float64)
+    fill = torch.full_like(qkv, 9.0)
+    for at in range(n):                       # token by token; another request takes the pages that are given back
+        for s, rows in ((slot, qkv), (other, fill)):
+            assert cache.reserve(s, at + 1)
+            cache.sync_tables()
+            ops.rope_kv_write(rows[at:at + 1], None, i32([at]), i32([s]), torch.empty(1, kv_heads * hd, device=DEV), cache.view(0), kv_heads, 0)
+            cache.commit(s, at + 1)
+            cache.flush()
+    seen = max(0, n - window + 1)
+    held = seen // ps * ps
+    k, v = cache.read(slot, 0)
+    assert k.shape[0] == n - seen and k.dtype == torch.float32
+    for first in range(held, n + 1):
+        k, v = cache.read(slot, 0, first=first)
+        assert (k.double().cpu().numpy() == want[first:, 0]).all() and (v.double().cpu().numpy() == want[first:, 1]).all()
+    for first in range(-1, held):
+        with pytest.raises(ValueError, match="holds positions"):
+            cache.read(slot, 0, first=first, count=1)
