@@ -478,6 +478,11 @@ def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: 
     if got is not None:
         return got
     n_seg = len(ctx.seg_q_len)
+    if ctx.segments.dtype != torch.int32 or not ctx.segments.is_cuda or not ctx.segments.is_contiguous() or ctx.segments.numel() != 4 * n_seg:
+        raise ValueError(f"attention takes the step's segments as contiguous int32 [4, {n_seg}] on the device, not "
+                         f"{ctx.segments.dtype} {list(ctx.segments.shape)} on {ctx.segments.device}")
+    if any(q < 0 or q > kv for q, kv in zip(ctx.seg_q_len, ctx.seg_kv_len)) or sum(ctx.seg_q_len) > ctx.n_tokens:
+        raise ValueError(f"segments of {ctx.seg_q_len} tokens do not fit requests of {ctx.seg_kv_len} positions and {ctx.n_tokens} tokens")
     long = set(_q4_long(ctx, group, kv_heads, hd, window, takes_short))
     short = [s for s in range(n_seg) if s not in long and ctx.seg_q_len[s] > 0]
     launches = []

@@ -958,3 +958,33 @@ def test_reading_a_part_with_a_window(ops, bits, window, n):
     for first in range(-1, held):
         with pytest.raises(ValueError, match="holds positions"):
             cache.read(slot, 0, first=first, count=1)
+
+
+def test_attention_refuses_operands_that_it_would_read_past(ops):
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import Runtime, StepContext
+    cache = Cache(ops, [20, 30], 2, 64, 16)
+    q, pos, slot = torch.zeros(2, 4 * 64, device=DEV), i32([19, 29]), i32([0, 1])
+    out = torch.full_like(q, -7.0)
+    for bad in ((pos.long(), slot), (pos, slot.long()), (pos[:1].contiguous(), slot), (pos, slot[:1].contiguous())):
+        with pytest.raises(ValueError, match="position and slot"):
+            ops.attention_plain(q, cache.view, *bad, out, 4, 0.1)
+    scratch, arrived = torch.zeros(4096, device=DEV), torch.zeros(64, dtype=torch.int32, device=DEV)
+    for shares in (ops.KeyShares(2, scratch.double(), arrived), ops.KeyShares(2, scratch, arrived.long()), ops.KeyShares(2, scratch), ops.KeyShares(2, None, arrived)):
+        with pytest.raises(ValueError, match="scratch and int32 counters"):
+            ops.attention_plain(q, cache.view, pos, slot, out, 4, 0.1, shares=shares)
+    with pytest.raises(ValueError, match="contiguous CUDA"):
+        ops.attention_plain(q, cache.view, pos, slot, out, 4, 0.1, shares=ops.KeyShares(2, scratch.cpu(), arrived))
+    assert (out == -7.0).all()
+    seg = [[0, 1], [0, 1], [1, 1], [20, 30]]
+    good = dict(rt=Runtime(torch.bfloat16, DEV, kv_bits=4), n_tokens=2, tokens=None, positions=pos, token_slot=slot, seg_slot=seg[0], seg_q_start=seg[1],
+                seg_q_len=seg[2], seg_kv_len=seg[3], segments=i32(seg))
+    qb, ob = q.bfloat16(), torch.full_like(q, -7.0, dtype=torch.bfloat16)
+    for change, what in ((dict(segments=i32(seg).long()), "int64"), (dict(segments=i32(seg)[:3].contiguous()), r"\[3, 2\]"),
+                         (dict(segments=i32(seg).cpu()), "on cpu"), (dict(segments=i32(seg).T.contiguous().T), "contiguous"),
+                         (dict(seg_q_len=[1, 31]), "do not fit"), (dict(seg_q_len=[1, 2]), "do not fit")):
+        with pytest.raises(ValueError, match=what):
+            linear.attention(qb, cache.view, StepContext(**{**good, **change}), ob, 4, 0.1)
+    assert (ob == -7.0).all()
+    linear.attention(qb, cache.view, StepContext(**good), ob, 4, 0.1)
+    assert torch.isfinite(ob).all() and (ob != -7.0).any()
