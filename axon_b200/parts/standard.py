@@ -151,7 +151,7 @@ class Attention(Mixer):
         """The split count of the decode-shape attention, which follows the longest context among
         the segments short enough for that shape (every segment, in a step of single tokens)."""
         from ..kernels import fast
-        if self.rt.kv_bits:
+        if self.rt.kv_bits in self.kv_bits:
             return fast.q4_graph_key(ctx, self.heads, self.kv_heads, self.head_dim, self.window, self.rt.precise)
         if self.rt.precise:
             return ()

@@ -221,3 +221,23 @@ def test_memory_that_prompts_are_read_back_into():
     assert each[0] == pages * 64 * 2 * 4 * 128 * 2 + 4 * ints and quantised_workspace_bytes(needs, 16, 4096) == sum(each)
     assert quantised_workspace_bytes(needs, 16, 4096, torch.float32) == 0
     assert quantised_workspace_bytes([{"x": KvNeed(1, 256, bits=4)}], 16, 4096) == 0
+
+
+def test_an_attention_that_keeps_the_models_dtype_keys_its_steps_by_its_split_count():
+    """A part that does not take the 4-bit format launches the kernels of whole elements beside parts that do."""
+    from types import SimpleNamespace
+    from axon_b200.parts.standard import Attention
+
+    class Whole(Attention):
+        kv_bits = ()
+
+    keys = {}
+    for cls in (Attention, Whole):
+        part = object.__new__(cls)
+        part.rt = SimpleNamespace(kv_bits=4, precise=False, kv_page_size=16)
+        part.heads, part.kv_heads, part.head_dim, part.window = 28, 4, 128, 0
+        for kv in (100, 30000):
+            ctx = SimpleNamespace(rt=part.rt, seg_q_len=[1], seg_kv_len=[kv], n_tokens=1, max_q_len=1, max_kv_len=kv, scratch={})
+            keys[cls, kv] = part.graph_key(ctx)
+    assert keys[Attention, 100] == keys[Attention, 30000] == ()
+    assert keys[Whole, 100] != keys[Whole, 30000]
