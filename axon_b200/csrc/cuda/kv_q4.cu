@@ -223,8 +223,11 @@ __device__ __forceinline__ void q4_store8<__nv_bfloat16>(__nv_bfloat16* dst, uin
 
 constexpr int Q4_READ_ROWS = 32, Q4_READ_THREADS = 256, Q4_READ_BATCH = 4;      // (threads: for one plane, or half for each of two)
 // Writes a CTA's rows r0 .. once `rec` (a row's record of kv head 0; -1: not written, -2: zeros) and `at` (its place in
-// the page) are known.
-template <typename T>
+// the page) are known.  ATTEND (both planes, of one width): rows for an attention that multiplies values with weights of zero
+// where a token does not see them.  Values of a group that is not finite become zeros, and the same channels of their key NaN
+// instead: a score that a mask hides is hidden whatever it is, so such a value reaches the tokens that see it (all
+// channels of the head) and no others.
+template <typename T, bool ATTEND>
 __device__ __forceinline__ void q4_read_rows(const uint8_t* __restrict__ pool, const PagedQ4& kv, const long long* rec, const int* at,
                                              long long r0, int rows_per_cta, const Q4Out& out) {
     // with both planes to write the first half of the threads takes keys, the second values
@@ -232,7 +235,7 @@ __device__ __forceinline__ void q4_read_rows(const uint8_t* __restrict__ pool, c
     const int threads = both ? Q4_READ_THREADS / 2 : Q4_READ_THREADS, tid = both ? threadIdx.x % (Q4_READ_THREADS / 2) : threadIdx.x;
     T* const base = (T*)(is_v ? out.v : out.k);
     const int words = (is_v ? kv.vd : kv.hd) / 8, codes = is_v ? kv.v_codes : 0, steps = is_v ? kv.v_steps : kv.k_steps;
-    const int r_step = max(threads / words, 1);
+    const int r_step = max(threads / words, 1), to_value = is_v ? 0 : kv.v_steps - kv.k_steps;
     for (int i = tid; i < (threads / words > 0 ? r_step * words : words); i += threads) {      // (a row of more words than threads: several of them)
         const int w = i % words;
         constexpr int ROWS = 2;                                // a thread's rows whose loads are in flight together
@@ -253,14 +256,20 @@ __device__ __forceinline__ void q4_read_rows(const uint8_t* __restrict__ pool, c
             }
             auto batch = [&](auto n) {                         // `n` heads
                 uint32_t word[ROWS][decltype(n)::value];
-                int byte[ROWS][decltype(n)::value];
+                int byte[ROWS][decltype(n)::value], of_value[ROWS][decltype(n)::value];
 #pragma unroll
                 for (int q = 0; q < ROWS; ++q)
 #pragma unroll
                     for (int k = 0; k < decltype(n)::value; ++k) {
                         word[q][k] = *reinterpret_cast<const uint32_t*>(word_at[q] + k * kv.record);
                         byte[q][k] = step_at[q][k * kv.record];
+                        if (ATTEND) of_value[q][k] = step_at[q][k * kv.record + to_value];
                     }
+#pragma unroll
+                for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+                    for (int k = 0; k < decltype(n)::value; ++k)
+                        if (ATTEND && of_value[q][k] == Q4_NAN) byte[q][k] = is_v ? 0 : Q4_NAN;
 #pragma unroll
                 for (int q = 0; q < ROWS; ++q) {
                     if (where[q] != -1) {
@@ -315,7 +324,7 @@ kv_read_q4_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int32_t* _
         at[threadIdx.x] = in_page;
     }
     __syncthreads();
-    q4_read_rows<T>(pool, kv, rec, at, r0, rows_per_cta, out);
+    q4_read_rows<T, false>(pool, kv, rec, at, r0, rows_per_cta, out);
 }
 
 // Keys and values of whole prompts for the attention that takes bfloat16 pages: of each of the n_long segments named in `which`
@@ -379,7 +388,7 @@ kv_read_q4_pages_kernel(const uint8_t* __restrict__ pool, PagedQ4 kv, const int3
         at[threadIdx.x] = held ? pos - lp * kv.page_size : 0;
     }
     __syncthreads();
-    q4_read_rows<T>(pool, kv, rec, at, r0, Q4_READ_ROWS, out);
+    q4_read_rows<T, true>(pool, kv, rec, at, r0, Q4_READ_ROWS, out);
 }
 
 // ---------------------------------------------------------------------------

@@ -988,3 +988,29 @@ def test_attention_refuses_operands_that_it_would_read_past(ops):
     assert (ob == -7.0).all()
     linear.attention(qb, cache.view, StepContext(**good), ob, 4, 0.1)
     assert torch.isfinite(ob).all() and (ob != -7.0).any()
+
+
+@pytest.mark.parametrize("way", ["read back", "4-bit"])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(14, 2, 128), (6, 2, 64), (6, 2, 32)])
+@pytest.mark.parametrize("window", [0, 60])
+def test_what_is_not_finite_in_a_prompt_stays_with_who_sees_it(ops, monkeypatch, way, heads, kv_heads, hd, window):
+    """A NaN key or value anywhere in a prompt, or before a portion: tokens that do not see it have the bits they have without it,
+    whichever way the portion takes; those that see it have NaN in its channels, and no other head has any."""
+    if way == "4-bit" and hd == 32:
+        return
+    force(monkeypatch, way)
+    group = heads // kv_heads
+    for total, q_len in ((300, 300), (300, 130)):
+        for at in (0, 63, 64, 200, 255, 299):
+            for part in (1, 3):
+                cache = Cache(ops, [total, 70], kv_heads, hd, 16, window=window, seed=35)
+                clean = attend(ops, cache, [q_len, 70], heads, torch.bfloat16)[0].clone().view(-1, heads, hd)
+                page, i = int(cache.table[0, at // 16]), at % 16
+                cache.pool[page, 1, cache.record + cache.places[part][0] + i * cache.places[part][1]] = 0xFF       # kv head 1, its first group
+                out = attend(ops, cache, [q_len, 70], heads, torch.bfloat16)[0].view(-1, heads, hd)
+                pos = torch.arange(total - q_len, total, device=DEV)
+                sees = (pos >= at) & ((pos - at < window) if window else True)
+                assert torch.equal(out[q_len:], clean[q_len:]), "another request"
+                assert torch.equal(out[:q_len, :group], clean[:q_len, :group]), "another kv head"
+                assert torch.equal(out[:q_len][~sees], clean[:q_len][~sees]), f"a token that does not see position {at}"
+                assert torch.isnan(out[:q_len][sees][:, group:, :16]).all(), f"a token that sees position {at}"
