@@ -14,7 +14,8 @@
 //   * O^T = V^T P^T contracts over keys: pairs of keys are put side by side by two byte permutations per pair
 //     of words, then widened the same way; P^T is the transpose (movmatrix) of the scores' own registers.
 // Halves rather than bfloat16 because the weights P then keep 11 bits; queries are scaled by a power of two
-// per row to the range of halves (exact, but for elements 2^-24 below the row's largest).
+// per row, their largest element into [1, 2): exact down to elements of 2^-17 there, whose eight bits end at the 2^-24 that subnormal
+// halves count in, and off by 2^-25 at most below.
 //
 // A warp works alone: its own ring of shared memory, filled by asynchronous copies of 16 bytes (with pages of 16
 // positions a kv head's codes and steps of keys and values are one run of 18 HD bytes), its own running

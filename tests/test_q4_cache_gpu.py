@@ -740,7 +740,7 @@ def random_pages(ops, positions, kv_heads, hd, seed, ps=16):
     return view, k, v
 
 
-def check_rows(out, q, k, v, rows, first, heads, scale, weight_half):
+def check_rows(out, q, k, v, rows, first, heads, scale, weight_half, window=0):
     """Some rows of a portion whose first token is at position ``first``, against float64 on the device, within
     ``check_attention``'s bound and what 4-bit attention's half-precision queries may lose: rows are scaled to the largest element
     in [1, 2), where halves are off by 2^-25 at most below 2^-14 and hold a bfloat16 element's eight bits above 2^-17."""
@@ -750,13 +750,15 @@ def check_rows(out, q, k, v, rows, first, heads, scale, weight_half):
         kd, vd = k[:, h].double(), v[:, h].double()
         for r in rows:
             n = first + r + 1
+            lo = max(0, n - window) if window else 0
+            kr, vr = kd[lo:n], vd[lo:n]
             qr = q[r].view(heads, hd)[h * group:(h + 1) * group].double()
-            s = qr @ kd[:n].T * scale
+            s = qr @ kr.T * scale
             w = torch.softmax(s, -1)
-            want, mass = w @ vd[:n], w @ vd[:n].abs()
-            e_s = ((qr.abs() @ kd[:n].abs().T).amax(-1) * ((hd + 4) * 2.0 ** -23 + 2.0 ** -22) +
-                   qr.abs().amax(-1) * 2.0 ** -25 * kd[:n].abs().sum(-1).amax()) * abs(scale)
-            tol = (2.0 ** -25 * vd[:n].abs().sum(0) + mass * (weight_half + 2 * e_s[:, None] + 2.0 ** -20 + (n + 8) * 2.0 ** -23) +
+            want, mass = w @ vr, w @ vr.abs()
+            e_s = ((qr.abs() @ kr.abs().T).amax(-1) * ((hd + 4) * 2.0 ** -23 + 2.0 ** -22) +
+                   qr.abs().amax(-1) * 2.0 ** -25 * kr.abs().sum(-1).amax()) * abs(scale)
+            tol = (2.0 ** -25 * vr.abs().sum(0) + mass * (weight_half + 2 * e_s[:, None] + 2.0 ** -20 + (n + 8) * 2.0 ** -23) +
                    1.01 * 2.0 ** -8 * want.abs() + 1e-30)
             err = (out[r].view(heads, hd)[h * group:(h + 1) * group].double() - want).abs()
             assert bool((err <= tol).all()), f"token {r}, kv head {h}: {float((err / tol).max()):.2f} of its bound"
@@ -1014,3 +1016,52 @@ def test_what_is_not_finite_in_a_prompt_stays_with_who_sees_it(ops, monkeypatch,
                 assert torch.equal(out[:q_len, :group], clean[:q_len, :group]), "another kv head"
                 assert torch.equal(out[:q_len][~sees], clean[:q_len][~sees]), f"a token that does not see position {at}"
                 assert torch.isnan(out[:q_len][sees][:, group:, :16]).all(), f"a token that sees position {at}"
+
+
+# -- the 4-bit kernel's own bound -------------------------------------------
+
+def check_tight(ops, cache, q_lens, heads, window=0, **kw):
+    """Every token against float64 with weights of eleven bits, which the 4-bit kernel's are and bfloat16's are not."""
+    out, _, q, pos, slot, scale = attend(ops, cache, q_lens, heads, torch.bfloat16, window, **kw)
+    at = 0
+    for s, n in enumerate(q_lens):
+        if n:
+            k, v = torch.from_numpy(cache.k[s]).to(DEV), torch.from_numpy(cache.v[s]).to(DEV)
+            check_rows(out[at:at + n], q[at:at + n], k, v, range(n), cache.lens[s] - n, heads, scale, 2.0 ** -11, window)
+        at += n
+
+
+TIGHT = [l for l in LAYOUTS if l[2] in (64, 128, 256) and l[3] % max(1, 256 // l[2]) == 0]
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,ps", TIGHT)
+@pytest.mark.parametrize("window", [0, 19])
+def test_portions_keep_eleven_bits_of_weights(ops, monkeypatch, heads, kv_heads, hd, ps, window):
+    """One, two and four row tiles, with and without a work list; peaked and flat weights."""
+    force(monkeypatch, "4-bit")
+    cache = Cache(ops, [2, 40, 5, 64, 81, 33], kv_heads, hd, ps, window=window, seed=42)
+    for q_lens in ([1, 1, 1, 1, 1, 1], [2, 2, 0, 2, 1, 2], [1, 4, 0, 3, 4, 2], [2, 3, 0, 9, 1, 33]):
+        for scale in (None, 1.0):
+            check_tight(ops, cache, q_lens, heads, window, scale=scale)
+
+
+def test_more_portions_keep_eleven_bits_of_weights(ops):
+    rng = np.random.default_rng(7)
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(900), 75))]
+    for hd, heads, kv_heads in ((128, 6, 2), (64, 4, 4)):
+        check_tight(ops, Cache(ops, lens, kv_heads, hd, 16, seed=43), [min(l, 1 + i % 5) for i, l in enumerate(lens)], heads)
+    for scale in (-0.2, 0.0, 3.0):
+        check_tight(ops, Cache(ops, [70, 300], 2, 128, 16, seed=44), [1, 4], 6, scale=scale)
+    check_tight(ops, Cache(ops, [5003], 4, 128, 16, seed=45, loud=1.0), [4], 28)
+    check_tight(ops, Cache(ops, [5003], 4, 128, 16, seed=45, loud=1.0, window=1000), [4], 28, 1000)
+
+
+def test_queries_that_span_many_powers_of_two(ops):
+    """A row's largest element against others down to 2^-30 of it, where halves no longer hold them exactly."""
+    heads, hd = 6, 128
+    cache = Cache(ops, [90, 33], 2, hd, 16, seed=46)
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(3, heads * hd, generator=g) * torch.exp2(-30.0 * torch.rand(3, heads * hd, generator=g))
+    q.view(3, heads, hd)[:, :, 5] = 1.9
+    for size in (1.0, 2.0 ** -100, 2.0 ** 60):
+        check_tight(ops, cache, [2, 1], heads, q=(q * size).bfloat16().to(DEV), scale=0.5 / size)
