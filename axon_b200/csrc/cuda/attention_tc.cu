@@ -451,6 +451,7 @@ AXON_API int axon_attention_tc(const void* q, const void* pool, void* out, const
     if (tokens_per_tile < 1 || tokens_per_tile * group > AT_SUB * AT_BM) { set_error("axon_attention_tc: %d tokens x %d heads do not fit %d rows", tokens_per_tile, group, AT_SUB * AT_BM); return AXON_BAD_ARGUMENT; }
     if (((uintptr_t)q | (uintptr_t)pool | (uintptr_t)out) & 15) { set_error("axon_attention_tc: operands must be 16-byte aligned"); return AXON_BAD_ARGUMENT; }
     if (items == nullptr) { set_error("axon_attention_tc: needs a work list"); return AXON_BAD_ARGUMENT; }
+    if (!(scale > 0.f)) { set_error("axon_attention_tc: the scale has to be positive, not %g", (double)scale); return AXON_BAD_ARGUMENT; }
     if (layout->planes == 1 || (layout->v_dim > 0 && layout->v_dim != AT_HD)) { set_error("axon_attention_tc: takes caches with key and value planes of one width"); return AXON_BAD_ARGUMENT; }
     AtParams p;
     p.q = (const __nv_bfloat16*)q; p.pool = (const __nv_bfloat16*)pool; p.out = (__nv_bfloat16*)out;

@@ -313,6 +313,11 @@ def attention_decode_fused(qkv, pending, table, rot: int, adjacent: bool, kv, ct
     return True
 
 
+def _takes_tc(head_dim: int, scale: float) -> bool:
+    """Whether prompts take the tcgen05 attention, which finds a row's largest score before it scales it."""
+    return ENABLED["attention_tc"] and head_dim == 128 and scale > 0
+
+
 def attention(q, kv, ctx, out, heads: int, scale: float) -> bool:
     """Tensor-core attention over the paged cache; refuses head sizes other than
     16/32/64/128, groups of more than 64 heads, and dtypes other than bfloat16."""
@@ -328,7 +333,7 @@ def attention(q, kv, ctx, out, heads: int, scale: float) -> bool:
         return False
     group = heads // kv.kv_heads
     # prompt portions at head size 128 take the tcgen05 kernel with tiles of 256 rows (two sub-tiles of 128)
-    use_tc = ENABLED["attention_tc"] and kv.head_dim == 128 and ctx.unit_items is None
+    use_tc = _takes_tc(kv.head_dim, scale) and ctx.unit_items is None
     it = _attention_items(ctx, group, 256 if use_tc else 64)
     cu = lib.cuda()
     n_seg = len(ctx.seg_slot)
@@ -407,7 +412,8 @@ Q4_LONG_KEY = {128: (0.022, SM_COUNT), 64: (0.031, 3 * SM_COUNT)}
 
 def _q4_long(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: bool):
     """The segments that attend over keys and values read back into bfloat16 pages, because that is modelled to be
-    faster than the 4-bit kernel, which widens the keys anew for every 32 query rows.  Without ``takes_short`` (the 4-bit kernel
+    faster than the 4-bit kernel, which widens the keys anew for every 32 query rows.  Decided for all segments of more than a few
+    rows together, not one by one: a prompt beside a few tokens at a much longer context can go the slower way.  Without ``takes_short`` (the 4-bit kernel
     refuses the sizes): all of them if any has more than a few rows, else none."""
     if hd not in FA_HEAD_DIMS or ctx.max_q_len * group <= Q4_SHORT_ROWS:
         return ()
@@ -470,10 +476,10 @@ def _q4_prompt_sizes(ctx, segs, window: int):
     return _q4_bucket(sum(n)), _q4_bucket(max(n))
 
 
-def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: bool):
+def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: bool, use_tc: bool):
     """The step's work for the 4-bit attention, cached per step: launches of the 4-bit kernel (row tiles, items, list or None,
     scratch, its floats), and groups of segments whose keys are read back."""
-    key = ("q4_work", group, kv_heads, hd, window, takes_short)
+    key = ("q4_work", group, kv_heads, hd, window, takes_short, use_tc)
     got = ctx.scratch.get(key)
     if got is not None:
         return got
@@ -518,7 +524,7 @@ def _q4_work(ctx, group: int, kv_heads: int, hd: int, window: int, takes_short: 
     plans = []
     for k, segs in enumerate(groups):
         pages, stride = _q4_prompt_sizes(ctx, segs, window)
-        rows = 256 if hd == 128 and ENABLED["attention_tc"] else 64
+        rows = 256 if use_tc else 64
         tpt = rows // group
         work = [(ctx.seg_kv_len[s] - ctx.seg_q_len[s] + min(t0 + tpt, ctx.seg_q_len[s]), i, t0)
                 for i, s in enumerate(segs) for t0 in range(0, ctx.seg_q_len[s], tpt)]
@@ -562,7 +568,7 @@ def attention_q4(q, kv, ctx, out, heads: int, scale: float) -> bool:
     takes_short = _q4_takes(hd, kv.page_size)
     if not takes_short and not _q4_long(ctx, group, kv.kv_heads, hd, kv.window, False):
         return False
-    launches, plans = _q4_work(ctx, group, kv.kv_heads, hd, kv.window, takes_short)
+    launches, plans = _q4_work(ctx, group, kv.kv_heads, hd, kv.window, takes_short, _takes_tc(hd, scale))
     cu = lib.cuda()
     for nt, n_items, which, scratch, floats, _held in launches:
         check(cu.axon_attention_q4(q.data_ptr(), kv.pool.data_ptr(), out.data_ptr(), ctx.segments.data_ptr(), len(ctx.seg_q_len),

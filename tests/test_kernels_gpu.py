@@ -1034,3 +1034,21 @@ def test_decode_attention_waits_for_lists_just_written(ops, heads, kv_heads, hd,
     other = torch.zeros_like(table)
     late_view = ops.KvView(view.pool, other, 1, 16, kv_heads, hd)
     assert torch.equal(step(i32(segments), late_view, False, (table, other)), want), "the block table was read too early"
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_prompt_attention_at_scales_that_are_not_positive(ops, scale):
+    """At head size 128, where the tcgen05 kernel takes positive scales only."""
+    from axon_b200.kernels import fast
+    heads, kv_heads, hd, n = 14, 2, 128, 300
+    view, table = make_cache(ops, torch.bfloat16, kv_heads, hd, 16, 40, 1, 320, seed=23)
+    view.pool.copy_(rand(*view.pool.shape, dtype=torch.bfloat16, seed=150))
+    q = rand(n, heads * hd, dtype=torch.bfloat16, seed=151, std=0.3)
+    out = torch.full((n, heads * hd), float("nan"), dtype=torch.bfloat16, device=DEV)
+    assert fast.attention(q, view, _ctx_for([(0, n, n)]), out, heads, scale)
+    at = torch.arange(n, device=DEV)
+    pages = table[0, at // 16].long()
+    k, v = (x[pages, :, at % 16].double().transpose(0, 1).repeat_interleave(heads // kv_heads, 0) for x in (view.keys(), view.values()))
+    s = q.double().view(n, heads, hd).transpose(0, 1) @ k.transpose(1, 2) * scale
+    s.masked_fill_(at[None, :] > at[:, None], -math.inf)
+    close(out.view(n, heads, hd).transpose(0, 1), torch.softmax(s, -1) @ v, OUT_TOL[torch.bfloat16], f"scale {scale}")

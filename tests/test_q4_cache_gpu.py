@@ -1065,3 +1065,13 @@ def test_queries_that_span_many_powers_of_two(ops):
     q.view(3, heads, hd)[:, :, 5] = 1.9
     for size in (1.0, 2.0 ** -100, 2.0 ** 60):
         check_tight(ops, cache, [2, 1], heads, q=(q * size).bfloat16().to(DEV), scale=0.5 / size)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,ps", [(14, 2, 128, 16), (8, 1, 128, 1), (6, 2, 64, 32), (3, 1, 32, 16), (5, 5, 48, 16)])
+@pytest.mark.parametrize("scale", [0.0, -0.2, -0.0])
+@pytest.mark.parametrize("window", [0, 60])
+def test_prompts_at_scales_that_are_not_positive(ops, monkeypatch, heads, kv_heads, hd, ps, scale, window):
+    """Whichever way their length would send them.  Rows read back meet weights of bfloat16, off by 2^-8 at most."""
+    force(monkeypatch, "read back")
+    cache = Cache(ops, [300, 3, 90], kv_heads, hd, ps, window=window, seed=47)
+    check_attention(ops, cache, [300, 1, 40], heads, torch.bfloat16, window, weight_half=2.0 ** -8, scale=scale)
