@@ -20,8 +20,8 @@
 // A warp works alone: its own ring of shared memory, filled by asynchronous copies of 16 bytes (with pages of 16
 // positions a kv head's codes and steps of keys and values are one run of 18 HD bytes), its own running
 // maximum and sum.  The maximum lags: O is rescaled only when a score exceeds it by 2^8.  The warps of a CTA take
-// tiles of 16 keys in turn and are merged at the end.  (Bulk copies counted by mbarriers were measured first: a
-// copy's uniform operands cost the issuing warp some 30 instructions, these 5 a tile.)
+// tiles of 16 keys in turn and are merged at the end.  (Bulk copies counted by mbarriers were measured first: with them, and
+// pieces folded by a second kernel, 64 ragged requests took 62 us where 54 were reached without.)
 //
 // The grid is as many CTAs as fit at once, and the 16-key tiles of all (item, kv head) pairs, laid
 // end to end, are cut into one equal range for each: contexts of any lengths load the GPU evenly, and
@@ -30,9 +30,10 @@
 // of the others go to scratch (at most two per CTA: the one its range begins in and the one it ends in), and the
 // CTA whose piece arrives last folds them in ascending order, so results do not depend on the order of arrival.
 //
-// Measured on a B200 (28 query and 4 kv heads of 128): 64 requests of 300 to 8,192 positions, 157 MB, 43 us = 3.65 TB/s,
-// 0.56 of the measured copy rate; 8 of 32,768 39 us (0.59); 8 of 2,048 7.8 us; one of 519 5.3 us.  The loop alone runs
-// at 0.8 of the copy rate, issuing 54 % of the time; the rest is the chain at both ends of a launch.
+// Measured on a B200 (28 query and 4 kv heads of 128, staged steps in a graph): 64 requests of 300 to 8,192 positions, 157 MB,
+// 43.7 us = 3.6 TB/s, 0.55 of the measured copy rate; 8 of 32,768 39.1 us (0.59); 8 of 2,048 8.5 us; one of 519 6.0 us.  Of the
+// ragged requests' cycles 55 % issue, at 364 instructions a tile; what warps wait for otherwise is fixed latencies and memory, in
+// equal parts.
 #include "kv_q4.cuh"
 
 #include <type_traits>
@@ -40,11 +41,11 @@
 namespace axon {
 
 constexpr int QA_WARPS = 8, QA_THREADS = QA_WARPS * 32;
-// Tiles in a warp's ring (8 requests of 32,768 positions: 40.7 us; four 42.9; two times two tiles 41.6)
+// Tiles in a warp's ring (8 requests of 32,768 positions: 39.1 us; two 38.7; four 40.6)
 constexpr int QA_STAGES = 3;
 // A pair counts as its tiles and so many more when ranges are cut: what starting on it and merging the warps'
-// results cost the CTA, in tiles.  64 requests of 300 to 8,192 positions: 53.8 us with none (CTAs that met a dozen short
-// requests finished last), 51.9 with 8, 47.3 with 16, 45.9 with 24.
+// results cost the CTA, in tiles.  64 requests of 300 to 8,192 positions: 51.1 us with none (CTAs that met a dozen short
+// requests finished last), 48.5 with 8, 45.2 with 16, 43.7 with 24, 43.4 with 40.
 constexpr int QA_PAIR_COST = 24;
 constexpr int QA_LEAST = QA_WARPS;               // the shortest range: one tile for each warp
 constexpr float QA_LAZY = 8.f;                   // log2 units a score may exceed the running maximum
@@ -108,7 +109,8 @@ __device__ __forceinline__ uint32_t qa_mul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// (w & mask) | magic in one instruction: with both as constants the compiler takes two, as an instruction holds one.
+// (w & mask) | magic as one logic operation, `magic` in a register (as an expression of two constants: 49.1 us for the 64 ragged
+// requests, 44.0 so).
 template <uint32_t MASK> __device__ __forceinline__ uint32_t qa_pick(uint32_t w, uint32_t magic) {
     uint32_t r;
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(magic));
@@ -225,8 +227,8 @@ struct QaDivision {
     // the length of ranges that pairs are padded to
     __host__ __device__ __forceinline__ QaDivision(uint32_t tiles, uint32_t longest, uint32_t ctas) {
         // one CTA folds a pair's pieces (about 0.12 us each): with few long pairs, ranges as long as the fold of their
-        // number, which is about the square root of a pair's tiles (one request of 32,768 positions: 16.2 us; with 1.5 times
-        // as long ranges 17.7, twice 19.9, 0.7 times 15.9)
+        // number, which is about the square root of a pair's tiles (one request of 32,768 positions: 14.5 us; with 1.5 times
+        // as long ranges 15.3, twice 16.5, 0.7 times 13.6)
         least = (uint32_t)sqrtf((float)longest);
         least = least > (uint32_t)QA_LEAST ? least : (uint32_t)QA_LEAST;
         const uint32_t even = (tiles + ctas - 1) / ctas;
@@ -614,8 +616,8 @@ attention_q4_kernel(const QaParams p) {
             }
         }
     };
-    // Tiles that every row sees whole go through a loop of their own: joined with the masked code behind one
-    // branch, the compiler moved the accumulators from register to register every tile.
+    // Tiles that every row sees whole go through a loop of their own: it was faster than one loop with the masked
+    // code behind a branch.
     for (int tile = tile0 + warp, stage = 0;;) {
         auto take = [&](auto edge) {
             qa_copy_wait<QA_STAGES - 1>();
