@@ -203,7 +203,8 @@ def rope_kv_write(qkv: torch.Tensor, table: Optional[torch.Tensor], positions: t
                   adjacent: bool = False, write_kv: bool = True, pending=None, staged: bool = False) -> None:
     """Rotates queries and keys and writes queries to ``q_out``, keys and values to the cache (quantised
     when ``kv`` has 4 bits).  ``pending`` (a ``fast.PendingFold`` whose output is ``qkv``): the product is
-    still in partial sums; they are folded here (with the bias) and ``qkv`` itself is not read.  ``staged``:
+    still in partial sums; they are folded here (with the bias) and ``qkv`` itself is not read.  No two rows of a call may
+    name one position of one slot (what it then holds is a mixture of both).  ``staged``:
     positions, slots and the block table were there before the kernels in flight were launched
     (``StepContext.staged``), so that they may be read while the kernel before is still running."""
     if kv.bits:

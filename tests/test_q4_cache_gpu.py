@@ -1075,3 +1075,35 @@ def test_prompts_at_scales_that_are_not_positive(ops, monkeypatch, heads, kv_hea
     force(monkeypatch, "read back")
     cache = Cache(ops, [300, 3, 90], kv_heads, hd, ps, window=window, seed=47)
     check_attention(ops, cache, [300, 1, 40], heads, torch.bfloat16, window, weight_half=2.0 ** -8, scale=scale)
+
+
+@pytest.mark.parametrize("hd,ps", [(128, 16), (64, 16), (128, 1), (32, 16), (48, 16), (256, 16)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window", [0, 1])
+def test_calls_with_nothing_to_do(ops, hd, ps, dtype, window):
+    """No rows, no spans, no tokens; and segments without tokens, or without positions, beside others in one step."""
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import Runtime, StepContext
+    heads, kv_heads = 6, 2
+    cache = Cache(ops, [300, 64, 20, 40], kv_heads, hd, ps, window=window, seed=48)
+    before = cache.pool.clone()
+    none = i32([])
+    ops.rope_kv_write(torch.empty(0, (heads + 2 * kv_heads) * hd, device=DEV), None, none, none, torch.empty(0, heads * hd, dtype=dtype, device=DEV),
+                      cache.view, heads, 0)
+    keys = torch.full((3, kv_heads, hd), -5.0, device=DEV)
+    ops.kv_read(cache.view, torch.empty(4, 0, dtype=torch.int32, device=DEV), keys)
+    ops.kv_read(cache.view, i32([[0], [0], [3], [0]]), keys[:0])
+    assert (keys == -5.0).all() and torch.equal(cache.pool, before)
+    rt = Runtime(dtype, DEV, kv_bits=4)
+    empty = dict(rt=rt, n_tokens=0, tokens=None, positions=none, token_slot=none, seg_slot=[], seg_q_start=[], seg_q_len=[], seg_kv_len=[],
+                 segments=torch.empty(4, 0, dtype=torch.int32, device=DEV))
+    q = torch.empty(0, heads * hd, dtype=dtype, device=DEV)
+    linear.attention(q, cache.view, StepContext(**empty), torch.empty_like(q), heads, 0.1, precise=dtype == torch.float32)
+    for q_lens in ([300, 0, 0, 1], [1, 0, 0, 3], [200, 0, 0, 40]):
+        want, _, qs, pos, slot, scale = attend(ops, cache, q_lens, heads, dtype)
+        seg = [[0, 1, 2, 3], [0, q_lens[0], q_lens[0], q_lens[0]], q_lens, [300, 64, 0, 40]]
+        ctx = StepContext(rt=rt, n_tokens=len(pos), tokens=None, positions=i32(pos), token_slot=i32(slot), seg_slot=seg[0], seg_q_start=seg[1],
+                          seg_q_len=seg[2], seg_kv_len=seg[3], segments=i32(seg))
+        out = torch.full_like(want, float("nan"))
+        linear.attention(qs, cache.view, ctx, out, heads, scale, precise=dtype == torch.float32)
+        assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -6), q_lens
