@@ -112,7 +112,7 @@ rope_kv_write_q4_kernel(const float* __restrict__ qkv, const float2* __restrict_
 // The same for the common layout (pairs (i, i + hd / 2) over the whole head, hd % 32 == 0, keys and values of one
 // width, 16-byte aligned operands): a thread owns four channels of each half of a row, so that nothing is read twice
 // and the groups of both halves are again four neighbouring lanes.  2,048 tokens at 28 + 4 + 4 heads of 128 move
-// 57 MB in 12.2 us (0.71 of the measured copy rate); one token takes 1.9 us.
+// 57 MB in 12.3 us (0.71 of the measured copy rate), 12.9 where the step is not staged; one token takes 1.9 and 2.2 us.
 template <typename T>
 __device__ __forceinline__ void q4_store4(T* dst, const float (&x)[4]);
 template <>
