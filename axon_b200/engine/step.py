@@ -370,5 +370,6 @@ class Engine:
                 else:
                     self.cuda_graphs = False
         else:
+            self._graphs.clear()              # this very step moved a buffer that the captured ones read and write
             self._graph_generation = self.rt.generation
         return result

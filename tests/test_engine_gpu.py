@@ -651,3 +651,28 @@ def test_steps_queued_without_waiting_keep_their_own_tables(model_folders):
         torch.cuda.synchronize()
         outs[waited] = torch.cat(res)
     assert torch.equal(outs[True], outs[False])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_larger_step_drops_the_graphs_of_smaller_ones(model_folders, dtype):
+    """A step of more requests than any before grows the engine's buffers while it runs for its capture: steps captured earlier hold
+    the old addresses, which may be anyone's by then, and are not replayed."""
+    from axon_b200.engine.build import build_engine
+    from axon_b200.engine.step import StepEntry
+    toks = [tokens_for("C", i, 6) for i in range(5)]
+    got = []
+    for graphs in (True, False):
+        e = build_engine(model_folders["C"], dtype=dtype, max_slots=5, max_tokens=256, max_positions=64)
+        e.cuda_graphs = graphs
+        slots, fed, rows, others = [e.open_request() for _ in toks], [0] * 5, [], []
+        for who in ((0, 1), (0, 1), (0, 1, 2, 3, 4), (0, 1), (2, 3, 4), (0, 1), (0, 1, 2, 3)):
+            rows.append(e.step([StepEntry(slots[i], [toks[i][fed[i]]], [0]) for i in who]).clone())
+            for i in who:
+                fed[i] += 1
+            # whatever the engine has set free belongs to others from here on
+            others += [torch.full((n,), 7.0, device="cuda:0") for n in (64, 128, 256, 512, 1024, 2048, 4096, 8192) for _ in range(4)]
+            assert not graphs or len(who) != 5 or not e._graphs, "captured steps with old addresses are still there"
+        assert all(bool((x == 7.0).all()) for x in others), "a replayed step wrote into memory that is not the engine's"
+        got.append(rows)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
