@@ -109,9 +109,12 @@ class Engine:
         self._graph_generation = self.rt.generation
         #: steps run, for reports
         self.steps = 0
-        # the metadata buffer of eager steps at its largest from the start: a buffer that grows later
-        # moves, and every captured graph is dropped when any scratch buffer moves
+        # the metadata buffer of eager steps at its largest from the start, and what follows the number of
+        # requests at its largest for one logit row each: a buffer that grows later moves, and every captured
+        # graph is dropped when any scratch buffer moves
         self.rt.buffer("step_meta", (4 * max_step_tokens + 6 * cache.max_slots,), torch.int32)
+        self.rt.buffer("head_in", (cache.max_slots, model.spec.hidden_size))
+        self.rt.buffer("greedy_picks", (cache.max_slots,), torch.int32)
 
     # -- requests ---------------------------------------------------------
     def open_request(self) -> int:

@@ -266,10 +266,9 @@ def _decode_splits(n_dec: int, kv, tiles: int, rt):
     splits = _key_splits(n_dec * kv.kv_heads, tiles)
     scratch = None
     if splits > 1:
-        # sized for the most splits this batch can get, so that the buffer never moves
-        # while the contexts grow (captured graphs hold its address)
-        most = max(1, min(FA_MAX_SPLITS, FA_TARGET_CTAS // (n_dec * kv.kv_heads)))
-        scratch = rt.buffer("fa_scratch", (n_dec * kv.kv_heads * most * 16 * (kv.head_dim + 2),), torch.float32)
+        # sized for the most CTAs that any launch of several shares has, so that the buffer never moves
+        # while contexts grow or batches change (captured graphs hold its address)
+        scratch = rt.buffer("fa_scratch", (FA_TARGET_CTAS * 16 * (kv.head_dim + 2),), torch.float32)
     return splits, scratch
 
 

@@ -81,3 +81,13 @@ def test_the_rule_picks_the_faster_kernel_of_the_measured_chains():
                 got = model(kind, M, N, K, fast.SPLIT_TARGET_CTAS)
                 assert abs(got - seen) <= 0.4 * seen, (M, N, K, "swapped tiled".split()[kind], got, seen)
     assert picked <= 1.02 * best
+
+
+def test_scratch_of_key_shares_is_never_outgrown():
+    """One buffer for every batch and context: launches of several shares have no more CTAs than it is sized for."""
+    from axon_b200.kernels import fast
+    for kv_heads in (1, 2, 4, 8, 40):
+        for n in (1, 2, 7, 8, 36, 72, 74, 75, 148, 296, 300):
+            for tiles in (1, 2, 9, 33, 128, 512, 2048):
+                splits = fast._key_splits(n * kv_heads, tiles)
+                assert splits == 1 or n * kv_heads * splits <= fast.FA_TARGET_CTAS

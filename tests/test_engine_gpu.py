@@ -676,3 +676,20 @@ def test_a_larger_step_drops_the_graphs_of_smaller_ones(model_folders, dtype):
         got.append(rows)
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+def test_batches_of_any_size_keep_the_captured_steps(model_folders):
+    """Requests that come and go while contexts grow move no buffer once a prompt of the step's size has run."""
+    from axon_b200.engine.build import build_engine
+    from axon_b200.engine.step import StepEntry
+    e = build_engine(model_folders["C"], dtype="bfloat16", max_slots=12, max_tokens=4096, max_positions=1000, max_step_tokens=600)
+    slots = [e.open_request() for _ in range(12)]
+    e.step([StepEntry(slots[0], tokens_for("C", 0, 600), [599])])
+    generation, kept = e.rt.generation, {}
+    for n in (1, 12, 3, 8, 2, 5, 12, 1):
+        for _ in range(2):
+            e.step([StepEntry(s, [5], [0]) for s in slots[:n]])
+        e.step([StepEntry(slots[11 - i], tokens_for("C", i, 40), [39]) for i in range(n)], greedy=True)
+        assert all(e._graphs.get(k) is g for k, g in kept.items()), f"captured steps were dropped at {n} requests"
+        kept = dict(e._graphs)
+    assert e.rt.generation == generation and kept
