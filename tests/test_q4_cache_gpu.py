@@ -1107,3 +1107,65 @@ def test_calls_with_nothing_to_do(ops, hd, ps, dtype, window):
         out = torch.full_like(want, float("nan"))
         linear.attention(qs, cache.view, ctx, out, heads, scale, precise=dtype == torch.float32)
         assert torch.allclose(out.float(), want.float(), rtol=2.0 ** -6, atol=2.0 ** -6), q_lens
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("way", ["read back", "4-bit"])
+@pytest.mark.parametrize("heads,kv_heads,hd,window,pairing", [(4, 2, 16, None, "adjacent"), (8, 1, 128, 7, "half"), (6, 2, 64, 33, "adjacent"),
+                                                              (14, 2, 128, 40, "half"), (3, 3, 48, 1, "half")])
+def test_attention_part_over_a_quantised_cache(ops, monkeypatch, dtype, way, heads, kv_heads, hd, window, pairing):
+    """The mixer with its rotation, write and attention, in cuts, while a window gives pages back to another request: against
+    float64 attention over what the cache took."""
+    from axon_b200.cache import PagedCache
+    from axon_b200.parts import PartSpec, Runtime, part_class
+    from dataclasses import replace
+    import plain_qwen2 as plain
+    from test_parts_gpu import TOL, commit, make_ctx, rand
+    force(monkeypatch, way)
+    D, T, ps = 72, 150, 4
+    rt = Runtime(dtype, DEV, kv_bits=4)
+    spec = PartSpec("attention", {"hidden_size": D, "heads": heads, "kv_heads": kv_heads, "head_dim": hd, "qkv_bias": True, "out_bias": False,
+                                  "window": window, "scale": None}, {k: k for k in ("q", "k", "v", "o", "q_bias", "k_bias", "v_bias")},
+                    {"position": PartSpec("rope", {"head_dim": hd, "theta": 1e4, "pairing": pairing})})
+    cls = part_class("mixer", "attention")
+    w = {n: rand(*d.shape, seed=200 + i, std=0.3, dtype=torch.float32 if d.kind == "bias" else dtype) for i, (n, d) in enumerate(cls.tensors(spec).items())}
+    ref = {k: v.double().cpu() for k, v in w.items()}
+    mixer = cls(spec, dict(w), rt, lambda sub: part_class("position", sub.kind)(sub, {}, rt, None))
+    cache = PagedCache([replace(cls.cache_need(spec), bits=4)], dtype, DEV, page_size=ps, max_tokens=400, max_slots=2, max_positions=160, shuffle_seed=3)
+    rt.kv_page_size = ps
+    hs = [rand(T, D, seed=8 + r, dtype=dtype) for r in range(2)]
+    for cuts in ([T], [70, 1, 1, 30, 2, 40, 6], [1] * 9 + [141]):
+        slots = [cache.open(), cache.open()]
+        outs = [torch.zeros(T, D, device=DEV) for _ in slots]
+        held = [([], []) for _ in slots]
+        at = 0
+        for n in cuts:
+            cache.flush()
+            ctx = make_ctx(rt, cache, [(s, n) for s in slots])
+            xs = torch.zeros(2 * n, D, device=DEV)
+            mixer.forward(torch.cat([h[at:at + n] for h in hs]).contiguous(), xs, ctx, cache.view(0), True)
+            k, v = (torch.empty(2 * n, kv_heads, hd, dtype=dtype, device=DEV) for _ in range(2))
+            ops.kv_read(cache.view(0), i32([slots, [at, at], [n, n], [0, n]]), k, v)
+            commit(cache, ctx)
+            for r in range(2):
+                outs[r][at:at + n] = xs[r * n:(r + 1) * n]
+                held[r][0].append(k[r * n:(r + 1) * n].double().cpu())
+                held[r][1].append(v[r * n:(r + 1) * n].double().cpu())
+            at += n
+        for r in range(2):
+            q = plain.linear(hs[r].double().cpu(), ref["q"], ref["q_bias"]).view(T, heads, hd)
+            q = (plain.rope_half if pairing == "half" else plain_rope_adjacent)(q, range(T), 1e4)
+            o = plain.causal_gqa_attention(q, torch.cat(held[r][0]), torch.cat(held[r][1]), window=window)
+            want = plain.linear(o.reshape(T, heads * hd), ref["o"])
+            err = float((outs[r].double().cpu() - want).abs().max() / want.abs().max())
+            assert err <= TOL[dtype], f"request {r}, cuts {cuts}: {err:.2e}"
+            cache.close(slots[r])
+
+
+def plain_rope_adjacent(x, positions, theta):
+    """Rotation of pairs (2 i, 2 i + 1) in float64."""
+    half = x.shape[-1] // 2
+    ang = torch.tensor(list(positions), dtype=torch.float64)[:, None] * theta ** (-torch.arange(half, dtype=torch.float64) / half)[None]
+    c, s = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
+    a, b = x[..., 0::2], x[..., 1::2]
+    return torch.stack((a * c - b * s, a * s + b * c), -1).flatten(-2)
