@@ -27,6 +27,7 @@ checkpoint before anything is copied and so that random models can be written.
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import Any, Callable, ClassVar, Dict, List, Mapping, Optional, Tuple, Type, Union
 
@@ -78,8 +79,13 @@ class Runtime:
         return buf[:n].view(shape)
 
     def zeroed_buffer(self, name: str, shape: Tuple[int, ...], dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-        """A scratch buffer that is zero when it is first handed out (its users leave zero what must be)."""
+        """A scratch buffer that is zero when it is first handed out (its users leave zero what must be).  One that
+        would be made inside a graph capture is refused: it would be zeroed when the graph is replayed, and whoever
+        used it before that would find anything in it."""
         before = self._buffers.get(name)
+        fits = before is not None and before.dtype == (dtype or self.dtype) and before.numel() >= math.prod(shape)
+        if not fits and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"scratch '{name}' would be made and zeroed inside a graph capture: run the call once before it is captured")
         buf = self.buffer(name, shape, dtype)
         if self._buffers[name] is not before:
             self._buffers[name].zero_()

@@ -1169,3 +1169,34 @@ def plain_rope_adjacent(x, positions, theta):
     c, s = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
     a, b = x[..., 0::2], x[..., 1::2]
     return torch.stack((a * c - b * s, a * s + b * c), -1).flatten(-2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_capture_wants_the_call_to_have_run_once(ops, dtype):
+    """Counters that must be zero are not made inside a capture; after one eager call capture, replay and eager calls mix in any order."""
+    from axon_b200.kernels import linear
+    from axon_b200.parts.base import Runtime, StepContext
+    heads, kv_heads, hd = 14, 2, 128
+    cache = Cache(ops, [900, 33], kv_heads, hd, 16, seed=49)
+    want, _, q, pos, slot, scale = attend(ops, cache, [1, 1], heads, dtype)
+    want = want.clone()
+    ctx = StepContext(rt=Runtime(dtype, DEV, kv_bits=4), n_tokens=2, tokens=None, positions=i32(pos), token_slot=i32(slot), seg_slot=[0, 1],
+                      seg_q_start=[0, 1], seg_q_len=[1, 1], seg_kv_len=[900, 33], segments=i32([[0, 1], [0, 1], [1, 1], [900, 33]]))
+    out = torch.zeros_like(want)
+
+    def run():
+        ctx.scratch.clear()
+        linear.attention(q, cache.view, ctx, out, heads, scale, precise=dtype == torch.float32)
+
+    with pytest.raises(RuntimeError, match="before it is captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            run()
+    run()
+    assert torch.equal(out, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for call in (run, graph.replay, run, graph.replay, graph.replay):
+        out.zero_()
+        call()
+        assert torch.equal(out, want)
