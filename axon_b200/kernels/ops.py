@@ -292,16 +292,14 @@ def attention_plain(q: torch.Tensor, kv: KvView, positions: torch.Tensor, token_
     (4-bit caches only): into how many shares each token's keys are cut, with their scratch."""
     n = q.shape[0]
     if kv.bits:
-        quantised("attention_plain", kv, q, positions, token_slot, out)
+        x = shares or KeyShares()
+        quantised("attention_plain", kv, q, positions, token_slot, out, x.scratch, x.arrived)
         if out.dtype != q.dtype or out.numel() != n * heads * kv.v_dim or q.numel() != n * heads * kv.head_dim:
             raise ValueError("attention_plain takes queries [n][heads * head_dim] and writes [n][heads * v_dim] in their dtype")
         if positions.dtype != torch.int32 or token_slot.dtype != torch.int32 or positions.numel() < n or token_slot.numel() < n:
             raise ValueError("attention_plain takes an int32 position and slot for each row of queries")
-        x = shares or KeyShares()
-        if x.count > 1:
-            quantised("attention_plain", kv, x.scratch, x.arrived)
-            if x.scratch is None or x.scratch.dtype != torch.float32 or x.arrived is None or x.arrived.dtype != torch.int32:
-                raise ValueError("key shares come with float32 scratch and int32 counters")
+        if x.count > 1 and (x.scratch is None or x.scratch.dtype != torch.float32 or x.arrived is None or x.arrived.dtype != torch.int32):
+            raise ValueError("key shares come with float32 scratch and int32 counters")
         check(lib.cuda().axon_attention_q4_plain(_ptr(q), _ptr(kv.pool), dtype_code(q), _ptr(positions), _ptr(token_slot), _ptr(out),
                                                  kv._ref, n, heads, float(scale), int(kv.window), x.count, _ptr(x.scratch),
                                                  0 if x.scratch is None else x.scratch.numel(), _ptr(x.arrived),
